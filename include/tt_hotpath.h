@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define TT_ABI_VERSION 4
+#define TT_ABI_VERSION 5
 
 typedef void* tt_stream_t; /* hipStream_t */
 
@@ -673,6 +673,98 @@ const float* tt_engine_last_loss(const tt_engine* e);
  * `stream`.  reset != 0 zeroes the accumulator afterwards. */
 int tt_engine_read_stats(tt_engine* e, double* loss_sum, int64_t* n_batches, float* last_loss,
                          int reset, tt_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Encoder operators and the softmax loss (float, bf16, fp16; fp32 sums)      */
+/* ------------------------------------------------------------------------- */
+
+/* element types of the operators below */
+#define TT_F32 1
+#define TT_BF16 2
+#define TT_F16 3
+
+#define TT_ACT_NONE 0
+#define TT_ACT_RELU 1
+#define TT_ACT_GELU 2      /* z (1 + erf(z / sqrt 2)) / 2 */
+#define TT_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+#define TT_ACT_SILU 4      /* z / (1 + exp(-z)) */
+
+/*
+ * y = act(z) + residual,  z = x w^T + bias: a Linear layer with its activation and the residual add behind it in the
+ * product's epilogue (the nn.Linear calls of the frozen encoder that backend/model.py:51-52 runs).
+ *   x [M,K], w [N,K], residual / y [M,N] of `dtype`, row strides ldx / ldw / ldr / ldy in elements; bias [N]; bias, residual
+ *   and preact may be null.  preact [M,N] (contiguous): z, for tt_linear_act_bwd.  z and the sums are fp32; y and preact are
+ *   rounded once.  Any size and row stride; rows that are not multiples of 16 bytes are copied to the workspace first.
+ *   M == 0 is a no-op.  y may not overlap x or w; y == residual is allowed.
+ */
+size_t tt_linear_act_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K, int dtype);
+int tt_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                  void* y, int64_t ldy, void* preact, int64_t M, int N, int K, int dtype, int act, void* workspace,
+                  size_t workspace_bytes, tt_stream_t stream);
+/*
+ * Gradients of tt_linear_act: dz = dy act'(preact);  dx [M,K] = dz w,  dw [N,K] = dz^T x,  dbias [N] = column sums of dz
+ * (each may be null; all contiguous, of `dtype`).  The residual's gradient is dy itself.  preact may be null for
+ * TT_ACT_NONE.  dz is rounded to `dtype` for the products (dbias is summed before that).  M == 0: dw and dbias are zero.
+ */
+size_t tt_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                         int64_t M, int N, int K, int dtype, int act);
+int tt_linear_act_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* preact,
+                      void* dx, void* dw, void* dbias, int64_t M, int N, int K, int dtype, int act, void* workspace,
+                      size_t workspace_bytes, tt_stream_t stream);
+
+/* one [T, heads, head_dim] operand; strides in elements, head_dim contiguous; 16-byte aligned base and strides */
+typedef struct {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} tt_head_view;
+
+/*
+ * Attention inside documents packed back to back, and its gradients.
+ *   s_ij = softcap * tanh(scale q_i.k_j / softcap)  (softcap > 0; else scale q_i.k_j)  - slopes[h] * |i - j|
+ *   o_i = sum_j softmax_j(s_ij) v_j over the keys j that query i sees: those of its own document whose key_mask byte is not
+ *   zero, and with causal only j <= i, with prefix only j <= i or j < prefix[document] (positions count from the document's
+ *   start).  A query that sees no key gets o = 0, lse = -inf and no gradient.
+ *   Document b holds tokens [cu_seqlens[b], cu_seqlens[b + 1]); cu_seqlens[0] = 0, ascending, at most T; documents may be
+ *   empty.  Tokens behind the last document get o = 0 and zero gradients.  What masked keys hold (NaN included) does not matter.
+ *   heads % kv_heads == 0: query head h reads key head h / (heads / kv_heads).  head_dim: a multiple of 8, 8..128.
+ *   lse [heads, T] fp32: natural logarithm of the softmax's denominator (output of the forward, input of the backward call).
+ *   delta [heads, T] fp32: scratch of the backward call.  Null: slopes, key_mask, prefix where not used.
+ *   dq / dk / dv may be column blocks of one buffer, and may not overlap the inputs.
+ */
+typedef struct {
+  tt_head_view q, k, v, out;
+  tt_head_view dout, dq, dk, dv; /* backward only */
+  float* lse;
+  float* delta;
+  const int32_t* cu_seqlens; /* [docs + 1] */
+  const int32_t* prefix;     /* [docs] or null */
+  const float* slopes;       /* [heads] or null */
+  const uint8_t* key_mask;   /* [T] or null */
+  int64_t T;
+  int32_t docs, heads, kv_heads, head_dim, dtype, causal;
+  float scale, softcap;
+} tt_attention_args;
+int tt_packed_attention(const tt_attention_args* args /* host */, tt_stream_t stream);
+int tt_packed_attention_bwd(const tt_attention_args* args /* host */, tt_stream_t stream);
+
+/*
+ * Softmax cross entropy of each row over V candidates, logits never stored:  l_ij = scale x_i.w_j,
+ *   lse[i] = log sum_j exp l_ij,   loss[i] = lse[i] - l_i,target[i]      (fp32)
+ *   target [N] int64; a row whose target is ignore_index has loss 0 and no gradient, one whose target is otherwise outside
+ *   [0, V) has loss NaN (and poisons the gradients).  row_ids [N] / cand_ids [V] (both or neither): candidates j != target
+ *   with cand_ids[j] == row_ids[i] are left out of row i's sum.
+ * tt_softmax_loss_bwd: row_coef [N] = d objective / d loss[i];  dx [N,D], dw [V,D] contiguous, of `dtype`, either may be null.
+ */
+size_t tt_softmax_loss_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int V, int D, int dtype);
+int tt_softmax_loss(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, const int64_t* row_ids,
+                    const int64_t* cand_ids, int64_t N, int V, int D, int dtype, float scale, int64_t ignore_index, float* loss,
+                    float* lse, void* workspace, size_t workspace_bytes, tt_stream_t stream);
+size_t tt_softmax_loss_bwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int V, int D, int dtype);
+int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target,
+                        const int64_t* row_ids, const int64_t* cand_ids, const float* lse, int64_t N, int V, int D, int dtype,
+                        float scale, int64_t ignore_index, void* dx, void* dw, void* workspace, size_t workspace_bytes,
+                        tt_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -22,7 +22,9 @@ TT_K1_SHARE_AUTO = -1  # tt_engine_config.k1_blocks_per_cu: pair the K1 form wit
 TT_K1_AUTO, TT_K1_PER_TEXT, TT_K1_ROW_SLICES, TT_K1_COLUMN_SLICES, TT_K1_STREAM, TT_K1_BINNED = 0, 1, 2, 3, 4, 5
 K1_FORMS = {"auto": TT_K1_AUTO, "per_text": TT_K1_PER_TEXT, "rows": TT_K1_ROW_SLICES, "columns": TT_K1_COLUMN_SLICES,
             "stream": TT_K1_STREAM, "binned": TT_K1_BINNED}
-ABI_VERSION = 4
+TT_F32, TT_BF16, TT_F16 = 1, 2, 3
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+ABI_VERSION = 5
 
 _lib = None
 _lock = threading.Lock()
@@ -63,6 +65,21 @@ class TTAdamTensor(C.Structure):
 
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
                 ("n", C.c_int64)]
+
+
+class TTHeadView(C.Structure):
+    """tt_head_view: one [T, heads, head_dim] operand of packed attention."""
+
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class TTAttentionArgs(C.Structure):
+    """tt_attention_args (include/tt_hotpath.h)."""
+
+    _fields_ = [(n, TTHeadView) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")] + [
+        ("lse", C.c_void_p), ("delta", C.c_void_p), ("cu_seqlens", C.c_void_p), ("prefix", C.c_void_p), ("slopes", C.c_void_p),
+        ("key_mask", C.c_void_p), ("T", C.c_int64), ("docs", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float)]
 
 
 class TTTuning(C.Structure):
@@ -146,6 +163,16 @@ SIGNATURES = {
     "tt_cosine_scores_workspace_bytes": (_sz, [_i64, _i64, _i]),
     "tt_cosine_scores_f32": (_i, [_vp, _vp, _vp, _i64, _i64, _i, _vp, _sz, _vp]),
     "tt_ndcg_at_k_f32": (_i, [_vp, _vp, _vp, _i64, _i64, C.POINTER(_i32), _i, _vp, _vp, _vp]),
+    "tt_linear_act_workspace_bytes": (_sz, [_vp, _i64, _vp, _i64, _i64, _i, _i, _i]),
+    "tt_linear_act": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "tt_linear_act_bwd_workspace_bytes": (_sz, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _i, _i]),
+    "tt_linear_act_bwd": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "tt_packed_attention": (_i, [C.POINTER(TTAttentionArgs), _vp]),
+    "tt_packed_attention_bwd": (_i, [C.POINTER(TTAttentionArgs), _vp]),
+    "tt_softmax_loss_workspace_bytes": (_sz, [_vp, _i64, _vp, _i64, _i64, _i, _i, _i]),
+    "tt_softmax_loss": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i, _i, _i, _f, _i64, _vp, _vp, _vp, _sz, _vp]),
+    "tt_softmax_loss_bwd_workspace_bytes": (_sz, [_vp, _i64, _vp, _i64, _i64, _i, _i, _i]),
+    "tt_softmax_loss_bwd": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _f, _i64, _vp, _vp, _vp, _sz, _vp]),
     "tt_engine_workspace_bytes": (_sz, [C.POINTER(TTEngineConfig)]),
     "tt_engine_create": (_i, [C.POINTER(TTEngineConfig), _vp, _sz, _vp, C.POINTER(_vp)]),
     "tt_engine_destroy": (_i, [_vp]),

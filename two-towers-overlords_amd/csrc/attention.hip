@@ -1,0 +1,733 @@
+// packed_attention — attention inside documents that are packed back to back, and its gradients.
+//
+//   s_ij = cap tanh(scale q_i.k_j / cap) - slope |i - j|,  p = softmax_j over the keys query i sees,  o_i = sum_j p_ij v_j
+//   sees: same document, key mask set, and "causal" j <= i / "prefix" j <= i or j < prefix[document]
+//
+// One pass over the keys with a running maximum and sum (fp32, base 2); no score leaves the registers.
+//
+// Layout.  A wave owns 32 queries (the accumulator's columns, one per lane & 31) and walks tiles of 128 / sizeof(T) keys.  It
+// forms S^T = K Q^T, so a lane holds scores of ONE query: a row maximum is an in-lane maximum and one exchange with lane ^ 32,
+// and running maximum, sum and rescaling are one register per lane.  O^T = V^T P^T takes P^T straight from the score registers:
+// the K rows are read from LDS in an order (`fold`) that puts eight consecutive keys into a 16-bit lane's fragment (float:
+// four, in place).  V is transposed on its way into LDS.  The backward pass does the same from both sides: one kernel owns
+// queries (dq, and delta = dO.O), one owns keys (dk, dv); each recomputes S.  No atomics: results do not depend on the order.
+//
+// Which document a workgroup works on: document b gets floor(cu[b] / BM) + b as its first tile, which leaves every document
+// at least as many tiles as it has blocks of BM rows; a workgroup finds its document with a 64-wide search in cu.  So the
+// grid follows from T and the number of documents alone, and no length has to be known on the host.  Rows behind the last
+// document form a last "document" that is only zero-filled.
+#include <type_traits>
+#include "mfma_tile.h"
+
+using namespace ttm;
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Args {
+  const void *q, *k, *v, *o, *dout;
+  long long qt, qh, kt, kh, vt, vh, ot, oh, dot, doh;  // element strides per token and head
+  void *out, *dq, *dk, *dv;
+  long long dqt, dqh, dkt, dkh, dvt, dvh;
+  float *lse, *delta;                                   // [H, T]
+  const int *cu, *prefix;
+  const float* slopes;
+  const unsigned char* keep;
+  int T, docs, H, Hkv, Dh, causal;
+  float scale, cap;
+};
+
+struct Where {
+  int doc, start, len, tile;
+  bool tail;
+};
+
+// the document and tile of workgroup slot t (see above); every lane gets the same answer
+__device__ __forceinline__ Where locate(const int* __restrict__ cu, int docs, int T, int t, int bm) {
+  const int lane = threadIdx.x & 63;
+  auto at = [&](int b) { return min(max(cu[b], 0), T); };
+  int lo = 0, cnt = docs + 1;
+  while (cnt > 1) {
+    const int step = (cnt + 63) >> 6, b = lo + lane * step;
+    const bool in = b < lo + cnt;
+    const unsigned long long m = __ballot(in && at(in ? b : lo) / bm + (in ? b : lo) <= t);
+    const int k = m ? 63 - __builtin_clzll(m) : 0;
+    const int end = lo + cnt;
+    lo += k * step;
+    cnt = min(step, end - lo);
+  }
+  Where w;
+  w.doc = __builtin_amdgcn_readfirstlane(lo);
+  w.start = at(w.doc);
+  w.tail = w.doc == docs;
+  const int e = w.tail ? T : max(at(w.doc + 1), w.start);
+  w.len = e - w.start;
+  w.tile = t - (w.start / bm + w.doc);
+  return w;
+}
+
+// row of the K (or Q) image that feeds accumulator row r of a 32-row tile: 16-bit operands swap bits 2 and 3, so that
+// accumulator registers 8 g .. 8 g + 7 of lane half h are rows 16 g + 8 h + [0, 8) — a fragment's order
+template <class T>
+__device__ __forceinline__ int fold(int r) {
+  return sizeof(T) == 2 ? ((r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1)) : r;
+}
+// row (within the 32) that accumulator register i of lane half h holds after fold
+template <class T>
+__device__ __forceinline__ constexpr int row_of(int i, int h) {
+  return sizeof(T) == 2 ? 16 * (i >> 3) + 8 * h + (i & 7) : 8 * (i >> 2) + 4 * h + (i & 3);
+}
+// fragment g of a folded 32-row accumulator, rounded to T (16-bit: 2 fragments of 8; float: 4 of 4)
+template <class T>
+__device__ __forceinline__ u32x4 acc_frag(const f32x16& s, int g) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 v = {s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+    return __builtin_bit_cast(u32x4, v);
+  } else {
+    typedef float f32x8 __attribute__((ext_vector_type(8)));
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    f32x8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = s[8 * g + i];
+    return __builtin_bit_cast(u32x4, __builtin_convertvector(v, t8));
+  }
+}
+
+template <class T, int DP>
+struct Dim {
+  static constexpr int KPF = Type<T>::KPF;
+  static constexpr int TILE = kRowBytes / (int)sizeof(T);     // rows of a tile: 64 (16-bit) or 32 (float)
+  static constexpr int SUB = TILE / 32;                       // accumulator tiles of a tile
+  static constexpr int CH = DP / KPF;                         // 16-byte chunks of a row
+  static constexpr int G = CH / 2;                            // matrix instructions' groups along the head
+  static constexpr int GT = 4;                                // groups along a tile's rows
+  static constexpr int DT = DP / 32;                          // accumulator tiles along the head
+  static constexpr int ROWS = ((CH + 7) / 8) * TILE * kRowBytes;  // bytes of a row image
+  static constexpr int COLS = DP * kRowBytes;                     // bytes of a transposed image
+};
+
+// row image: TILE rows of the head's chunks, 128-byte column blocks
+template <class T, int DP>
+__device__ __forceinline__ u32x4 row_frag(const char* __restrict__ img, int row, int chunk) {
+  return frag(img + (chunk >> 3) * (Dim<T, DP>::TILE * kRowBytes), row, chunk & 7);
+}
+
+// Staging of a tile of rows [r0, r0 + TILE) of one head into a row image and / or a transposed image.  Rows at or behind
+// `end`, and rows the key mask takes out (`keep` non-null), arrive as zeros: 0 * NaN must not reach a sum.
+template <class T, int DP, int NT>
+struct RowStage {
+  using D = Dim<T, DP>;
+  static constexpr int N = (D::TILE * D::CH + NT - 1) / NT;
+  u32x4 c[N];
+  __device__ __forceinline__ void load(const T* __restrict__ p, long long ld, int r0, int end, int Dh, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int f = tid + i * NT, row = f / D::CH, ch = f % D::CH;
+      const bool ok = f < D::TILE * D::CH && r0 + row < end && ch * D::KPF < Dh;
+      c[i] = u32x4{0, 0, 0, 0};
+      if (ok) c[i] = *reinterpret_cast<const u32x4*>(p + (r0 + row) * ld + ch * D::KPF);
+    }
+  }
+  __device__ __forceinline__ void store(char* __restrict__ img, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int f = tid + i * NT, row = f / D::CH, ch = f % D::CH;
+      if (f < D::TILE * D::CH)
+        *reinterpret_cast<u32x4*>(img + (ch >> 3) * (D::TILE * kRowBytes) + swz(row, ch & 7)) = c[i];
+    }
+  }
+};
+template <class T, int DP, int NT>
+struct ColStage {
+  using D = Dim<T, DP>;
+  static constexpr int U = 8 * (DP / 4), N = (U + NT - 1) / NT;  // units of KPF rows x 4 columns
+  KsUnit<T> u[N];
+  __device__ __forceinline__ void load(const T* __restrict__ p, long long ld, int r0, int end, int Dh,
+                                       const unsigned char* __restrict__ keep, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int f = tid + i * NT, kg = f / (DP / 4), cq = f % (DP / 4);
+#pragma unroll
+      for (int j = 0; j < D::KPF; ++j) {
+        using V = decltype(u[i].v[0] + u[i].v[0]);
+        const int row = r0 + kg * D::KPF + j;
+        bool ok = f < U && row < end && 4 * cq < Dh;
+        if (keep && ok) ok = keep[row] != 0;
+        u[i].v[j] = V(0);
+        if (ok) u[i].v[j] = *reinterpret_cast<const V*>(p + row * ld + 4 * cq);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* __restrict__ img, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int f = tid + i * NT, kg = f / (DP / 4), cq = f % (DP / 4);
+      if (f < U) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(img + swz(4 * cq + j, kg)) = u[i].column(j);
+      }
+    }
+  }
+};
+
+// this lane's fragments of ONE row (its column of the accumulator): chunks 2 g + h
+template <class T, int DP>
+__device__ __forceinline__ void load_own(u32x4* __restrict__ f, const T* __restrict__ p, bool ok, int Dh, int h) {
+#pragma unroll
+  for (int g = 0; g < Dim<T, DP>::G; ++g) {
+    const int d = (2 * g + h) * Type<T>::KPF;
+    f[g] = u32x4{0, 0, 0, 0};
+    if (ok && d < Dh) f[g] = *reinterpret_cast<const u32x4*>(p + d);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ float tanh_(float x) {
+  if constexpr (sizeof(T) == 4) return tanhf(x);
+  return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * x));  // +-1 far out
+}
+
+// Scores of one 32x32 tile, in place, from raw products: to units in which p = exp2(s * c - ...) with c = unit(a).  `d` gets
+// d s / d (scale q.k), needed by the backward pass only.  dist0 = (query position) - (position of the tile's row 0) for
+// tiles whose rows are keys; its negative serves tiles whose rows are queries.
+__device__ __forceinline__ float unit(const Args& a) { return (a.cap > 0.f || a.slopes) ? kLog2e : a.scale * kLog2e; }
+template <class T, bool GRAD>
+__device__ __forceinline__ void shape_scores(f32x16& s, f32x16& d, const Args& a, float slope, int dist0, int h) {
+  if (a.cap > 0.f) {
+    const float r = a.scale / a.cap;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float t = tanh_<T>(s[i] * r);
+      s[i] = a.cap * t;
+      if (GRAD) d[i] = fmaf(-t, t, 1.f);
+    }
+  } else if (a.slopes) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= a.scale;
+  }
+  if (a.slopes) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope, fabsf((float)(dist0 - row_of<T>(i, h))), s[i]);
+  }
+}
+
+// number of keys (from the document's start) that some query of [i0, i1) sees, and the first from which masking is needed
+__device__ __forceinline__ int key_end(const Args& a, int prefix, int i1, int len) {
+  if (!a.causal && !a.prefix) return len;
+  return min(len, max(i1, prefix));
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attention_fwd_kernel(Args a, int slots) {
+  using D = Dim<T, DP>;
+  constexpr int NT = 64 * WAVES, BM = 32 * WAVES;
+  __shared__ __align__(16) char kimg[D::ROWS];
+  __shared__ __align__(16) char vimg[D::COLS];
+  const int id = xcd_tile(blockIdx.x, gridDim.x);
+  const int head = id % a.H, slot = id / a.H;
+  const Where w = locate(a.cu, a.docs, a.T, slot, BM);
+  const int i0 = w.tile * BM;
+  if (i0 < 0 || i0 >= w.len) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  const int i = i0 + wave * 32 + r;  // this lane's query, counted in its document
+  const bool live = i < w.len;
+  const long long tok = w.start + i;
+  T* __restrict__ out = static_cast<T*>(a.out) + tok * a.ot + (long long)head * a.oh;
+  if (w.tail) {
+    if (live) {
+      for (int d = h * (DP / 2); d < min(a.Dh, (h + 1) * (DP / 2)); ++d) out[d] = (T)0.f;
+      if (h == 0) a.lse[(long long)head * a.T + tok] = -INFINITY;
+    }
+    return;
+  }
+  const int kvh = head / (a.H / a.Hkv);
+  const T* __restrict__ kp = static_cast<const T*>(a.k) + w.start * a.kt + kvh * a.kh;
+  const T* __restrict__ vp = static_cast<const T*>(a.v) + w.start * a.vt + kvh * a.vh;
+  const unsigned char* __restrict__ keep = a.keep ? a.keep + w.start : nullptr;
+  const int prefix = a.prefix ? min(max(a.prefix[w.doc], 0), w.len) : 0;
+  const bool limited = a.causal || a.prefix;
+  const int kend = key_end(a, prefix, min(i0 + BM, w.len), w.len);
+  const int wend = key_end(a, prefix, min(i0 + wave * 32 + 32, w.len), w.len);  // this wave's own end
+  const int seen = limited ? max(i + 1, prefix) : w.len;                       // this query's
+  const float slope = a.slopes ? a.slopes[head] : 0.f;
+  const float c = unit(a);
+
+  u32x4 qf[D::G];
+  load_own<T, DP>(qf, static_cast<const T*>(a.q) + tok * a.qt + head * a.qh, live, a.Dh, h);
+  f32x16 o[D::DT];
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  RowStage<T, DP, NT> ks;
+  ColStage<T, DP, NT> vs;
+  ks.load(kp, a.kt, 0, w.len, a.Dh, tid);
+  vs.load(vp, a.vt, 0, w.len, a.Dh, keep, tid);
+  for (int k0 = 0; k0 < kend; k0 += D::TILE) {
+    ks.store(kimg, tid);
+    vs.store(vimg, tid);
+    __syncthreads();
+    if (k0 + D::TILE < kend) {
+      ks.load(kp, a.kt, k0 + D::TILE, w.len, a.Dh, tid);
+      vs.load(vp, a.vt, k0 + D::TILE, w.len, a.Dh, keep, tid);
+    }
+    if (k0 < wend && i0 + wave * 32 < w.len) {
+      f32x16 s[D::SUB];
+      const int rem = wend - k0;
+#pragma unroll
+      for (int t = 0; t < D::SUB; ++t) {
+        f32x16 acc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int g = 0; g < D::G; ++g) mma<T>(acc, row_frag<T, DP>(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
+        s[t] = acc;
+      }
+      unsigned long long vis = 0;
+      {
+        const int kk = k0 + lane;
+        bool v = kk < w.len && lane < D::TILE;
+        if (keep && v) v = keep[kk] != 0;
+        vis = __ballot(v);
+      }
+      const unsigned long long all = D::TILE == 64 ? ~0ull : 0xffffffffull;
+      const bool masked = vis != all || (limited && k0 + D::TILE > i0 + wave * 32 && k0 + D::TILE > prefix);
+      float mx = m;
+#pragma unroll
+      for (int t = 0; t < D::SUB; ++t) {
+        f32x16 unused;
+        shape_scores<T, false>(s[t], unused, a, slope, i - (k0 + 32 * t), h);
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int kk = 32 * t + row_of<T>(e, h);
+            if (!((vis >> kk) & 1) || k0 + kk >= seen) s[t][e] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mc = mx == -INFINITY ? 0.f : mx * c;
+      if (__any(mx > m)) {
+        const float f = __builtin_amdgcn_exp2f(fmaf(m, c, -mc));
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[t][e] *= f;
+        m = mx;
+      }
+#pragma unroll
+      for (int t = 0; t < D::SUB; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -mc));
+          l += s[t][e];
+        }
+#pragma unroll
+      for (int g = 0; g < D::GT; ++g) {
+        constexpr int PER = D::GT / D::SUB;
+        if (32 * (g / PER) >= rem) break;  // uniform: the second half of a tile behind the last key
+        const u32x4 pf = acc_frag<T>(s[g / PER], g % PER);
+#pragma unroll
+        for (int t = 0; t < D::DT; ++t) mma<T>(o[t], frag(vimg, 32 * t + r, 2 * g + h), pf);
+      }
+    }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!live) return;
+  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * t + 8 * q + 4 * h;
+      const f32x4 v = {o[t][4 * q] * inv, o[t][4 * q + 1] * inv, o[t][4 * q + 2] * inv, o[t][4 * q + 3] * inv};
+      if (d < a.Dh) *reinterpret_cast<typename Type<T>::quad*>(out + d) = to_quad<T>(v);
+    }
+  if (h == 0) a.lse[(long long)head * a.T + tok] = l == 0.f ? -INFINITY : (m * c + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ------------------------------------------------------------------------------------------------ dq, delta
+// dS = P (dO V^T - delta) d,  dq_i = scale sum_j dS_ij k_j,  delta_i = dO_i . o_i
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attention_dq_kernel(Args a, int slots) {
+  using D = Dim<T, DP>;
+  constexpr int NT = 64 * WAVES, BM = 32 * WAVES;
+  __shared__ __align__(16) char kimg[D::ROWS];
+  __shared__ __align__(16) char vimg[D::ROWS];
+  __shared__ __align__(16) char ktim[D::COLS];
+  const int id = xcd_tile(blockIdx.x, gridDim.x);
+  const int head = id % a.H, slot = id / a.H;
+  const Where w = locate(a.cu, a.docs, a.T, slot, BM);
+  const int i0 = w.tile * BM;
+  if (i0 < 0 || i0 >= w.len) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  const int i = i0 + wave * 32 + r;
+  const bool live = i < w.len;
+  const long long tok = w.start + i;
+  T* __restrict__ dq = static_cast<T*>(a.dq) + tok * a.dqt + (long long)head * a.dqh;
+  if (w.tail) {
+    if (live)
+      for (int d = h * (DP / 2); d < min(a.Dh, (h + 1) * (DP / 2)); ++d) dq[d] = (T)0.f;
+    return;
+  }
+  const int kvh = head / (a.H / a.Hkv);
+  const T* __restrict__ kp = static_cast<const T*>(a.k) + w.start * a.kt + kvh * a.kh;
+  const T* __restrict__ vp = static_cast<const T*>(a.v) + w.start * a.vt + kvh * a.vh;
+  const unsigned char* __restrict__ keep = a.keep ? a.keep + w.start : nullptr;
+  const int prefix = a.prefix ? min(max(a.prefix[w.doc], 0), w.len) : 0;
+  const bool limited = a.causal || a.prefix;
+  const int kend = key_end(a, prefix, min(i0 + BM, w.len), w.len);
+  const int wend = key_end(a, prefix, min(i0 + wave * 32 + 32, w.len), w.len);
+  const int seen = limited ? max(i + 1, prefix) : w.len;
+  const float slope = a.slopes ? a.slopes[head] : 0.f;
+  const float c = unit(a);
+
+  u32x4 qf[D::G], df[D::G];
+  load_own<T, DP>(qf, static_cast<const T*>(a.q) + tok * a.qt + head * a.qh, live, a.Dh, h);
+  load_own<T, DP>(df, static_cast<const T*>(a.dout) + tok * a.dot + head * a.doh, live, a.Dh, h);
+  float delta = 0.f, lse2 = INFINITY;  // an infinite normaliser: p = 0
+  {
+    u32x4 of[D::G];
+    load_own<T, DP>(of, static_cast<const T*>(a.o) + tok * a.ot + head * a.oh, live, a.Dh, h);
+    typedef T tv __attribute__((ext_vector_type(Type<T>::KPF)));
+#pragma unroll
+    for (int g = 0; g < D::G; ++g) {
+      const tv x = __builtin_bit_cast(tv, of[g]), y = __builtin_bit_cast(tv, df[g]);
+#pragma unroll
+      for (int e = 0; e < Type<T>::KPF; ++e) delta = fmaf((float)x[e], (float)y[e], delta);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (live) {
+      const float t = a.lse[(long long)head * a.T + tok];
+      if (t != -INFINITY) lse2 = t * kLog2e;
+      if (h == 0) a.delta[(long long)head * a.T + tok] = delta;
+    }
+  }
+  f32x16 acc[D::DT];
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+
+  RowStage<T, DP, NT> ks, vs;
+  ColStage<T, DP, NT> kc;
+  ks.load(kp, a.kt, 0, w.len, a.Dh, tid);
+  vs.load(vp, a.vt, 0, w.len, a.Dh, tid);
+  kc.load(kp, a.kt, 0, w.len, a.Dh, keep, tid);
+  for (int k0 = 0; k0 < kend; k0 += D::TILE) {
+    ks.store(kimg, tid);
+    vs.store(vimg, tid);
+    kc.store(ktim, tid);
+    __syncthreads();
+    if (k0 + D::TILE < kend) {
+      ks.load(kp, a.kt, k0 + D::TILE, w.len, a.Dh, tid);
+      vs.load(vp, a.vt, k0 + D::TILE, w.len, a.Dh, tid);
+      kc.load(kp, a.kt, k0 + D::TILE, w.len, a.Dh, keep, tid);
+    }
+    if (k0 < wend && i0 + wave * 32 < w.len) {
+      const int kk0 = k0 + lane;
+      bool v = kk0 < w.len && lane < D::TILE;
+      if (keep && v) v = keep[kk0] != 0;
+      const unsigned long long vis = __ballot(v);
+      const unsigned long long all = D::TILE == 64 ? ~0ull : 0xffffffffull;
+      const bool masked = vis != all || (limited && k0 + D::TILE > i0 + wave * 32 && k0 + D::TILE > prefix);
+      const int rem = wend - k0;
+#pragma unroll
+      for (int t = 0; t < D::SUB; ++t) {
+        if (32 * t >= rem) break;
+        f32x16 s, dp, d;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+        for (int g = 0; g < D::G; ++g) {
+          mma<T>(s, row_frag<T, DP>(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
+          mma<T>(dp, row_frag<T, DP>(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
+        }
+        shape_scores<T, true>(s, d, a, slope, i - (k0 + 32 * t), h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse2));
+          float ds = p * (dp[e] - delta);
+          if (a.cap > 0.f) ds *= d[e];
+          s[e] = ds;
+        }
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int kk = 32 * t + row_of<T>(e, h);
+            if (!((vis >> kk) & 1) || k0 + kk >= seen) s[e] = 0.f;
+          }
+        }
+        constexpr int PER = D::GT / D::SUB;
+#pragma unroll
+        for (int g = 0; g < PER; ++g) {
+          const u32x4 f = acc_frag<T>(s, g);
+#pragma unroll
+          for (int u = 0; u < D::DT; ++u) mma<T>(acc[u], frag(ktim, 32 * u + r, 2 * (t * PER + g) + h), f);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (!live) return;
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * t + 8 * q + 4 * h;
+      const f32x4 v = {acc[t][4 * q], acc[t][4 * q + 1], acc[t][4 * q + 2], acc[t][4 * q + 3]};
+      if (d < a.Dh) *reinterpret_cast<typename Type<T>::quad*>(dq + d) = to_quad<T>(v * a.scale);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ dk, dv
+// A wave owns 32 keys (columns) and walks the queries, for every query head that shares the key head:
+// dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attention_dkv_kernel(Args a, int slots) {
+  using D = Dim<T, DP>;
+  constexpr int NT = 64 * WAVES, BM = 32 * WAVES;
+  __shared__ __align__(16) char qimg[D::ROWS];
+  __shared__ __align__(16) char dimg[D::ROWS];
+  __shared__ __align__(16) char qtim[D::COLS];
+  __shared__ __align__(16) char dtim[D::COLS];
+  __shared__ __align__(16) float stat[2][D::TILE];
+  const int id = xcd_tile(blockIdx.x, gridDim.x);
+  const int kvh = id % a.Hkv, slot = id / a.Hkv;
+  const Where w = locate(a.cu, a.docs, a.T, slot, BM);
+  const int j0 = w.tile * BM;
+  if (j0 < 0 || j0 >= w.len) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  const int j = j0 + wave * 32 + r;  // this lane's key
+  const bool in = j < w.len;
+  const long long tok = w.start + j;
+  T* __restrict__ dk = static_cast<T*>(a.dk) + tok * a.dkt + (long long)kvh * a.dkh;
+  T* __restrict__ dv = static_cast<T*>(a.dv) + tok * a.dvt + (long long)kvh * a.dvh;
+  if (w.tail) {
+    if (in)
+      for (int d = h * (DP / 2); d < min(a.Dh, (h + 1) * (DP / 2)); ++d) dk[d] = dv[d] = (T)0.f;
+    return;
+  }
+  const bool live = in && (!a.keep || a.keep[tok] != 0);
+  const int rep = a.H / a.Hkv;
+  const int prefix = a.prefix ? min(max(a.prefix[w.doc], 0), w.len) : 0;
+  const bool limited = a.causal || a.prefix;
+  // queries from `first` on see this key; the workgroup starts at its own earliest
+  const int first = !limited || j < prefix ? 0 : j;
+  const int wfirst = !limited || j0 + wave * 32 < prefix ? 0 : j0 + wave * 32;
+  const int bfirst = (!limited || j0 < prefix ? 0 : j0) / D::TILE * D::TILE;
+  const float c = unit(a);
+
+  u32x4 kf[D::G], vf[D::G];
+  load_own<T, DP>(kf, static_cast<const T*>(a.k) + tok * a.kt + kvh * a.kh, live, a.Dh, h);
+  load_own<T, DP>(vf, static_cast<const T*>(a.v) + tok * a.vt + kvh * a.vh, live, a.Dh, h);
+  f32x16 ak[D::DT], av[D::DT];
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ak[t][e] = av[t][e] = 0.f;
+
+  for (int hq = 0; hq < rep; ++hq) {
+    const int head = kvh * rep + hq;
+    const T* __restrict__ qp = static_cast<const T*>(a.q) + w.start * a.qt + head * a.qh;
+    const T* __restrict__ dp_ = static_cast<const T*>(a.dout) + w.start * a.dot + head * a.doh;
+    const float* __restrict__ lse = a.lse + (long long)head * a.T + w.start;
+    const float* __restrict__ del = a.delta + (long long)head * a.T + w.start;
+    const float slope = a.slopes ? a.slopes[head] : 0.f;
+    for (int q0 = bfirst; q0 < w.len; q0 += D::TILE) {
+      {
+        RowStage<T, DP, NT> s;
+        s.load(qp, a.qt, q0, w.len, a.Dh, tid);
+        s.store(qimg, tid);
+        s.load(dp_, a.dot, q0, w.len, a.Dh, tid);
+        s.store(dimg, tid);
+      }
+      {
+        ColStage<T, DP, NT> s;
+        s.load(qp, a.qt, q0, w.len, a.Dh, nullptr, tid);
+        s.store(qtim, tid);
+        s.load(dp_, a.dot, q0, w.len, a.Dh, nullptr, tid);
+        s.store(dtim, tid);
+      }
+      if (tid < D::TILE) {
+        const float t = q0 + tid < w.len ? lse[q0 + tid] : -INFINITY;
+        stat[0][tid] = t == -INFINITY ? INFINITY : t * kLog2e;  // a row that sees nothing, or none: p = 0
+        stat[1][tid] = q0 + tid < w.len ? del[q0 + tid] : 0.f;
+      }
+      __syncthreads();
+      if (q0 + D::TILE > wfirst && j0 + wave * 32 < w.len) {
+        const bool masked = limited && q0 < j0 + wave * 32 + 31 && j0 + wave * 32 + 31 >= prefix;
+#pragma unroll
+        for (int t = 0; t < D::SUB; ++t) {
+          if (q0 + 32 * t >= w.len) break;
+          f32x16 s, dp, d;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+          for (int g = 0; g < D::G; ++g) {
+            mma<T>(s, row_frag<T, DP>(qimg, 32 * t + fold<T>(r), 2 * g + h), kf[g]);
+            mma<T>(dp, row_frag<T, DP>(dimg, 32 * t + fold<T>(r), 2 * g + h), vf[g]);
+          }
+          shape_scores<T, true>(s, d, a, slope, j - (q0 + 32 * t), h);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int qq = 32 * t + row_of<T>(e, h);
+            float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, -stat[0][qq]));
+            if (masked && q0 + qq < first) p = 0.f;
+            float ds = p * (dp[e] - stat[1][qq]);
+            if (a.cap > 0.f) ds *= d[e];
+            s[e] = p;
+            dp[e] = ds;
+          }
+          constexpr int PER = D::GT / D::SUB;
+#pragma unroll
+          for (int g = 0; g < PER; ++g) {
+            const u32x4 pf = acc_frag<T>(s, g), sf = acc_frag<T>(dp, g);
+#pragma unroll
+            for (int u = 0; u < D::DT; ++u) {
+              mma<T>(av[u], frag(dtim, 32 * u + r, 2 * (t * PER + g) + h), pf);
+              mma<T>(ak[u], frag(qtim, 32 * u + r, 2 * (t * PER + g) + h), sf);
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+  if (!in) return;
+#pragma unroll
+  for (int t = 0; t < D::DT; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * t + 8 * q + 4 * h;
+      f32x4 x = {ak[t][4 * q], ak[t][4 * q + 1], ak[t][4 * q + 2], ak[t][4 * q + 3]};
+      f32x4 y = {av[t][4 * q], av[t][4 * q + 1], av[t][4 * q + 2], av[t][4 * q + 3]};
+      x *= a.scale;
+      if (!live) x = y = f32x4{0.f, 0.f, 0.f, 0.f};  // a key nobody sees
+      if (d < a.Dh) {
+        *reinterpret_cast<typename Type<T>::quad*>(dk + d) = to_quad<T>(x);
+        *reinterpret_cast<typename Type<T>::quad*>(dv + d) = to_quad<T>(y);
+      }
+    }
+}
+
+template <class T, int DP>
+int launch_fwd(const Args& a, int waves, hipStream_t st) {
+  const long long slots = (long long)a.T / (32 * waves) + a.docs + 1, grid = slots * a.H;
+  TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
+  if (waves == 4) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, 4>), dim3((unsigned)grid), dim3(256), 0, st, a, (int)slots);
+  else hipLaunchKernelGGL((attention_fwd_kernel<T, DP, 2>), dim3((unsigned)grid), dim3(128), 0, st, a, (int)slots);
+  TT_CHECK_LAUNCH();
+  return TT_OK;
+}
+template <class T, int DP>
+int launch_bwd(const Args& a, int waves, hipStream_t st) {
+  const long long slots = (long long)a.T / (32 * waves) + a.docs + 1;
+  TT_REQUIRE(slots * a.H <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
+  const dim3 gq((unsigned)(slots * a.H)), gk((unsigned)(slots * a.Hkv));
+  if (waves == 4) {
+    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 4>), gq, dim3(256), 0, st, a, (int)slots);
+    TT_CHECK_LAUNCH();
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 4>), gk, dim3(256), 0, st, a, (int)slots);
+  } else {
+    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 2>), gq, dim3(128), 0, st, a, (int)slots);
+    TT_CHECK_LAUNCH();
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 2>), gk, dim3(128), 0, st, a, (int)slots);
+  }
+  TT_CHECK_LAUNCH();
+  return TT_OK;
+}
+
+// workgroups of 128 rows where the documents are long enough to fill them, of 64 rows for short ones
+int pick_waves(long long T, int docs) { return T >= 128LL * docs ? 4 : 2; }
+
+template <class F>
+int with_shape(int dtype, int Dh, F&& f) {
+  auto dim = [&](auto t) {
+    if (Dh <= 32) return f(t, std::integral_constant<int, 32>{});
+    if (Dh <= 64) return f(t, std::integral_constant<int, 64>{});
+    return f(t, std::integral_constant<int, 128>{});
+  };
+  switch (dtype) {
+    case TT_F32: return dim(float{});
+    case TT_BF16: return dim(__bf16{});
+    case TT_F16: return dim(_Float16{});
+    default: return (int)TT_ERR_BAD_DTYPE;
+  }
+}
+
+bool view_ok(const tt_head_view& v, int width, bool required) {
+  if (!v.data) return !required;
+  const int kpf = 16 / width;
+  return tt_aligned16(v.data) && v.token_stride % kpf == 0 && v.head_stride % kpf == 0;
+}
+
+int check(const tt_attention_args* p) {
+  TT_REQUIRE(p, TT_ERR_NULL_POINTER);
+  TT_REQUIRE(p->dtype == TT_F32 || p->dtype == TT_BF16 || p->dtype == TT_F16, TT_ERR_BAD_DTYPE);
+  TT_REQUIRE(p->T >= 0 && p->T <= 0x7fffffffLL - 1024 && p->docs >= 1 && p->heads >= 1 && p->kv_heads >= 1 &&
+                 p->heads % p->kv_heads == 0 && p->head_dim >= 8 && p->head_dim <= 128 && p->head_dim % 8 == 0,
+             TT_ERR_BAD_SHAPE);
+  TT_REQUIRE(p->scale > 0.f && p->softcap >= 0.f, TT_ERR_BAD_SHAPE);
+  TT_REQUIRE(!(p->causal && p->prefix), TT_ERR_UNSUPPORTED);
+  return TT_OK;
+}
+Args make_args(const tt_attention_args* p) {
+  Args a{};
+  a.q = p->q.data; a.qt = p->q.token_stride; a.qh = p->q.head_stride;
+  a.k = p->k.data; a.kt = p->k.token_stride; a.kh = p->k.head_stride;
+  a.v = p->v.data; a.vt = p->v.token_stride; a.vh = p->v.head_stride;
+  a.o = a.out = p->out.data; a.ot = p->out.token_stride; a.oh = p->out.head_stride;
+  a.dout = p->dout.data; a.dot = p->dout.token_stride; a.doh = p->dout.head_stride;
+  a.dq = p->dq.data; a.dqt = p->dq.token_stride; a.dqh = p->dq.head_stride;
+  a.dk = p->dk.data; a.dkt = p->dk.token_stride; a.dkh = p->dk.head_stride;
+  a.dv = p->dv.data; a.dvt = p->dv.token_stride; a.dvh = p->dv.head_stride;
+  a.lse = p->lse; a.delta = p->delta; a.cu = p->cu_seqlens; a.prefix = p->prefix; a.slopes = p->slopes; a.keep = p->key_mask;
+  a.T = (int)p->T; a.docs = p->docs; a.H = p->heads; a.Hkv = p->kv_heads; a.Dh = p->head_dim; a.causal = p->causal;
+  a.scale = p->scale; a.cap = p->softcap;
+  return a;
+}
+
+}  // namespace
+
+extern "C" int tt_packed_attention(const tt_attention_args* p, tt_stream_t stream) {
+  int rc = check(p);
+  if (rc != TT_OK) return rc;
+  if (p->T == 0) return TT_OK;
+  TT_REQUIRE(p->q.data && p->k.data && p->v.data && p->out.data && p->lse && p->cu_seqlens, TT_ERR_NULL_POINTER);
+  const int width = dtype_bytes(p->dtype);
+  TT_REQUIRE(view_ok(p->q, width, true) && view_ok(p->k, width, true) && view_ok(p->v, width, true) && view_ok(p->out, width, true),
+             TT_ERR_ALIGNMENT);
+  const Args a = make_args(p);
+  const int waves = pick_waves(p->T, p->docs);
+  return with_shape(p->dtype, p->head_dim, [&](auto t, auto dp) {
+    return launch_fwd<decltype(t), decltype(dp)::value>(a, waves, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int tt_packed_attention_bwd(const tt_attention_args* p, tt_stream_t stream) {
+  int rc = check(p);
+  if (rc != TT_OK) return rc;
+  if (p->T == 0) return TT_OK;
+  TT_REQUIRE(p->q.data && p->k.data && p->v.data && p->out.data && p->dout.data && p->dq.data && p->dk.data && p->dv.data && p->lse &&
+                 p->delta && p->cu_seqlens,
+             TT_ERR_NULL_POINTER);
+  const int width = dtype_bytes(p->dtype);
+  TT_REQUIRE(view_ok(p->q, width, true) && view_ok(p->k, width, true) && view_ok(p->v, width, true) &&
+                 view_ok(p->out, width, true) && view_ok(p->dout, width, true) && view_ok(p->dq, width, true) &&
+                 view_ok(p->dk, width, true) && view_ok(p->dv, width, true),
+             TT_ERR_ALIGNMENT);
+  const Args a = make_args(p);
+  const int waves = pick_waves(p->T, p->docs);
+  return with_shape(p->dtype, p->head_dim, [&](auto t, auto dp) {
+    return launch_bwd<decltype(t), decltype(dp)::value>(a, waves, static_cast<hipStream_t>(stream));
+  });
+}

@@ -1,0 +1,459 @@
+// linear_act — y = act(x W^T + b) + r with one epilogue, and its gradients.
+//
+//   forward   z = x W^T + b (fp32), y = act(z) + r rounded once; z is kept (rounded to the type) for the backward pass
+//   backward  dz = dy act'(z), db = column sums of dz       one pass over dy and z
+//             dx = dz W                                     K-strided W, transposed on its way into LDS
+//             dW = dz^T x                                   both operands K-strided, contraction over the rows split
+//
+// Replaces the nn.Linear (+ activation, + residual add) calls of the frozen encoder of backend/model.py:51-52.
+#include "mfma_tile.h"
+
+using namespace ttm;
+
+namespace {
+
+constexpr float kRsqrt2 = 0.70710678118654752f, kRsqrt2Pi = 0.39894228040143268f;
+constexpr float kGeluC = 0.79788456080286536f, kGeluA = 0.044715f;
+
+// erf.  16-bit results: Abramowitz & Stegun 7.1.26, |error| <= 1.5e-7 — 2^-14 of a bf16 step of 1.
+template <bool FAST>
+__device__ __forceinline__ float erf_(float x) {
+  if constexpr (!FAST) return erff(x);
+  const float a = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * a * a);
+  return copysignf(fmaf(-p, e, 1.f), x);
+}
+template <bool FAST>
+__device__ __forceinline__ float exp_(float x) {
+  return FAST ? __builtin_amdgcn_exp2f(1.4426950408889634f * x) : expf(x);
+}
+template <bool FAST>
+__device__ __forceinline__ float inv_(float x) {
+  return FAST ? __builtin_amdgcn_rcpf(x) : 1.f / x;
+}
+
+template <int ACT, bool FAST>
+__device__ __forceinline__ float act_(float z) {
+  if constexpr (ACT == TT_ACT_RELU) return z < 0.f ? 0.f : z;
+  if constexpr (ACT == TT_ACT_GELU) return 0.5f * z * (1.f + erf_<FAST>(z * kRsqrt2));
+  if constexpr (ACT == TT_ACT_GELU_TANH) {  // z / (1 + exp(-2u)) = 0.5 z (1 + tanh u)
+    const float u = kGeluC * z * fmaf(kGeluA * z, z, 1.f);
+    return z * inv_<FAST>(1.f + exp_<FAST>(-2.f * u));
+  }
+  if constexpr (ACT == TT_ACT_SILU) return z * inv_<FAST>(1.f + exp_<FAST>(-z));
+  return z;
+}
+// act'(z).  Far out the derivatives are their limits 0 and 1, where z times an exponential could be inf * 0; NaN stays NaN.
+template <int ACT, bool FAST>
+__device__ __forceinline__ float dact_(float z) {
+  if constexpr (ACT == TT_ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
+  if constexpr (ACT == TT_ACT_NONE) return 1.f;
+  z = z > 40.f ? 40.f : (z < -40.f ? -40.f : z);
+  if constexpr (ACT == TT_ACT_GELU)
+    return fmaf(z * kRsqrt2Pi, exp_<FAST>(-0.5f * z * z), 0.5f * (1.f + erf_<FAST>(z * kRsqrt2)));
+  if constexpr (ACT == TT_ACT_GELU_TANH) {
+    const float u = kGeluC * z * fmaf(kGeluA * z, z, 1.f);
+    const float s = inv_<FAST>(1.f + exp_<FAST>(-2.f * u));  // (1 + tanh u) / 2;  1 - tanh^2 = 4 s (1 - s)
+    return s + z * 2.f * s * (1.f - s) * kGeluC * fmaf(3.f * kGeluA * z, z, 1.f);
+  }
+  const float s = inv_<FAST>(1.f + exp_<FAST>(-z));
+  return s * fmaf(z, 1.f - s, 1.f);
+}
+
+template <class F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  switch (act) {  // uniform
+    case TT_ACT_RELU: f(std::integral_constant<int, TT_ACT_RELU>{}); break;
+    case TT_ACT_GELU: f(std::integral_constant<int, TT_ACT_GELU>{}); break;
+    case TT_ACT_GELU_TANH: f(std::integral_constant<int, TT_ACT_GELU_TANH>{}); break;
+    case TT_ACT_SILU: f(std::integral_constant<int, TT_ACT_SILU>{}); break;
+    default: f(std::integral_constant<int, TT_ACT_NONE>{}); break;
+  }
+}
+
+struct FwdArgs {
+  Operand X, W;
+  Shape s;
+  const void *bias, *res;
+  void *y, *z;
+  long long ldr, ldy;
+  int act, vec, gn;  // gn: tiles along N
+};
+
+template <class T, int BM, int BN>
+__global__ __launch_bounds__(256) void linear_fwd_kernel(FwdArgs a) {
+  __shared__ __align__(16) char lds[2 * (BM + BN) * kRowBytes];
+  const int t = xcd_tile(blockIdx.x, gridDim.x);
+  const int m0 = t / a.gn * BM, n0 = t % a.gn * BN;
+  f32x16 acc[BN / 64][BM / 64];
+  tile_product<T, false, false, BM, BN>(acc, lds, a.X, a.W, a.s, m0, n0, 0, a.s.K);
+  const T* __restrict__ bias = static_cast<const T*>(a.bias);
+  const T* __restrict__ res = static_cast<const T*>(a.res);
+  T* __restrict__ y = static_cast<T*>(a.y);
+  T* __restrict__ z = static_cast<T*>(a.z);
+  const int M = a.s.M, N = a.s.N;
+  const bool vec = a.vec;
+  with_act(a.act, [&](auto tag) {
+    constexpr int ACT = decltype(tag)::value;
+    for_quads<BM, BN>(acc, m0, n0, [&](int m, int n, f32x4 v) {
+      if (m >= M) return;
+      if (bias) v += load_quad<T>(bias, 0, 0, n, N, vec);
+      if (z) {
+        f32x4 k = v;
+        if constexpr (ACT == TT_ACT_RELU && __is_same(T, _Float16)) {
+          // a positive z below fp16's range must not be kept as 0: relu'(z) is 1 there
+#pragma unroll
+          for (int c = 0; c < 4; ++c) k[c] = v[c] > 0.f ? fmaxf(v[c], 5.9604645e-8f) : v[c];
+        }
+        store_quad<T>(z, N, m, n, N, vec, k);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = act_<ACT, sizeof(T) == 2>(v[c]);
+      if (res) v += load_quad<T>(res, a.ldr, m, n, N, vec);
+      store_quad<T>(y, a.ldy, m, n, N, vec, v);
+    });
+  });
+}
+
+// dz = dy act'(z) (written when dz != null, row stride ldz) and, per block of rows, the column sums of dz.
+// 256 threads = 64 quads of columns x 4 rows; grid (ceil(N / 256), row blocks).
+struct DzArgs {
+  const void *dy, *z;
+  void* dz;
+  float* part;  // [gridDim.y, N] or null
+  long long lddy, ldz;
+  int M, N, rows, act, vec;
+};
+template <class T>
+__global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
+  __shared__ f32x4 red[4][64];
+  const int q = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int n = (blockIdx.x * 64 + q) * 4;
+  const int m1 = min(a.M, (int)(blockIdx.y + 1) * a.rows);
+  const T* __restrict__ dy = static_cast<const T*>(a.dy);
+  const T* __restrict__ z = static_cast<const T*>(a.z);
+  T* __restrict__ dz = static_cast<T*>(a.dz);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  const bool vec = a.vec;
+  if (n < a.N) {
+    with_act(a.act, [&](auto tag) {
+      constexpr int ACT = decltype(tag)::value;
+      for (int m = blockIdx.y * a.rows + w; m < m1; m += 4) {
+        f32x4 v = load_quad<T>(dy, a.lddy, m, n, a.N, vec);
+        if constexpr (ACT != TT_ACT_NONE) {
+          const f32x4 zz = load_quad<T>(z, a.N, m, n, a.N, vec);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] *= dact_<ACT, sizeof(T) == 2>(zz[c]);
+        }
+        if (dz) *reinterpret_cast<typename Type<T>::quad*>(dz + m * a.ldz + n) = to_quad<T>(v);  // ldz covers whole quads
+        sum += v;
+      }
+    });
+  }
+  if (!a.part) return;
+  red[w][q] = sum;
+  __syncthreads();
+  if (w == 0 && n < a.N) {
+    const f32x4 s = (red[0][q] + red[1][q]) + (red[2][q] + red[3][q]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (n + c < a.N) a.part[(long long)blockIdx.y * a.N + n + c] = s[c];
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void slab_sum_kernel(const float* __restrict__ slab, int ns, long long n, T* __restrict__ out,
+                                                       float alpha, const float* __restrict__ alpha_dev) {
+  if (alpha_dev) alpha *= *alpha_dev;
+  const long long stride = (long long)gridDim.x * 256;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    float v = 0.f;
+    for (int z = 0; z < ns; ++z) v += slab[z * n + i];
+    out[i] = (T)(v * alpha);
+  }
+}
+
+__global__ __launch_bounds__(256) void pack_kernel(const char* __restrict__ src, long long ld, char* __restrict__ dst, long long ldp,
+                                                   long long rows, long long cols, int width) {
+  const long long n = rows * ldp, stride = (long long)gridDim.x * 256;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    const long long r = i / ldp, c = i - r * ldp;
+    if (width == 4)
+      reinterpret_cast<float*>(dst)[i] = c < cols ? reinterpret_cast<const float*>(src)[r * ld + c] : 0.f;
+    else
+      reinterpret_cast<uint16_t*>(dst)[i] = c < cols ? reinterpret_cast<const uint16_t*>(src)[r * ld + c] : (uint16_t)0;
+  }
+}
+
+struct GradArgs {
+  GradProduct g;
+  Shape s;
+  int gm, gn, vec;
+};
+template <class T, bool XKS, int BM, int BN>
+__global__ __launch_bounds__(256) void grad_product_kernel(GradArgs a) {
+  __shared__ __align__(16) char lds[2 * (BM + BN) * kRowBytes];
+  const int tiles = a.gm * a.gn;
+  const int id = xcd_tile(blockIdx.x, gridDim.x);
+  const int z = id / tiles, t = id - z * tiles;
+  const int m0 = t / a.gn * BM, n0 = t % a.gn * BN;
+  f32x16 acc[BN / 64][BM / 64];
+  const int kbeg = z * a.s.kper;
+  tile_product<T, XKS, true, BM, BN>(acc, lds, a.g.X, a.g.Y, a.s, m0, n0, kbeg, min(a.s.K, kbeg + a.s.kper));
+  const int M = a.s.M, N = a.s.N;
+  const bool vec = a.vec;
+  if (a.g.slab) {
+    float* __restrict__ c = a.g.slab + (long long)z * M * N;
+    const bool more = a.g.accumulate;
+    for_quads<BM, BN>(acc, m0, n0, [&](int m, int n, f32x4 v) {
+      if (m >= M) return;
+      if (more) v += load_quad<float>(c, N, m, n, N, vec);
+      store_quad<float>(c, N, m, n, N, vec, v);
+    });
+  } else {
+    T* __restrict__ c = static_cast<T*>(a.g.out);
+    const float alpha = a.g.alpha_dev ? a.g.alpha * *a.g.alpha_dev : a.g.alpha;
+    const long long ldo = a.g.ldo;
+    for_quads<BM, BN>(acc, m0, n0, [&](int m, int n, f32x4 v) {
+      if (m < M) store_quad<T>(c, ldo, m, n, N, vec, v * alpha);
+    });
+  }
+}
+
+// 128x128 tiles once they fill the chip, else 64x64
+bool big_tiles(long long M, long long N, long long splits) { return ((M + 127) / 128) * ((N + 127) / 128) * splits >= 256; }
+
+template <class F>
+int with_type(int dtype, F&& f) {
+  switch (dtype) {
+    case TT_F32: return f(float{});
+    case TT_BF16: return f(__bf16{});
+    case TT_F16: return f(_Float16{});
+    default: return TT_ERR_BAD_DTYPE;
+  }
+}
+bool known_dtype(int d) { return d == TT_F32 || d == TT_BF16 || d == TT_F16; }
+bool quad_ok(const void* p, long long ld, int width) { return !p || ((reinterpret_cast<uintptr_t>(p) % (4 * width)) == 0 && ld % 4 == 0); }
+
+}  // namespace
+
+int tt_launch_pack(const void* src, long long ld, void* dst, long long ldp, long long rows, long long cols, int width, hipStream_t st) {
+  const long long n = rows * ldp;
+  if (n == 0) return TT_OK;
+  const unsigned g = (unsigned)(n / 1024 + 1 < 8192 ? n / 1024 + 1 : 8192);
+  hipLaunchKernelGGL(pack_kernel, dim3(g), dim3(256), 0, st, (const char*)src, ld, (char*)dst, ldp, rows, cols, width);
+  TT_CHECK_LAUNCH();
+  return TT_OK;
+}
+
+int tt_launch_slab_sum(const float* slab, int ns, long long n, void* out, int dtype, float alpha, const float* alpha_dev, hipStream_t st) {
+  if (n == 0) return TT_OK;
+  const unsigned g = (unsigned)(n / 256 + 1 < 4096 ? n / 256 + 1 : 4096);
+  return with_type(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    hipLaunchKernelGGL(slab_sum_kernel<T>, dim3(g), dim3(256), 0, st, slab, ns, n, (T*)out, alpha, alpha_dev);
+    TT_CHECK_LAUNCH();
+    return (int)TT_OK;
+  });
+}
+
+int tt_grad_splits(long long M, long long N, long long K) {
+  const long long tiles = ((M + 127) / 128) * ((N + 127) / 128);
+  long long s = (512 + tiles - 1) / tiles;        // two workgroups per compute unit
+  if (s > K / 512) s = K / 512;                   // at least eight 16-bit K-steps each
+  if (s > 32) s = 32;
+  return s < 1 ? 1 : (int)s;
+}
+
+int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
+  GradArgs a{};
+  a.g = g;
+  const int bk = kRowBytes / dtype_bytes(dtype);
+  a.s = Shape{g.M, g.N, g.K, (int)(pad_to((g.K + g.nsplit - 1) / g.nsplit, bk))};
+  a.vec = g.slab ? (g.N % 4 == 0 && quad_ok(g.slab, g.N, 4)) : (g.N % 4 == 0 && quad_ok(g.out, g.ldo, dtype_bytes(dtype)));
+  const int b = big_tiles(g.M, g.N, g.nsplit) ? 128 : 64;
+  a.gm = (g.M + b - 1) / b;
+  a.gn = (g.N + b - 1) / b;
+  const long long grid = (long long)a.gm * a.gn * g.nsplit;
+  if (grid == 0) return TT_OK;
+  TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
+  return with_type(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    const dim3 gr((unsigned)grid), bl(256);
+    if (g.xks) {
+      if (b == 128) hipLaunchKernelGGL((grad_product_kernel<T, true, 128, 128>), gr, bl, 0, st, a);
+      else hipLaunchKernelGGL((grad_product_kernel<T, true, 64, 64>), gr, bl, 0, st, a);
+    } else {
+      if (b == 128) hipLaunchKernelGGL((grad_product_kernel<T, false, 128, 128>), gr, bl, 0, st, a);
+      else hipLaunchKernelGGL((grad_product_kernel<T, false, 64, 64>), gr, bl, 0, st, a);
+    }
+    TT_CHECK_LAUNCH();
+    return (int)TT_OK;
+  });
+}
+
+extern "C" size_t tt_linear_act_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K,
+                                                int dtype) {
+  if (!known_dtype(dtype) || M < 0 || N < 1 || K < 1) return 0;
+  return pack_bytes(x, ldx, M, K, dtype) + pack_bytes(w, ldw, N, K, dtype);
+}
+
+extern "C" int tt_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+                             int64_t ldr, void* y, int64_t ldy, void* preact, int64_t M, int N, int K, int dtype, int act,
+                             void* workspace, size_t workspace_bytes, tt_stream_t stream) {
+  TT_REQUIRE(known_dtype(dtype), TT_ERR_BAD_DTYPE);
+  TT_REQUIRE(act >= TT_ACT_NONE && act <= TT_ACT_SILU, TT_ERR_UNSUPPORTED);
+  TT_REQUIRE(M >= 0 && M <= 0x7fffffffLL - 256 && N >= 1 && K >= 1 && ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N),
+             TT_ERR_BAD_SHAPE);
+  if (M == 0) return TT_OK;
+  TT_REQUIRE(x && w && y, TT_ERR_NULL_POINTER);
+  const size_t need = tt_linear_act_workspace_bytes(x, ldx, w, ldw, M, N, K, dtype);
+  TT_REQUIRE(need == 0 || workspace, TT_ERR_NULL_POINTER);
+  TT_REQUIRE(workspace_bytes >= need, TT_ERR_WORKSPACE);
+  TT_REQUIRE(need == 0 || tt_aligned16(workspace), TT_ERR_ALIGNMENT);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int width = dtype_bytes(dtype);
+  char* ws = static_cast<char*>(workspace);
+  const long long ldp = pad_to(K, 16 / width);
+  FwdArgs a{};
+  a.X = Operand{x, ldx};
+  a.W = Operand{w, ldw};
+  if (size_t n = pack_bytes(x, ldx, M, K, dtype)) {
+    int rc = tt_launch_pack(x, ldx, ws, ldp, M, K, width, st);
+    if (rc != TT_OK) return rc;
+    a.X = Operand{ws, ldp};
+    ws += n;
+  }
+  if (pack_bytes(w, ldw, N, K, dtype)) {
+    int rc = tt_launch_pack(w, ldw, ws, ldp, N, K, width, st);
+    if (rc != TT_OK) return rc;
+    a.W = Operand{ws, ldp};
+  }
+  a.s = Shape{(int)M, N, K, K};
+  a.bias = bias; a.res = residual; a.y = y; a.z = preact; a.ldr = ldr; a.ldy = ldy; a.act = act;
+  a.vec = N % 4 == 0 && quad_ok(bias, 0, width) && quad_ok(residual, ldr, width) && quad_ok(y, ldy, width) && quad_ok(preact, N, width);
+  const int b = big_tiles(M, N, 1) ? 128 : 64;
+  a.gn = (N + b - 1) / b;
+  const long long grid = ((M + b - 1) / b) * (long long)a.gn;
+  TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
+  return with_type(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    if (b == 128) hipLaunchKernelGGL((linear_fwd_kernel<T, 128, 128>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((linear_fwd_kernel<T, 64, 64>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    TT_CHECK_LAUNCH();
+    return (int)TT_OK;
+  });
+}
+
+namespace {
+struct BwdPlan {
+  bool own_dz;        // dz is written to the workspace (an activation, or a dy that cannot be read in 16-byte chunks)
+  long long ldz;
+  int splits, row_blocks, rows;
+  size_t dz, x, w, slab, part, total;
+};
+BwdPlan bwd_plan(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K,
+                 int dtype, int act, bool need_dw) {
+  BwdPlan p{};
+  const int width = dtype_bytes(dtype);
+  p.own_dz = act != TT_ACT_NONE || !packed_ok(dy, lddy, N, dtype);
+  p.ldz = p.own_dz ? pad_to(N, 16 / width) : lddy;
+  p.splits = need_dw ? tt_grad_splits(N, K, M) : 1;
+  const long long gx = (N + 255) / 256;
+  long long rb = (1024 + gx - 1) / gx;
+  if (rb > (M + 15) / 16) rb = (M + 15) / 16;
+  if (rb < 1) rb = 1;
+  p.rows = (int)((M + rb - 1) / rb);
+  if (p.rows < 1) p.rows = 1;
+  p.row_blocks = (int)((M + p.rows - 1) / p.rows);
+  if (p.row_blocks < 1) p.row_blocks = 1;
+  p.dz = p.own_dz ? align256((size_t)M * p.ldz * width) : 0;
+  p.x = pack_bytes(x, ldx, M, K, dtype);
+  p.w = pack_bytes(w, ldw, N, K, dtype);
+  p.slab = p.splits > 1 ? align256((size_t)p.splits * N * K * 4) : 0;
+  p.part = align256((size_t)p.row_blocks * N * 4);
+  p.total = p.dz + p.x + p.w + p.slab + p.part;
+  return p;
+}
+}  // namespace
+
+extern "C" size_t tt_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
+                                                    int64_t ldw, int64_t M, int N, int K, int dtype, int act) {
+  if (!known_dtype(dtype) || M < 0 || N < 1 || K < 1) return 0;
+  return bwd_plan(dy, lddy, x, ldx, w, ldw, M, N, K, dtype, act, true).total;
+}
+
+extern "C" int tt_linear_act_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                 const void* preact, void* dx, void* dw, void* dbias, int64_t M, int N, int K, int dtype, int act,
+                                 void* workspace, size_t workspace_bytes, tt_stream_t stream) {
+  TT_REQUIRE(known_dtype(dtype), TT_ERR_BAD_DTYPE);
+  TT_REQUIRE(act >= TT_ACT_NONE && act <= TT_ACT_SILU, TT_ERR_UNSUPPORTED);
+  TT_REQUIRE(M >= 0 && M <= 0x7fffffffLL - 256 && N >= 1 && K >= 1 && lddy >= N && ldx >= K && ldw >= K, TT_ERR_BAD_SHAPE);
+  TT_REQUIRE(workspace, TT_ERR_NULL_POINTER);
+  TT_REQUIRE(M == 0 || (dy && (!dx || w) && (!dw || x) && (act == TT_ACT_NONE || preact)), TT_ERR_NULL_POINTER);
+  TT_REQUIRE(tt_aligned16(workspace), TT_ERR_ALIGNMENT);
+  const BwdPlan p = bwd_plan(dy, lddy, x, ldx, w, ldw, M, N, K, dtype, act, true);
+  TT_REQUIRE(workspace_bytes >= p.total, TT_ERR_WORKSPACE);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int width = dtype_bytes(dtype);
+  int rc;
+  if (M == 0) {  // empty sums
+    if (dw && (rc = tt_launch_slab_sum(nullptr, 0, (long long)N * K, dw, dtype, 0.f, nullptr, st)) != TT_OK) return rc;
+    if (dbias && (rc = tt_launch_slab_sum(nullptr, 0, N, dbias, dtype, 0.f, nullptr, st)) != TT_OK) return rc;
+    return TT_OK;
+  }
+  char* ws = static_cast<char*>(workspace);
+  char* dz = ws;              ws += p.dz;
+  char* xp = ws;              ws += p.x;
+  char* wp = ws;              ws += p.w;
+  float* slab = (float*)ws;   ws += p.slab;
+  float* part = (float*)ws;
+  Operand Z{dy, lddy}, X{x, ldx}, W{w, ldw};
+  const bool products = dx || dw;
+  const bool write_dz = p.own_dz && products;
+  if (write_dz || dbias) {
+    if (write_dz && p.ldz != N) {  // the zero columns behind N are part of the operand
+      rc = tt_launch_pack(dy, lddy, dz, p.ldz, M, N, width, st);
+      if (rc != TT_OK) return rc;
+    }
+    DzArgs a{};
+    a.dy = dy; a.z = preact; a.dz = write_dz ? dz : nullptr; a.part = dbias ? part : nullptr;
+    a.lddy = lddy; a.ldz = p.ldz; a.M = (int)M; a.N = N; a.rows = p.rows; a.act = act;
+    a.vec = N % 4 == 0 && quad_ok(dy, lddy, width) && quad_ok(act == TT_ACT_NONE ? nullptr : preact, N, width);
+    rc = with_type(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      hipLaunchKernelGGL(linear_dz_kernel<T>, dim3((N + 255) / 256, p.row_blocks), dim3(256), 0, st, a);
+      TT_CHECK_LAUNCH();
+      return (int)TT_OK;
+    });
+    if (rc != TT_OK) return rc;
+    if (dbias && (rc = tt_launch_slab_sum(part, p.row_blocks, N, dbias, dtype, 1.f, nullptr, st)) != TT_OK) return rc;
+  }
+  if (write_dz) Z = Operand{dz, p.ldz};
+  if (dx) {
+    if (p.w) {
+      rc = tt_launch_pack(w, ldw, wp, pad_to(K, 16 / width), N, K, width, st);
+      if (rc != TT_OK) return rc;
+      W = Operand{wp, pad_to(K, 16 / width)};
+    }
+    GradProduct g{};
+    g.X = Z; g.Y = W; g.M = (int)M; g.N = K; g.K = N; g.xks = 0; g.nsplit = 1; g.out = dx; g.ldo = K; g.alpha = 1.f;
+    rc = tt_launch_grad_product(g, dtype, st);
+    if (rc != TT_OK) return rc;
+  }
+  if (dw) {
+    if (p.x) {
+      rc = tt_launch_pack(x, ldx, xp, pad_to(K, 16 / width), M, K, width, st);
+      if (rc != TT_OK) return rc;
+      X = Operand{xp, pad_to(K, 16 / width)};
+    }
+    GradProduct g{};
+    g.X = Z; g.Y = X; g.M = N; g.N = K; g.K = (int)M; g.xks = 1; g.nsplit = p.splits; g.alpha = 1.f;
+    if (p.splits > 1) g.slab = slab; else { g.out = dw; g.ldo = K; }
+    rc = tt_launch_grad_product(g, dtype, st);
+    if (rc != TT_OK) return rc;
+    if (p.splits > 1) return tt_launch_slab_sum(slab, p.splits, (long long)N * K, dw, dtype, 1.f, nullptr, st);
+  }
+  return TT_OK;
+}

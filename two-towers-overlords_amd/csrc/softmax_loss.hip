@@ -1,0 +1,361 @@
+// softmax_loss — cross entropy over a large set of candidates without keeping the logits, and its gradients.
+//
+//   l_ij = scale x_i.w_j,  lse_i = log sum_j exp l_ij,  loss_i = lse_i - l_i,target
+//   G_ij = c_i (exp(l_ij - lse_i) - [j = target_i]),  dx = scale G w,  dw = scale G^T x
+//
+// Forward: the product's epilogue leaves each row's maximum and sum of a tile's candidates (fp32, base 2); a second launch
+// joins them.  Backward: pieces of the candidates; a piece's G is recomputed from x, w and lse into the workspace, then dw of
+// the piece is final and dx is summed in fp32 over the pieces.  8 N V D operations instead of 6 with stored logits.
+//
+// G is rounded to the operands' type (it feeds matrix instructions).  float and bf16 share fp32's exponent range, so c goes
+// into G; fp16 takes c / max|c| times 2^14, and the products' epilogues take both out again: probabilities keep their
+// precision down to 2^-28 of the largest.
+//
+// The candidates of the same group as a row (cand_ids[j] == row_ids[i], j not the target) are left out of its sum.
+#include <type_traits>
+#include "mfma_tile.h"
+
+using namespace ttm;
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kF16Up = 16384.f;
+
+struct Args {
+  Operand X, W;
+  Shape s;               // M rows, N candidates (all of them, or a piece), K features
+  const long long *target, *rid, *cid;
+  long long ignore;
+  int v0, V, gn;         // first candidate of the piece; candidates in all; tiles along N
+  float scale2;          // scale * log2 e
+  float2* part;          // [gn, M] (maximum, sum) of a tile's candidates
+  float* tlogit;         // [M] the target's logit, base 2
+  const float *lse, *coef, *cmax;  // backward
+  void* G;
+  long long ldg;
+};
+
+// loss candidates of one row that this lane holds: excluded ones and those behind the last are -inf
+__device__ __forceinline__ float logit2(const Args& a, float v, int j, long long t, long long rid) {
+  if (j >= a.V || (a.rid && a.cid[j] == rid && j != t)) return -INFINITY;
+  return v * a.scale2;
+}
+
+template <class T, int BM, int BN>
+__global__ __launch_bounds__(256) void softmax_lse_kernel(Args a) {
+  __shared__ __align__(16) char lds[2 * (BM + BN) * kRowBytes];
+  constexpr int NI = BN / 64, MJ = BM / 64;
+  const int tl = xcd_tile(blockIdx.x, gridDim.x);
+  const int m0 = tl / a.gn * BM, tn = tl % a.gn, n0 = tn * BN;
+  f32x16 acc[NI][MJ];
+  tile_product<T, false, false, BM, BN>(acc, lds, a.X, a.W, a.s, m0, n0, 0, a.s.K);  // ends with a barrier
+  float2* red = reinterpret_cast<float2*>(lds);  // [2][BM]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5, wm = wave & 1, wn = wave >> 1;
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const int ml = (wm * MJ + j) * 32 + r, m = m0 + ml;
+    const bool in = m < a.s.M;
+    const long long t = in ? a.target[m] : -1, rid = in && a.rid ? a.rid[m] : 0;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int n = n0 + (wn * NI + i) * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+        const float v = logit2(a, acc[i][j][e], n, t, rid);
+        acc[i][j][e] = v;
+        mx = fmaxf(mx, v);
+        if (in && n == t) a.tlogit[m] = v;
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(acc[i][j][e] - base);
+    sum += __shfl_xor(sum, 32, 64);
+    if (h == 0) red[wn * BM + ml] = make_float2(mx, sum);
+  }
+  __syncthreads();
+  if (threadIdx.x < BM && m0 + (int)threadIdx.x < a.s.M) {
+    const float2 p = red[threadIdx.x], q = red[BM + threadIdx.x];
+    const float mx = fmaxf(p.x, q.x), base = mx == -INFINITY ? 0.f : mx;
+    const float sum = p.y * __builtin_amdgcn_exp2f(p.x - base) + q.y * __builtin_amdgcn_exp2f(q.x - base);
+    a.part[(long long)tn * a.s.M + m0 + threadIdx.x] = make_float2(mx, sum);
+  }
+}
+
+// joins the tiles' (maximum, sum) of each row: 16 rows x 16 lanes per workgroup, tiles in a fixed order
+__global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restrict__ part, const float* __restrict__ tlogit,
+                                                           const long long* __restrict__ target, long long ignore, int M, int V,
+                                                           int gn, float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ float2 red[16][17];
+  const int rl = threadIdx.x & 15, q = threadIdx.x >> 4, m = blockIdx.x * 16 + rl;
+  float mx = -INFINITY, sum = 0.f;
+  if (m < M) {
+    for (int t = q; t < gn; t += 16) {
+      const float2 p = part[(long long)t * M + m];
+      if (p.x > mx) {
+        sum = fmaf(sum, __builtin_amdgcn_exp2f(mx - p.x), p.y);
+        mx = p.x;
+      } else if (p.y != 0.f) {
+        sum = fmaf(p.y, p.x == mx ? 1.f : __builtin_amdgcn_exp2f(p.x - mx), sum);  // also carries a NaN on
+      }
+    }
+  }
+  red[rl][q] = make_float2(mx, sum);
+  __syncthreads();
+  if (q != 0 || m >= M) return;
+  mx = -INFINITY;
+  for (int t = 0; t < 16; ++t) mx = fmaxf(mx, red[rl][t].x);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  sum = 0.f;
+  for (int t = 0; t < 16; ++t) sum += red[rl][t].y * __builtin_amdgcn_exp2f(red[rl][t].x - base);
+  const float l2 = mx == -INFINITY && sum == 0.f ? -INFINITY : base + log2f(sum);
+  lse[m] = l2 * kLn2;
+  const long long t = target[m];
+  loss[m] = t == ignore ? 0.f : (t < 0 || t >= V ? NAN : (l2 - tlogit[m]) * kLn2);
+}
+
+// G of a piece of the candidates, [M, ldg] in T; columns behind the last candidate are zero
+template <class T, int BM, int BN>
+__global__ __launch_bounds__(256) void softmax_grad_kernel(Args a) {
+  __shared__ __align__(16) char lds[2 * (BM + BN) * kRowBytes];
+  constexpr int NI = BN / 64, MJ = BM / 64;
+  const int tl = xcd_tile(blockIdx.x, gridDim.x);
+  const int m0 = tl / a.gn * BM, n0 = tl % a.gn * BN;
+  f32x16 acc[NI][MJ];
+  tile_product<T, false, false, BM, BN>(acc, lds, a.X, a.W, a.s, m0, n0, 0, a.s.K);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5, wm = wave & 1, wn = wave >> 1;
+  T* __restrict__ G = static_cast<T*>(a.G);
+  const float up = __is_same(T, _Float16) ? kF16Up / *a.cmax : 1.f;
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    const int m = m0 + (wm * MJ + j) * 32 + r;
+    if (m >= a.s.M) continue;
+    const long long t = a.target[m], rid = a.rid ? a.rid[m] : 0;
+    const bool off = t == a.ignore;
+    const float lse2 = a.lse[m] * kLog2e, c = off ? 0.f : (t < 0 || t >= a.V ? NAN : a.coef[m] * up);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int nl = n0 + (wn * NI + i) * 32 + 8 * q + 4 * h;
+        f32x4 g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = a.v0 + nl + e;
+          const float v = logit2(a, acc[i][j][4 * q + e], n, t, rid);
+          const float p = v == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v - lse2);
+          g[e] = off || n >= a.V ? 0.f : c * (n == t ? p - 1.f : p);
+        }
+        if (nl < a.ldg) *reinterpret_cast<typename Type<T>::quad*>(G + m * a.ldg + nl) = to_quad<T>(g);
+      }
+  }
+}
+
+// cmax[0] = max |coef| over the rows that have a target (1 if that is 0 or not finite), cmax[1] = cmax[0] / kF16Up
+__global__ __launch_bounds__(1024) void softmax_cmax_kernel(const float* __restrict__ coef, const long long* __restrict__ target,
+                                                            long long ignore, int M, float* __restrict__ cmax) {
+  __shared__ float red[16];
+  float v = 0.f;
+  for (int m = threadIdx.x; m < M; m += 1024)
+    if (target[m] != ignore) v = fmaxf(v, fabsf(coef[m]));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; ++i) v = fmaxf(v, red[i]);
+  if (!(v > 0.f) || v == INFINITY) v = 1.f;
+  cmax[0] = v;
+  cmax[1] = v / kF16Up;
+}
+
+template <class F>
+int with_type(int dtype, F&& f) {
+  switch (dtype) {
+    case TT_F32: return f(float{});
+    case TT_BF16: return f(__bf16{});
+    case TT_F16: return f(_Float16{});
+    default: return TT_ERR_BAD_DTYPE;
+  }
+}
+
+int tile_of(long long M, long long N) { return ((M + 127) / 128) * ((N + 127) / 128) >= 256 ? 128 : 64; }
+
+struct Plan {
+  int gn, fwd_tile;
+  long long piece;      // candidates of a piece (a multiple of 128)
+  int pieces, sx, sw;   // splits of the two gradient products
+  size_t x, w, part, tlogit, cmax, G, dx, dw, fwd, bwd;
+};
+constexpr long long kPieceBytes = 256LL << 20;  // of G: what the Infinity Cache holds
+Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long M, int V, int D, int dtype) {
+  Plan p{};
+  const int width = dtype_bytes(dtype);
+  p.fwd_tile = tile_of(M, V);
+  p.gn = (V + p.fwd_tile - 1) / p.fwd_tile;
+  p.x = pack_bytes(x, ldx, M, D, dtype);
+  p.w = pack_bytes(w, ldw, V, D, dtype);
+  p.part = align256((size_t)p.gn * M * sizeof(float2));
+  p.tlogit = align256((size_t)M * 4);
+  p.fwd = p.x + p.w + p.part + p.tlogit;
+  const long long cap = kPieceBytes / (M * width) / 128 * 128;
+  const long long vp = pad_to(V, 128), most = cap < 1024 ? 1024 : cap;
+  p.pieces = (int)((vp + most - 1) / most);
+  p.piece = pad_to((vp + p.pieces - 1) / p.pieces, 128);
+  p.pieces = (int)((vp + p.piece - 1) / p.piece);
+  p.sx = tt_grad_splits(M, D, p.piece);
+  p.sw = tt_grad_splits(p.piece, D, M);
+  p.cmax = 256;
+  p.G = align256((size_t)M * p.piece * width);
+  p.dx = p.pieces > 1 || p.sx > 1 ? align256((size_t)p.sx * M * D * 4) : 0;
+  p.dw = p.sw > 1 ? align256((size_t)p.sw * p.piece * D * 4) : 0;
+  p.bwd = p.x + p.w + p.cmax + p.G + p.dx + p.dw;
+  return p;
+}
+
+int check(int64_t ldx, int64_t ldw, int64_t N, int V, int D, int dtype, float scale) {
+  TT_REQUIRE(dtype == TT_F32 || dtype == TT_BF16 || dtype == TT_F16, TT_ERR_BAD_DTYPE);
+  TT_REQUIRE(N >= 0 && N <= 0x7fffffffLL - 256 && V >= 1 && V <= 0x7fffffff - 256 && D >= 1 && ldx >= D && ldw >= D && scale > 0.f,
+             TT_ERR_BAD_SHAPE);
+  return TT_OK;
+}
+
+int operand(Operand& o, const void* p, long long ld, long long rows, int D, int dtype, size_t bytes, char* ws, hipStream_t st) {
+  o = Operand{p, ld};
+  if (!bytes) return TT_OK;
+  const long long ldp = pad_to(D, 16 / dtype_bytes(dtype));
+  o = Operand{ws, ldp};
+  return tt_launch_pack(p, ld, ws, ldp, rows, D, dtype_bytes(dtype), st);
+}
+
+}  // namespace
+
+extern "C" size_t tt_softmax_loss_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int V, int D,
+                                                  int dtype) {
+  if (check(ldx, ldw, N, V, D, dtype, 1.f) != TT_OK || N == 0) return 0;
+  return plan(x, ldx, w, ldw, N, V, D, dtype).fwd;
+}
+extern "C" size_t tt_softmax_loss_bwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int V, int D,
+                                                      int dtype) {
+  if (check(ldx, ldw, N, V, D, dtype, 1.f) != TT_OK || N == 0) return 0;
+  return plan(x, ldx, w, ldw, N, V, D, dtype).bwd;
+}
+
+extern "C" int tt_softmax_loss(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, const int64_t* row_ids,
+                               const int64_t* cand_ids, int64_t N, int V, int D, int dtype, float scale, int64_t ignore_index,
+                               float* loss, float* lse, void* workspace, size_t workspace_bytes, tt_stream_t stream) {
+  int rc = check(ldx, ldw, N, V, D, dtype, scale);
+  if (rc != TT_OK) return rc;
+  TT_REQUIRE((row_ids == nullptr) == (cand_ids == nullptr), TT_ERR_NULL_POINTER);
+  if (N == 0) return TT_OK;
+  TT_REQUIRE(x && w && target && loss && lse && workspace, TT_ERR_NULL_POINTER);
+  const Plan p = plan(x, ldx, w, ldw, N, V, D, dtype);
+  TT_REQUIRE(workspace_bytes >= p.fwd, TT_ERR_WORKSPACE);
+  TT_REQUIRE(tt_aligned16(workspace), TT_ERR_ALIGNMENT);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  Args a{};
+  if ((rc = operand(a.X, x, ldx, N, D, dtype, p.x, ws, st)) != TT_OK) return rc;
+  ws += p.x;
+  if ((rc = operand(a.W, w, ldw, V, D, dtype, p.w, ws, st)) != TT_OK) return rc;
+  ws += p.w;
+  a.part = (float2*)ws;    ws += p.part;
+  a.tlogit = (float*)ws;
+  a.s = Shape{(int)N, V, D, D};
+  a.target = (const long long*)target; a.rid = (const long long*)row_ids; a.cid = (const long long*)cand_ids;
+  a.ignore = ignore_index; a.V = V; a.gn = p.gn; a.scale2 = scale * kLog2e;
+  const int b = p.fwd_tile;
+  const long long grid = ((N + b - 1) / b) * (long long)p.gn;
+  TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
+  rc = with_type(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    if (b == 128) hipLaunchKernelGGL((softmax_lse_kernel<T, 128, 128>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((softmax_lse_kernel<T, 64, 64>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    TT_CHECK_LAUNCH();
+    return (int)TT_OK;
+  });
+  if (rc != TT_OK) return rc;
+  hipLaunchKernelGGL(softmax_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, a.part, a.tlogit, a.target, a.ignore,
+                     (int)N, V, p.gn, loss, lse);
+  TT_CHECK_LAUNCH();
+  return TT_OK;
+}
+
+extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target,
+                                   const int64_t* row_ids, const int64_t* cand_ids, const float* lse, int64_t N, int V, int D,
+                                   int dtype, float scale, int64_t ignore_index, void* dx, void* dw, void* workspace,
+                                   size_t workspace_bytes, tt_stream_t stream) {
+  int rc = check(ldx, ldw, N, V, D, dtype, scale);
+  if (rc != TT_OK) return rc;
+  TT_REQUIRE((row_ids == nullptr) == (cand_ids == nullptr), TT_ERR_NULL_POINTER);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (N == 0) return dw ? tt_launch_slab_sum(nullptr, 0, (long long)V * D, dw, dtype, 0.f, nullptr, st) : (int)TT_OK;
+  TT_REQUIRE(row_coef && x && w && target && lse && workspace, TT_ERR_NULL_POINTER);
+  const Plan p = plan(x, ldx, w, ldw, N, V, D, dtype);
+  TT_REQUIRE(workspace_bytes >= p.bwd, TT_ERR_WORKSPACE);
+  TT_REQUIRE(tt_aligned16(workspace), TT_ERR_ALIGNMENT);
+  if (!dx && !dw) return TT_OK;
+  const int width = dtype_bytes(dtype);
+  char* ws = static_cast<char*>(workspace);
+  Args a{};
+  if ((rc = operand(a.X, x, ldx, N, D, dtype, p.x, ws, st)) != TT_OK) return rc;
+  ws += p.x;
+  Operand W;
+  if ((rc = operand(W, w, ldw, V, D, dtype, p.w, ws, st)) != TT_OK) return rc;
+  ws += p.w;
+  float* cmax = (float*)ws;   ws += p.cmax;
+  a.G = ws;                   ws += p.G;
+  float* dxs = (float*)ws;    ws += p.dx;
+  float* dws = (float*)ws;
+  const float* alpha_dev = nullptr;
+  if (dtype == TT_F16) {
+    hipLaunchKernelGGL(softmax_cmax_kernel, dim3(1), dim3(1024), 0, st, row_coef, (const long long*)target, (long long)ignore_index,
+                       (int)N, cmax);
+    TT_CHECK_LAUNCH();
+    alpha_dev = cmax + 1;
+  }
+  a.target = (const long long*)target; a.rid = (const long long*)row_ids; a.cid = (const long long*)cand_ids;
+  a.ignore = ignore_index; a.V = V; a.scale2 = scale * kLog2e; a.lse = lse; a.coef = row_coef; a.cmax = cmax; a.ldg = p.piece;
+  for (int i = 0; i < p.pieces; ++i) {
+    const long long v0 = i * p.piece;
+    const int vc = (int)(V - v0 < p.piece ? V - v0 : p.piece);
+    a.v0 = (int)v0;
+    a.W = Operand{static_cast<const char*>(W.p) + v0 * W.ld * width, W.ld};
+    a.s = Shape{(int)N, vc, D, D};
+    const int b = tile_of(N, p.piece);
+    a.gn = (int)((p.piece + b - 1) / b);
+    const long long grid = ((N + b - 1) / b) * (long long)a.gn;
+    TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
+    rc = with_type(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      if (b == 128) hipLaunchKernelGGL((softmax_grad_kernel<T, 128, 128>), dim3((unsigned)grid), dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((softmax_grad_kernel<T, 64, 64>), dim3((unsigned)grid), dim3(256), 0, st, a);
+      TT_CHECK_LAUNCH();
+      return (int)TT_OK;
+    });
+    if (rc != TT_OK) return rc;
+    if (dx) {
+      GradProduct g{};
+      g.X = Operand{a.G, p.piece}; g.Y = a.W; g.M = (int)N; g.N = D; g.K = vc; g.xks = 0; g.nsplit = p.sx;
+      g.alpha = scale; g.alpha_dev = alpha_dev;
+      if (p.dx) { g.slab = dxs; g.accumulate = i > 0; } else { g.out = dx; g.ldo = D; }
+      if ((rc = tt_launch_grad_product(g, dtype, st)) != TT_OK) return rc;
+    }
+    if (dw) {
+      GradProduct g{};
+      g.X = Operand{a.G, p.piece}; g.Y = a.X; g.M = vc; g.N = D; g.K = (int)N; g.xks = 1; g.nsplit = p.sw;
+      g.alpha = scale; g.alpha_dev = alpha_dev;
+      char* out = static_cast<char*>(dw) + v0 * D * width;
+      if (p.sw > 1) g.slab = dws; else { g.out = out; g.ldo = D; }
+      if ((rc = tt_launch_grad_product(g, dtype, st)) != TT_OK) return rc;
+      if (p.sw > 1 && (rc = tt_launch_slab_sum(dws, p.sw, (long long)vc * D, out, dtype, scale, alpha_dev, st)) != TT_OK) return rc;
+    }
+  }
+  if (dx && p.dx) return tt_launch_slab_sum(dxs, p.sx, (long long)N * D, dx, dtype, scale, alpha_dev, st);
+  return TT_OK;
+}

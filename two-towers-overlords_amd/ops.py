@@ -427,3 +427,277 @@ def inbatch_triplet_fwd_bwd(q: torch.Tensor, d: torch.Tensor, margin: float, pos
         call("tt_inbatch_triplet_fwd_bwd_f32", q.data_ptr(), d.data_ptr(), _ptr(pos_index), _ptr(qid_q), _ptr(qid_d), margin,
              gs, den, Bq, Bd, P, loss.data_ptr(), dq.data_ptr(), dd.data_ptr(), 0, ws.data_ptr(), nbytes, _stream())
     return loss, dq, dd
+
+
+# --------------------------------------------------------------------------- encoder operators and the softmax loss
+_FLOAT = {torch.float32: _lib.TT_F32, torch.bfloat16: _lib.TT_BF16, torch.float16: _lib.TT_F16}
+
+
+def _float_type(t: torch.Tensor, name: str) -> int:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t)}")
+    if t.dtype not in _FLOAT:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return _FLOAT[t.dtype]
+
+
+def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, shape=None) -> int:
+    """Checks a [rows, cols] operand whose rows are contiguous and returns its row stride in elements."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t)}")
+    if not t.is_cuda:
+        _req(t, name)  # the "no CPU fallback" refusal
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name}: expected shape {'2-D' if shape is None else tuple(shape)}, got {tuple(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise TypeError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous (stride {t.stride()})")
+    if rows <= 1:
+        return max(cols, 1)
+    if t.stride(0) < cols:
+        raise ValueError(f"{name}: rows overlap (stride {t.stride()}); materialise a broadcast tensor first")
+    return t.stride(0)
+
+
+def _activation(name: str) -> int:
+    if name not in _lib.ACTIVATIONS:
+        raise ValueError(f"activation: one of {', '.join(_lib.ACTIVATIONS)}, got {name!r}")
+    return _lib.ACTIVATIONS[name]
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor:
+    # from the caching allocator on every call: a buffer kept between calls would be shared by captured graphs and streams
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+               activation: str = "none", save_preact: bool = False, out: Optional[torch.Tensor] = None):
+    """act(x @ w.T + bias) + residual -> [M, N]: a Linear layer ([N, K] weights) with its activation ("none", "relu", "gelu",
+    "gelu_tanh", "silu") and the residual add in the product's epilogue.  float32, bfloat16 or float16 throughout, fp32 sums,
+    one rounding.  x / residual / out may be row-strided views.  save_preact=True also returns the pre-activation [M, N] that
+    `linear_act_bwd` needs (None for "none").  `out` may be `residual`, and may not overlap x or w.
+    What the nn.Linear calls of the frozen encoder do (backend/model.py:51-52)."""
+    dt = _float_type(x, "x")
+    act = _activation(activation)
+    ldx = _rows(x, "x")
+    M, K = x.shape
+    ldw = _rows(w, "w", like=x)
+    N = w.shape[0]
+    if w.shape[1] != K or K < 1 or N < 1:
+        raise ValueError(f"linear_act: x {tuple(x.shape)} and w {tuple(w.shape)} must share a last dimension >= 1, w needs a row")
+    if bias is not None:
+        _req(bias, "bias", x.dtype, 1)
+        if bias.shape[0] != N or bias.device != x.device:
+            raise ValueError(f"bias: expected shape {(N,)} on {x.device}")
+    ldr = _rows(residual, "residual", like=x, shape=(M, N)) if residual is not None else 0
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device) if out is None else out
+    ldy = _rows(y, "out", like=x, shape=(M, N))
+    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if save_preact and act else None
+    if M:
+        with _on(x.device):
+            nbytes = _lib.load().tt_linear_act_workspace_bytes(x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K, dt)
+            ws = _workspace(nbytes, x.device) if nbytes else None
+            call("tt_linear_act", x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(bias), _ptr(residual), ldr, y.data_ptr(), ldy, _ptr(z),
+                 M, N, K, dt, act, _ptr(ws), nbytes, _stream())
+    return (y, z) if save_preact else y
+
+
+def linear_act_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact: Optional[torch.Tensor] = None,
+                   activation: str = "none", bias: bool = True, need_dx: bool = True, need_dw: bool = True):
+    """Gradients of `linear_act` -> (dx [M, K], dw [N, K], dbias [N]); None where not asked for.  preact: what
+    `linear_act(save_preact=True)` returned.  The residual's gradient is dy."""
+    dt = _float_type(x, "x")
+    act = _activation(activation)
+    ldx = _rows(x, "x")
+    M, K = x.shape
+    ldw = _rows(w, "w", like=x)
+    N = w.shape[0]
+    if w.shape[1] != K or K < 1 or N < 1:
+        raise ValueError(f"linear_act_bwd: x {tuple(x.shape)} and w {tuple(w.shape)} must share a last dimension >= 1")
+    lddy = _rows(dy, "dy", like=x, shape=(M, N))
+    if act:
+        if preact is None:
+            raise ValueError(f"linear_act_bwd: activation {activation!r} needs the pre-activation (save_preact=True)")
+        _req(preact, "preact", x.dtype, 2)
+        if tuple(preact.shape) != (M, N) or preact.device != x.device:
+            raise ValueError(f"preact: expected shape {(M, N)} on {x.device}")
+    dx = torch.empty((M, K), dtype=x.dtype, device=x.device) if need_dx else None
+    dw = torch.empty((N, K), dtype=x.dtype, device=x.device) if need_dw else None
+    db = torch.empty(N, dtype=x.dtype, device=x.device) if bias else None
+    if dx is not None or dw is not None or db is not None:
+        with _on(x.device):
+            nbytes = _lib.load().tt_linear_act_bwd_workspace_bytes(dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K,
+                                                                   dt, act)
+            ws = _workspace(nbytes, x.device)
+            call("tt_linear_act_bwd", dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(preact) if act else None,
+                 _ptr(dx), _ptr(dw), _ptr(db), M, N, K, dt, act, ws.data_ptr(), nbytes, _stream())
+    return dx, dw, db
+
+
+def _head_view(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, shape=None) -> _lib.TTHeadView:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t)}")
+    if not t.is_cuda:
+        _req(t, name)
+    if t.dim() != 3 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name}: expected shape {'[tokens, heads, head_dim]' if shape is None else tuple(shape)}, got {tuple(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise TypeError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    st, sh, sd = t.stride()
+    st, sh = (0 if t.shape[0] <= 1 else st), (0 if t.shape[1] <= 1 else sh)
+    kpf = 16 // t.element_size()
+    if sd != 1 or st % kpf or sh % kpf or t.data_ptr() % 16:
+        raise ValueError(f"{name}: head_dim must be contiguous, rows and base 16-byte aligned (stride {t.stride()})")
+    return _lib.TTHeadView(t.data_ptr(), st, sh)
+
+
+def _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask) -> _lib.TTAttentionArgs:
+    a = _lib.TTAttentionArgs()
+    a.dtype = _float_type(q, "q")
+    a.q = _head_view(q, "q")
+    T, H, Dh = q.shape
+    Hkv = k.shape[1] if k.dim() == 3 else 0
+    a.k = _head_view(k, "k", like=q, shape=(T, Hkv, Dh))
+    a.v = _head_view(v, "v", like=q, shape=(T, Hkv, Dh))
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise ValueError(f"packed_attention: {H} query heads are not a multiple of {Hkv} key heads")
+    if not 8 <= Dh <= 128 or Dh % 8:
+        raise ValueError(f"packed_attention: head_dim must be a multiple of 8 in 8..128, got {Dh}")
+    _req(cu_seqlens, "cu_seqlens", torch.int32, 1)
+    docs = cu_seqlens.shape[0] - 1
+    if docs < 1 or cu_seqlens.device != q.device:
+        raise ValueError(f"cu_seqlens: expected [documents + 1] on {q.device}, got {tuple(cu_seqlens.shape)} on {cu_seqlens.device}")
+    if causal and prefix is not None:
+        raise ValueError("packed_attention: causal and prefix exclude each other (a prefix of 0 is causal)")
+    for t, name, dtype, n in ((prefix, "prefix", torch.int32, docs), (slopes, "slopes", torch.float32, H)):
+        if t is not None:
+            _req(t, name, dtype, 1)
+            if t.shape[0] != n or t.device != q.device:
+                raise ValueError(f"{name}: expected shape {(n,)} on {q.device}")
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise ValueError("slopes: the distance bias has no gradient")
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8):
+            raise TypeError(f"key_mask: expected bool or uint8, got {key_mask.dtype}")
+        _req(key_mask, "key_mask", ndim=1)
+        if key_mask.shape[0] != T or key_mask.device != q.device:
+            raise ValueError(f"key_mask: expected shape {(T,)} on {q.device}")
+    scale = Dh ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf") or not 0.0 <= softcap < float("inf"):
+        raise ValueError(f"packed_attention: scale must be positive and softcap >= 0, got {scale}, {softcap}")
+    a.T, a.docs, a.heads, a.kv_heads, a.head_dim, a.causal = T, docs, H, Hkv, Dh, int(bool(causal))
+    a.scale, a.softcap = scale, softcap
+    a.cu_seqlens, a.prefix, a.slopes, a.key_mask = cu_seqlens.data_ptr(), _ptr(prefix), _ptr(slopes), _ptr(key_mask)
+    return a
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: Optional[float] = None,
+                     causal: bool = False, prefix: Optional[torch.Tensor] = None, softcap: float = 0.0,
+                     slopes: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None):
+    """Attention inside documents packed back to back -> (out [T, H, Dh], lse [H, T] float32).
+    q [T, H, Dh], k / v [T, Hkv, Dh] (float32, bfloat16 or float16; column blocks of one projection's output are fine), H a
+    multiple of Hkv.  Document b holds tokens [cu_seqlens[b], cu_seqlens[b+1]) (int32 on the device, from 0, ascending, empty
+    documents allowed; tokens behind the last document get 0).  scale: 1/sqrt(Dh) by default.  A query sees the keys of its own
+    document whose `key_mask` is set; causal: only j <= i; prefix [documents] int32: only j <= i or j < prefix.  softcap > 0: the
+    scores become softcap * tanh(score / softcap); slopes [H] float32: slopes[h] * |i - j| is subtracted.  A query that sees
+    nothing gets 0 (lse -inf).  What masked keys hold does not matter, NaN included.
+    The attention of the frozen encoder (backend/model.py:51-52) without its padding."""
+    a = _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((a.heads, a.T), dtype=torch.float32, device=q.device)
+    if a.T:
+        a.out, a.lse = _head_view(out, "out"), lse.data_ptr()
+        with _on(q.device):
+            call("tt_packed_attention", a, _stream())
+    return out, lse
+
+
+def packed_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
+                         cu_seqlens: torch.Tensor, scale: Optional[float] = None, causal: bool = False,
+                         prefix: Optional[torch.Tensor] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                         key_mask: Optional[torch.Tensor] = None, grads: Optional[Tuple[torch.Tensor, ...]] = None):
+    """Gradients of `packed_attention` -> (dq, dk, dv), given its arguments and what it returned.  grads: (dq, dk, dv) to write
+    into — column blocks of one buffer, say, when q, k, v are; they may not overlap the inputs.  No atomics: the same
+    inputs give the same bits."""
+    a = _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask)
+    a.out = _head_view(out, "out", like=q, shape=q.shape)
+    a.dout = _head_view(dout, "dout", like=q, shape=q.shape)
+    _req(lse, "lse", torch.float32, 2)
+    if tuple(lse.shape) != (a.heads, a.T) or lse.device != q.device:
+        raise ValueError(f"lse: expected shape {(a.heads, a.T)} on {q.device}")
+    if grads is None:
+        grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = grads
+    a.dq = _head_view(dq, "dq", like=q, shape=q.shape)
+    a.dk = _head_view(dk, "dk", like=q, shape=k.shape)
+    a.dv = _head_view(dv, "dv", like=q, shape=v.shape)
+    if a.T:
+        delta = torch.empty((a.heads, a.T), dtype=torch.float32, device=q.device)
+        a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
+        with _on(q.device):
+            call("tt_packed_attention_bwd", a, _stream())
+    return dq, dk, dv
+
+
+def _softmax_args(x, w, target, scale, row_ids, cand_ids):
+    dt = _float_type(x, "x")
+    ldx = _rows(x, "x")
+    N, D = x.shape
+    ldw = _rows(w, "w", like=x)
+    V = w.shape[0]
+    if w.shape[1] != D or D < 1 or V < 1:
+        raise ValueError(f"softmax_loss: x {tuple(x.shape)} and w {tuple(w.shape)} must share a last dimension >= 1, w needs a row")
+    if (row_ids is None) != (cand_ids is None):
+        raise ValueError("softmax_loss: give both row_ids and cand_ids or neither")
+    for t, name, n in ((target, "target", N), (row_ids, "row_ids", N), (cand_ids, "cand_ids", V)):
+        if t is None and name != "target":
+            continue
+        _req(t, name, torch.int64, 1)
+        if t.shape[0] != n or t.device != x.device:
+            raise ValueError(f"{name}: expected shape {(n,)} on {x.device}")
+    if not 0.0 < float(scale) < float("inf"):
+        raise ValueError(f"softmax_loss: scale must be positive, got {scale}")
+    return dt, ldx, ldw, N, V, D
+
+
+def softmax_loss(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, scale: float = 1.0, row_ids: Optional[torch.Tensor] = None,
+                 cand_ids: Optional[torch.Tensor] = None, ignore_index: int = -100):
+    """Softmax cross entropy of every row of x [N, D] over the candidates w [V, D] -> (loss [N], lse [N]), both float32: the logits
+    are scale * x @ w.T and are never stored.  target [N] int64: the row's candidate; `ignore_index` = no loss and no gradient
+    for the row; any other value outside [0, V) gives NaN.  row_ids [N] / cand_ids [V] int64: candidates of the row's own id
+    other than its target are left out of its sum (the documents of the same query in an in-batch loss).
+    x and w: float32, bfloat16 or float16, row-strided views allowed."""
+    dt, ldx, ldw, N, V, D = _softmax_args(x, w, target, scale, row_ids, cand_ids)
+    loss = torch.empty(N, dtype=torch.float32, device=x.device)
+    lse = torch.empty(N, dtype=torch.float32, device=x.device)
+    if N:
+        with _on(x.device):
+            nbytes = _lib.load().tt_softmax_loss_workspace_bytes(x.data_ptr(), ldx, w.data_ptr(), ldw, N, V, D, dt)
+            ws = _workspace(nbytes, x.device)
+            call("tt_softmax_loss", x.data_ptr(), ldx, w.data_ptr(), ldw, target.data_ptr(), _ptr(row_ids), _ptr(cand_ids), N, V, D, dt,
+                 float(scale), int(ignore_index), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes, _stream())
+    return loss, lse
+
+
+def softmax_loss_bwd(row_coef: torch.Tensor, x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, lse: torch.Tensor,
+                     scale: float = 1.0, row_ids: Optional[torch.Tensor] = None, cand_ids: Optional[torch.Tensor] = None,
+                     ignore_index: int = -100, need_dx: bool = True, need_dw: bool = True):
+    """Gradients of sum_i row_coef[i] * loss[i] -> (dx [N, D], dw [V, D]), None where not asked for.  lse: what `softmax_loss`
+    returned.  row_coef [N] float32: 1/N everywhere for a mean."""
+    dt, ldx, ldw, N, V, D = _softmax_args(x, w, target, scale, row_ids, cand_ids)
+    for t, name in ((row_coef, "row_coef"), (lse, "lse")):
+        _req(t, name, torch.float32, 1)
+        if t.shape[0] != N or t.device != x.device:
+            raise ValueError(f"{name}: expected shape {(N,)} on {x.device}")
+    dx = torch.empty((N, D), dtype=x.dtype, device=x.device) if need_dx else None
+    dw = torch.empty((V, D), dtype=x.dtype, device=x.device) if need_dw else None
+    if dx is not None or dw is not None:
+        with _on(x.device):
+            nbytes = _lib.load().tt_softmax_loss_bwd_workspace_bytes(x.data_ptr(), ldx, w.data_ptr(), ldw, N, V, D, dt)
+            ws = _workspace(nbytes, x.device)
+            call("tt_softmax_loss_bwd", row_coef.data_ptr(), x.data_ptr(), ldx, w.data_ptr(), ldw, target.data_ptr(), _ptr(row_ids),
+                 _ptr(cand_ids), lse.data_ptr(), N, V, D, dt, float(scale), int(ignore_index), _ptr(dx), _ptr(dw), ws.data_ptr(),
+                 nbytes, _stream())
+    return dx, dw
