@@ -25,6 +25,29 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// Eight 16-bit rows x four columns (or four float rows x four columns), one 8- / 16-byte load per row, to four 16-byte
+// chunks of consecutive rows: two v_perm_b32 make the pairs of two columns, the rest is register naming.
+template <class T> struct KsUnit;
+template <> struct KsUnit<float> {
+  f32x4 v[4];
+  __device__ __forceinline__ u32x4 column(int c) const {
+    f32x4 o = {v[0][c], v[1][c], v[2][c], v[3][c]};
+    return __builtin_bit_cast(u32x4, o);
+  }
+};
+struct KsUnit16 {
+  u32x2 v[8];
+  __device__ __forceinline__ u32x4 column(int c) const {
+    const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;  // high / low halves of (row k + 1, row k)
+    u32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = __builtin_amdgcn_perm(v[2 * j + 1][c >> 1], v[2 * j][c >> 1], sel);
+    return o;
+  }
+};
+template <> struct KsUnit<__bf16> : KsUnit16 {};
+template <> struct KsUnit<_Float16> : KsUnit16 {};
+
 struct Args {
   const void *q, *k, *v, *o, *dout;
   long long qt, qh, kt, kh, vt, vh, ot, oh, dot, doh;  // element strides per token and head
@@ -109,8 +132,8 @@ struct Dim {
 
 // row image: TILE rows of the head's chunks, 128-byte column blocks
 template <class T, int DP>
-__device__ __forceinline__ u32x4 row_frag(const char* __restrict__ img, int row, int chunk) {
-  return frag(img + (chunk >> 3) * (Dim<T, DP>::TILE * kRowBytes), row, chunk & 7);
+__device__ __forceinline__ u32x4 head_frag(const char* __restrict__ img, int row, int chunk) {
+  return row_frag(img + (chunk >> 3) * (Dim<T, DP>::TILE * kRowBytes), row, chunk & 7);
 }
 
 // Staging of a tile of rows [r0, r0 + TILE) of one head into a row image and / or a transposed image.  Rows at or behind
@@ -284,7 +307,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_fwd_kernel(Args a, int s
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 #pragma unroll
-        for (int g = 0; g < D::G; ++g) mma<T>(acc, row_frag<T, DP>(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
+        for (int g = 0; g < D::G; ++g) mma<T>(acc, head_frag<T, DP>(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
         s[t] = acc;
       }
       unsigned long long vis = 0;
@@ -335,7 +358,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_fwd_kernel(Args a, int s
         if (32 * (g / PER) >= rem) break;  // uniform: the second half of a tile behind the last key
         const u32x4 pf = acc_frag<T>(s[g / PER], g % PER);
 #pragma unroll
-        for (int t = 0; t < D::DT; ++t) mma<T>(o[t], frag(vimg, 32 * t + r, 2 * g + h), pf);
+        for (int t = 0; t < D::DT; ++t) mma<T>(o[t], row_frag(vimg, 32 * t + r, 2 * g + h), pf);
       }
     }
     __syncthreads();
@@ -448,8 +471,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dq_kernel(Args a, int sl
         for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
 #pragma unroll
         for (int g = 0; g < D::G; ++g) {
-          mma<T>(s, row_frag<T, DP>(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
-          mma<T>(dp, row_frag<T, DP>(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
+          mma<T>(s, head_frag<T, DP>(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
+          mma<T>(dp, head_frag<T, DP>(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
         }
         shape_scores<T, true>(s, d, a, slope, i - (k0 + 32 * t), h);
 #pragma unroll
@@ -471,7 +494,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dq_kernel(Args a, int sl
         for (int g = 0; g < PER; ++g) {
           const u32x4 f = acc_frag<T>(s, g);
 #pragma unroll
-          for (int u = 0; u < D::DT; ++u) mma<T>(acc[u], frag(ktim, 32 * u + r, 2 * (t * PER + g) + h), f);
+          for (int u = 0; u < D::DT; ++u) mma<T>(acc[u], row_frag(ktim, 32 * u + r, 2 * (t * PER + g) + h), f);
         }
       }
     }
@@ -573,8 +596,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv_kernel(Args a, int s
           for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
 #pragma unroll
           for (int g = 0; g < D::G; ++g) {
-            mma<T>(s, row_frag<T, DP>(qimg, 32 * t + fold<T>(r), 2 * g + h), kf[g]);
-            mma<T>(dp, row_frag<T, DP>(dimg, 32 * t + fold<T>(r), 2 * g + h), vf[g]);
+            mma<T>(s, head_frag<T, DP>(qimg, 32 * t + fold<T>(r), 2 * g + h), kf[g]);
+            mma<T>(dp, head_frag<T, DP>(dimg, 32 * t + fold<T>(r), 2 * g + h), vf[g]);
           }
           shape_scores<T, true>(s, d, a, slope, j - (q0 + 32 * t), h);
 #pragma unroll
@@ -593,8 +616,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv_kernel(Args a, int s
             const u32x4 pf = acc_frag<T>(s, g), sf = acc_frag<T>(dp, g);
 #pragma unroll
             for (int u = 0; u < D::DT; ++u) {
-              mma<T>(av[u], frag(dtim, 32 * u + r, 2 * (t * PER + g) + h), pf);
-              mma<T>(ak[u], frag(qtim, 32 * u + r, 2 * (t * PER + g) + h), sf);
+              mma<T>(av[u], row_frag(dtim, 32 * u + r, 2 * (t * PER + g) + h), pf);
+              mma<T>(ak[u], row_frag(qtim, 32 * u + r, 2 * (t * PER + g) + h), sf);
             }
           }
         }

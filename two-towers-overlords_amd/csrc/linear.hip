@@ -81,13 +81,14 @@ struct FwdArgs {
   int act, vec, gn;  // gn: tiles along N
 };
 
-template <class T, int BM, int BN>
-__global__ __launch_bounds__(256) void linear_fwd_kernel(FwdArgs a) {
-  __shared__ __align__(16) char lds[2 * (BM + BN) * kRowBytes];
+template <class T, class B>
+__global__ __launch_bounds__(B::THREADS) void linear_fwd_kernel(FwdArgs a) {
+  __shared__ __align__(16) char b0[B::BYTES];
+  __shared__ __align__(16) char b1[B::BYTES];
   const int t = xcd_tile(blockIdx.x, gridDim.x);
-  const int m0 = t / a.gn * BM, n0 = t % a.gn * BN;
-  f32x16 acc[BN / 64][BM / 64];
-  tile_product<T, false, false, BM, BN>(acc, lds, a.X, a.W, a.s, m0, n0, 0, a.s.K);
+  const int m0 = t / a.gn * B::BM, n0 = t % a.gn * B::BN;
+  B blk;
+  blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
   const T* __restrict__ bias = static_cast<const T*>(a.bias);
   const T* __restrict__ res = static_cast<const T*>(a.res);
   T* __restrict__ y = static_cast<T*>(a.y);
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(256) void linear_fwd_kernel(FwdArgs a) {
   const bool vec = a.vec;
   with_act(a.act, [&](auto tag) {
     constexpr int ACT = decltype(tag)::value;
-    for_quads<BM, BN>(acc, m0, n0, [&](int m, int n, f32x4 v) {
+    blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
       if (m >= M) return;
       if (bias) v += load_quad<T>(bias, 0, 0, n, N, vec);
       if (z) {
@@ -191,22 +192,23 @@ struct GradArgs {
   Shape s;
   int gm, gn, vec;
 };
-template <class T, bool XKS, int BM, int BN>
-__global__ __launch_bounds__(256) void grad_product_kernel(GradArgs a) {
-  __shared__ __align__(16) char lds[2 * (BM + BN) * kRowBytes];
+template <class T, bool XKS, class B>
+__global__ __launch_bounds__(B::THREADS) void grad_product_kernel(GradArgs a) {
+  __shared__ __align__(16) char b0[B::BYTES];
+  __shared__ __align__(16) char b1[B::BYTES];
   const int tiles = a.gm * a.gn;
   const int id = xcd_tile(blockIdx.x, gridDim.x);
   const int z = id / tiles, t = id - z * tiles;
-  const int m0 = t / a.gn * BM, n0 = t % a.gn * BN;
-  f32x16 acc[BN / 64][BM / 64];
+  const int m0 = t / a.gn * B::BM, n0 = t % a.gn * B::BN;
+  B blk;
   const int kbeg = z * a.s.kper;
-  tile_product<T, XKS, true, BM, BN>(acc, lds, a.g.X, a.g.Y, a.s, m0, n0, kbeg, min(a.s.K, kbeg + a.s.kper));
+  blk.template product<T, XKS, true>(b0, b1, a.g.X, a.g.Y, a.s, m0, n0, kbeg, min(a.s.K, kbeg + a.s.kper));
   const int M = a.s.M, N = a.s.N;
   const bool vec = a.vec;
   if (a.g.slab) {
     float* __restrict__ c = a.g.slab + (long long)z * M * N;
     const bool more = a.g.accumulate;
-    for_quads<BM, BN>(acc, m0, n0, [&](int m, int n, f32x4 v) {
+    blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
       if (m >= M) return;
       if (more) v += load_quad<float>(c, N, m, n, N, vec);
       store_quad<float>(c, N, m, n, N, vec, v);
@@ -215,7 +217,7 @@ __global__ __launch_bounds__(256) void grad_product_kernel(GradArgs a) {
     T* __restrict__ c = static_cast<T*>(a.g.out);
     const float alpha = a.g.alpha_dev ? a.g.alpha * *a.g.alpha_dev : a.g.alpha;
     const long long ldo = a.g.ldo;
-    for_quads<BM, BN>(acc, m0, n0, [&](int m, int n, f32x4 v) {
+    blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
       if (m < M) store_quad<T>(c, ldo, m, n, N, vec, v * alpha);
     });
   }
@@ -282,11 +284,11 @@ int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
     using T = decltype(tag);
     const dim3 gr((unsigned)grid), bl(256);
     if (g.xks) {
-      if (b == 128) hipLaunchKernelGGL((grad_product_kernel<T, true, 128, 128>), gr, bl, 0, st, a);
-      else hipLaunchKernelGGL((grad_product_kernel<T, true, 64, 64>), gr, bl, 0, st, a);
+      if (b == 128) hipLaunchKernelGGL((grad_product_kernel<T, true, Mid>), gr, bl, 0, st, a);
+      else hipLaunchKernelGGL((grad_product_kernel<T, true, Small>), gr, bl, 0, st, a);
     } else {
-      if (b == 128) hipLaunchKernelGGL((grad_product_kernel<T, false, 128, 128>), gr, bl, 0, st, a);
-      else hipLaunchKernelGGL((grad_product_kernel<T, false, 64, 64>), gr, bl, 0, st, a);
+      if (b == 128) hipLaunchKernelGGL((grad_product_kernel<T, false, Mid>), gr, bl, 0, st, a);
+      else hipLaunchKernelGGL((grad_product_kernel<T, false, Small>), gr, bl, 0, st, a);
     }
     TT_CHECK_LAUNCH();
     return (int)TT_OK;
@@ -339,8 +341,8 @@ extern "C" int tt_linear_act(const void* x, int64_t ldx, const void* w, int64_t 
   TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
   return with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
-    if (b == 128) hipLaunchKernelGGL((linear_fwd_kernel<T, 128, 128>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((linear_fwd_kernel<T, 64, 64>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    if (b == 128) hipLaunchKernelGGL((linear_fwd_kernel<T, Mid>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((linear_fwd_kernel<T, Small>), dim3((unsigned)grid), dim3(256), 0, st, a);
     TT_CHECK_LAUNCH();
     return (int)TT_OK;
   });

@@ -60,39 +60,54 @@ __device__ __forceinline__ f32x4 from_quad(typename Type<T>::quad v) {
   return __builtin_convertvector(v, f32x4);
 }
 
-// LDS image of an operand tile: rows of 128 bytes (BK = 128 / sizeof(T) consecutive k), eight 16-byte chunks whose position
-// is XORed with a function of the row.  Reads (lanes = consecutive rows, one chunk) meet 16 different slots per 16 rows;
-// so do the transposing writes of stage_ks (lanes = every fourth row, one chunk): conflict-free both ways.
+// LDS images.  Every operand tile is kept as it lies in memory, in blocks of rows of 128 bytes: eight 16-byte chunks whose
+// position is XORed with a function of the row.  A block is read two ways:
+//   along its rows (row_frag: lanes = 16 consecutive rows, one chunk): a K-contiguous operand;
+//   across them (col_frag: lanes = 32 consecutive columns, KPF rows each): a K-strided operand, transposed by the read itself —
+//   16-bit by two ds_read_b64_tr_b16 (16 lanes hand in four rows of 32 bytes, each gets four rows of its column), float by
+//   four ds_read_b32.
+// The XOR reverses bits 1..3 of the row: 16 rows at one chunk lie in 16 different slots, and four rows at one 64-byte window
+// in the four quarters of the banks: both reads are free of bank conflicts.
 constexpr int kRowBytes = 128;
-__device__ __forceinline__ int swz(int row, int chunk) { return row * kRowBytes + ((chunk ^ ((row >> 1) ^ (row >> 4))) & 7) * 16; }
+__device__ __forceinline__ int twist(int row) { return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1); }
+__device__ __forceinline__ int swz(int row, int chunk) { return row * kRowBytes + (chunk ^ twist(row)) * 16; }
 
-__device__ __forceinline__ u32x4 frag(const char* __restrict__ tile, int row, int chunk) {
-  return *reinterpret_cast<const u32x4*>(tile + swz(row, chunk));
+__device__ __forceinline__ u32x4 row_frag(const char* __restrict__ block, int row, int chunk) {
+  return *reinterpret_cast<const u32x4*>(block + swz(row, chunk));
 }
 
-// Eight 16-bit rows x four columns (or four float rows x four columns), one 8- / 16-byte load per row, to four 16-byte
-// chunks of consecutive k: the transposition of a K-strided operand on its way into LDS.  16-bit: two v_perm_b32 make the
-// (k, k+1) pairs of two columns, the rest is register naming.
-template <class T> struct KsUnit;
-template <> struct KsUnit<float> {
-  f32x4 v[4];
-  __device__ __forceinline__ u32x4 column(int c) const {
-    f32x4 o = {v[0][c], v[1][c], v[2][c], v[3][c]};
-    return __builtin_bit_cast(u32x4, o);
-  }
-};
-struct KsUnit16 {
-  u32x2 v[8];
-  __device__ __forceinline__ u32x4 column(int c) const {
-    const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;  // high / low halves of (row k + 1, row k)
-    u32x4 o;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+__device__ __forceinline__ u32x2 tr_read(const char* __restrict__ p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+}
+// rows [k, k + KPF) of column (col0 + lane & 31), k = k0 + KPF * (lane >> 5);  k0 % (2 KPF) == 0, col0 % 32 == 0
+template <class T>
+__device__ __forceinline__ u32x4 col_frag(const char* __restrict__ block, int k0, int col0, int lane) {
+  if constexpr (sizeof(T) == 4) {
+    const int c = col0 + (lane & 31), k = k0 + 4 * (lane >> 5);
+    u32x4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = __builtin_amdgcn_perm(v[2 * j + 1][c >> 1], v[2 * j][c >> 1], sel);
-    return o;
+    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t*>(block + swz(k + j, c >> 2) + (c & 3) * 4);
+    return v;
+  } else {
+    const int j = lane & 15;
+    const int c = col0 + (lane & 16) + 4 * (j & 3), k = k0 + 8 * (lane >> 5) + (j >> 2);
+    const int at = (c & 4) * 2;  // the second half of a 16-byte chunk
+    const u32x2 lo = tr_read(block + swz(k, c >> 3) + at), hi = tr_read(block + swz(k + 4, c >> 3) + at);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
-};
-template <> struct KsUnit<__bf16> : KsUnit16 {};
-template <> struct KsUnit<_Float16> : KsUnit16 {};
+}
+
+// Global memory to LDS without registers: each lane names its 16 bytes, a wave fills 1024 contiguous bytes (8 rows of a
+// block).  The caller waits (stage_wait) before anyone reads.
+typedef __attribute__((address_space(1))) const void gas_void;
+typedef __attribute__((address_space(3))) void las_void;
+__device__ __forceinline__ void lds_fill(const char* src, char* dst) {
+  __builtin_amdgcn_global_load_lds((gas_void*)src, (las_void*)dst, 16, 0, 0);
+}
+// This wave's outstanding fills have landed and its LDS accesses are done; then the whole workgroup's.
+__device__ __forceinline__ void stage_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // ---- a product's operand in global memory ------------------------------------------------------------------
 // `p` is 16-byte aligned, `ld` a multiple of KPF elements, and so is the contiguous extent (callers pack what is not).
@@ -102,59 +117,51 @@ struct Operand {
   long long ld;
 };
 
-// One operand's staging registers for a tile of R rows x BK, 256 threads.
-template <class T, bool KS, int R>
-struct Stage {
-  static constexpr int KPF = Type<T>::KPF, BK = kRowBytes / (int)sizeof(T);
-  static constexpr int kChunks = R * 8 / 256;                       // KS = false: 16-byte chunks per thread
-  static constexpr int kUnits = 8 * (R / 4), kPer = (kUnits + 255) / 256;  // KS = true: transposing units per thread
-  u32x4 c[KS ? 1 : kChunks];
-  KsUnit<T> u[KS ? kPer : 1];
+// A tile of an operand in LDS: K-contiguous one block of R rows (128 bytes of k each); K-strided BK rows in R * sizeof(T) / 128
+// column blocks.  Either way R * 128 bytes, filled in groups of 8 rows x 128 bytes, one group per wave and instruction.
+template <class T, bool KS, int R, int WAVES>
+struct Tile {
+  static constexpr int KPF = Type<T>::KPF, BK = kRowBytes / (int)sizeof(T), BYTES = R * kRowBytes;
+  static constexpr int N = R / 8 / WAVES;  // groups per wave
+  static_assert(R % (8 * WAVES) == 0 && R % BK == 0, "whole groups per wave, whole column blocks");
+  uint32_t off[N];  // of this lane's 16 bytes of each group, from the tile's first element
 
-  __device__ __forceinline__ void load(const Operand& o, int r0, int rows, int k0, int kend, int tid) {
-    const T* __restrict__ p = static_cast<const T*>(o.p);
-    if constexpr (!KS) {
+  // r0: first row of the output side, r0 < rows: how many there are (K-strided: readable columns)
+  __device__ __forceinline__ void init(const Operand& o, int r0, int rows, int wave, int lane) {
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int f = tid + i * 256, row = f >> 3, ch = f & 7;
-        const int gr = min(r0 + row, rows - 1), gk = k0 + ch * KPF;  // rows past the end: any row, their results are not stored
-        const u32x4 v = *reinterpret_cast<const u32x4*>(p + gr * o.ld + min(gk, (kend - 1) / KPF * KPF));
-        c[i] = gk < kend ? v : u32x4{0, 0, 0, 0};
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int f = tid + i * 256;
-        if (kUnits % 256 != 0 && f >= kUnits) break;
-        const int kg = f / (R / 4), cq = f % (R / 4);
-        const int gr = min(r0 + 4 * cq, rows - 4);
-#pragma unroll
-        for (int j = 0; j < KPF; ++j) {
-          const int gk = k0 + kg * KPF + j;
-          using V = decltype(u[i].v[0] + u[i].v[0]);
-          const V v = *reinterpret_cast<const V*>(p + min(gk, kend - 1) * o.ld + gr);
-          u[i].v[j] = gk < kend ? v : V(0);
-        }
+    for (int i = 0; i < N; ++i) {
+      const int g = i * WAVES + wave, row = 8 * g + (lane >> 3);
+      if constexpr (!KS) {
+        const int ch = (lane & 7) ^ twist(row);
+        off[i] = (uint32_t)(((long long)(min(r0 + row, rows - 1) - r0) * o.ld + ch * KPF) * (int)sizeof(T));
+      } else {
+        const int blk = row / BK, k = row % BK, ch = (lane & 7) ^ twist(k);
+        off[i] = (uint32_t)((k * o.ld + min(r0 + blk * BK + ch * KPF, rows - KPF) - r0) * (int)sizeof(T));
       }
     }
   }
-  __device__ __forceinline__ void store(char* __restrict__ tile, int tid) const {
-    if constexpr (!KS) {
+  static __device__ __forceinline__ const char* base(const Operand& o, int r0, int k0) {
+    return static_cast<const char*>(o.p) + (KS ? k0 * o.ld + r0 : r0 * o.ld + k0) * (long long)sizeof(T);
+  }
+  __device__ __forceinline__ void fill(const char* __restrict__ src, char* __restrict__ tile, int wave) const {
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int f = tid + i * 256;
-        *reinterpret_cast<u32x4*>(tile + swz(f >> 3, f & 7)) = c[i];
-      }
-    } else {
+    for (int i = 0; i < N; ++i) lds_fill(src + off[i], tile + (i * WAVES + wave) * 1024);
+  }
+  // the last, partial step of k: what lies at or behind kend arrives as zero
+  __device__ __forceinline__ void fill_tail(const char* __restrict__ src, char* __restrict__ tile, int left, int wave, int lane) const {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int f = tid + i * 256;
-        if (kUnits % 256 != 0 && f >= kUnits) break;
-        const int kg = f / (R / 4), cq = f % (R / 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(tile + swz(4 * cq + j, kg)) = u[i].column(j);
-      }
+    for (int i = 0; i < N; ++i) {
+      const int row = 8 * (i * WAVES + wave) + (lane >> 3);
+      const int k = KS ? row % BK : ((lane & 7) ^ twist(row)) * KPF;
+      u32x4 v = {0, 0, 0, 0};
+      if (k < left) v = *reinterpret_cast<const u32x4*>(src + off[i]);
+      *reinterpret_cast<u32x4*>(tile + (i * WAVES + wave) * 1024 + lane * 16) = v;
     }
+  }
+  // fragment of rows [row0, row0 + 32) of the output side, group g of the step's k
+  static __device__ __forceinline__ u32x4 get(const char* __restrict__ tile, int row0, int g, int lane) {
+    if constexpr (!KS) return row_frag(tile, row0 + (lane & 31), 2 * g + (lane >> 5));
+    else return col_frag<T>(tile + row0 / BK * (BK * kRowBytes), g * 2 * KPF, row0 % BK, lane);
   }
 };
 
@@ -171,77 +178,115 @@ struct Shape {
   int kper;         // k of one split (a multiple of BK unless there is one split)
 };
 
-// The product of one BM x BN tile: acc[i][j] is the 32x32 tile of output columns n0 + 32 (wn * NI + i) + ..., output rows
-// m0 + 32 (wm * MJ + j) + ...  256 threads, waves 2 x 2.  `lds` holds 2 * (BM + BN) * 128 bytes.
-// X: output rows (M), Y: output columns (N).
-template <class T, bool XKS, bool YKS, int BM, int BN>
-__device__ __forceinline__ void tile_product(f32x16 (&acc)[BN / 64][BM / 64], char* __restrict__ lds, const Operand& X,
-                                             const Operand& Y, const Shape& s, int m0, int n0, int kbeg, int kend) {
-  constexpr int BK = kRowBytes / (int)sizeof(T);
-  constexpr int NI = BN / 64, MJ = BM / 64;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int r = lane & 31, h = lane >> 5, wm = wave & 1, wn = wave >> 1;
+// A workgroup's tile: BM x BN outputs, WM x WN waves of MJ x NI accumulators each; two LDS buffers of BYTES.
+template <int BM_, int BN_, int WM_, int WN_>
+struct Block {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int MJ = BM / 32 / WM, NI = BN / 32 / WN, BYTES = (BM + BN) * kRowBytes;
+  f32x16 acc[NI][MJ];
+  int lane, wave, r, h, wm, wn;
+
+  __device__ __forceinline__ Block() {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    r = lane & 31;
+    h = lane >> 5;
+    wm = wave % WM;
+    wn = wave / WM;
+  }
+
+  // acc[i][j]: output columns n0 + 32 (wn * NI + i) + row, output rows m0 + 32 (wm * MJ + j) + (lane & 31).
+  // X: output rows (M), Y: output columns (N).  One step ahead: the next step's tiles stream into the other buffer under
+  // this step's matrix instructions; one barrier a step.  LDS may be reused after the caller's next barrier.
+  // float: every other step goes to a second set of accumulators, which halves the length of the chains of additions.
+  template <class T, bool XKS, bool YKS>
+  __device__ __forceinline__ void product(char* __restrict__ b0, char* __restrict__ b1, const Operand& X, const Operand& Y,
+                                          const Shape& s, int m0, int n0, int kbeg, int kend) {
+    using TX = Tile<T, XKS, BM, WAVES>;
+    using TY = Tile<T, YKS, BN, WAVES>;
+    constexpr int BK = TX::BK;
+    constexpr bool TWO = sizeof(T) == 4;
+    f32x16 acc2[TWO ? NI : 1][TWO ? MJ : 1];
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int j = 0; j < MJ; ++j)
+      for (int j = 0; j < MJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  if (kbeg >= kend) return;
-  char* const xt[2] = {lds, lds + BM * kRowBytes};
-  char* const yt[2] = {lds + 2 * BM * kRowBytes, lds + (2 * BM + BN) * kRowBytes};
-  Stage<T, XKS, BM> sx;
-  Stage<T, YKS, BN> sy;
-  // a padded contiguous extent bounds what a row clamp may touch
-  const int xr = XKS ? (s.M + Type<T>::KPF - 1) / Type<T>::KPF * Type<T>::KPF : s.M;
-  const int yr = YKS ? (s.N + Type<T>::KPF - 1) / Type<T>::KPF * Type<T>::KPF : s.N;
-  sx.load(X, m0, xr, kbeg, kend, tid);
-  sy.load(Y, n0, yr, kbeg, kend, tid);
-  sx.store(xt[0], tid);
-  sy.store(yt[0], tid);
-  __syncthreads();
-  int b = 0;
-  for (int k = kbeg; k < kend; k += BK, b ^= 1) {
-    const bool more = k + BK < kend;
-    if (more) {
-      sx.load(X, m0, xr, k + BK, kend, tid);
-      sy.load(Y, n0, yr, k + BK, kend, tid);
+        for (int e = 0; e < 16; ++e) {
+          acc[i][j][e] = 0.f;
+          if constexpr (TWO) acc2[i][j][e] = 0.f;
+        }
+    if (kbeg >= kend) return;
+    constexpr int KPF = Type<T>::KPF;
+    // a padded contiguous extent bounds what a column clamp may touch
+    const int xr = XKS ? (s.M + KPF - 1) / KPF * KPF : s.M, yr = YKS ? (s.N + KPF - 1) / KPF * KPF : s.N;
+    TX tx;
+    TY ty;
+    tx.init(X, m0, xr, wave, lane);
+    ty.init(Y, n0, yr, wave, lane);
+    const char* xs = TX::base(X, m0, kbeg);
+    const char* ys = TY::base(Y, n0, kbeg);
+    const long long xstep = (XKS ? X.ld * BK : BK) * (long long)sizeof(T), ystep = (YKS ? Y.ld * BK : BK) * (long long)sizeof(T);
+    const int steps = (kend - kbeg + BK - 1) / BK, left = kend - kbeg - (steps - 1) * BK;
+    auto issue = [&](int t, char* __restrict__ b) {
+      if (t + 1 < steps || left == BK) {
+        tx.fill(xs, b, wave);
+        ty.fill(ys, b + BM * kRowBytes, wave);
+        xs += xstep;
+        ys += ystep;
+      } else {
+        tx.fill_tail(xs, b, left, wave, lane);
+        ty.fill_tail(ys, b + BM * kRowBytes, left, wave, lane);
+      }
+    };
+    auto step = [&](int t, char* __restrict__ cur, char* __restrict__ nxt, auto& c) {
+      stage_wait();
+      if (t + 1 < steps) issue(t + 1, nxt);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        u32x4 fy[NI], fx[MJ];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) fy[i] = TY::get(cur + BM * kRowBytes, (wn * NI + i) * 32, g, lane);
+#pragma unroll
+        for (int j = 0; j < MJ; ++j) fx[j] = TX::get(cur, (wm * MJ + j) * 32, g, lane);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int j = 0; j < MJ; ++j) mma<T>(c[i][j], fy[i], fx[j]);
+      }
+    };
+    issue(0, b0);
+    for (int t = 0; t < steps; t += 2) {
+      step(t, b0, b1, acc);
+      if (t + 1 < steps) {
+        if constexpr (TWO) step(t + 1, b1, b0, acc2);
+        else step(t + 1, b1, b0, acc);
+      }
     }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      u32x4 fy[NI], fx[MJ];
-#pragma unroll
-      for (int i = 0; i < NI; ++i) fy[i] = frag(yt[b], (wn * NI + i) * 32 + r, 2 * g + h);
-#pragma unroll
-      for (int j = 0; j < MJ; ++j) fx[j] = frag(xt[b], (wm * MJ + j) * 32 + r, 2 * g + h);
+    if constexpr (TWO) {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < MJ; ++j) mma<T>(acc[i][j], fy[i], fx[j]);
+        for (int j = 0; j < MJ; ++j) acc[i][j] += acc2[i][j];
     }
-    if (more) {
-      sx.store(xt[b ^ 1], tid);
-      sy.store(yt[b ^ 1], tid);
-    }
-    __syncthreads();
   }
-}
 
-// Calls fn(m, n, quad) for every quad of four consecutive output columns this lane holds, tile by tile.
-template <int BM, int BN, class F>
-__device__ __forceinline__ void for_quads(f32x16 (&acc)[BN / 64][BM / 64], int m0, int n0, F&& fn) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = lane & 31, h = lane >> 5, wm = wave & 1, wn = wave >> 1;
+  // Calls fn(m, n, quad) for every quad of four consecutive output columns this lane holds.
+  template <class F>
+  __device__ __forceinline__ void for_quads(int m0, int n0, F&& fn) {
 #pragma unroll
-  for (int j = 0; j < BM / 64; ++j)
+    for (int j = 0; j < MJ; ++j)
 #pragma unroll
-    for (int i = 0; i < BN / 64; ++i)
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const f32x4 v = {acc[i][j][4 * a], acc[i][j][4 * a + 1], acc[i][j][4 * a + 2], acc[i][j][4 * a + 3]};
-        fn(m0 + (wm * (BM / 64) + j) * 32 + r, n0 + (wn * (BN / 64) + i) * 32 + 8 * a + 4 * h, v);
-      }
-}
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 v = {acc[i][j][4 * a], acc[i][j][4 * a + 1], acc[i][j][4 * a + 2], acc[i][j][4 * a + 3]};
+          fn(m0 + (wm * MJ + j) * 32 + r, n0 + (wn * NI + i) * 32 + 8 * a + 4 * h, v);
+        }
+  }
+};
+using Small = Block<64, 64, 2, 2>;
+using Mid = Block<128, 128, 2, 2>;
 
 // one row's quad at columns [n, n + 4) of a row-major matrix; `vec`: whole quads are in range and aligned
 template <class T>
@@ -278,7 +323,8 @@ inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // Can a [rows, cols] matrix of row stride ld be read in 16-byte chunks as it is?
 inline bool packed_ok(const void* p, long long ld, long long cols, int dtype) {
   const int kpf = 16 / dtype_bytes(dtype);
-  return tt_aligned16(p) && ld % kpf == 0 && cols % kpf == 0;
+  // (the last bound keeps a tile's 32-bit offsets in range)
+  return tt_aligned16(p) && ld % kpf == 0 && cols % kpf == 0 && ld < (1 << 22);
 }
 // bytes of its packed copy (row stride padded to 16 bytes, the padding zero), 0 if it needs none
 inline size_t pack_bytes(const void* p, long long ld, long long rows, long long cols, int dtype) {

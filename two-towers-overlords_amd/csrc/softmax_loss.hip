@@ -36,22 +36,24 @@ struct Args {
   long long ldg;
 };
 
-// loss candidates of one row that this lane holds: excluded ones and those behind the last are -inf
-__device__ __forceinline__ float logit2(const Args& a, float v, int j, long long t, long long rid) {
-  if (j >= a.V || (a.rid && a.cid[j] == rid && j != t)) return -INFINITY;
-  return v * a.scale2;
+// Is candidate j left out of the row's sum (its own group, or behind the last)?
+__device__ __forceinline__ bool left_out(const Args& a, int j, long long t, long long rid) {
+  return j >= a.V || (a.rid && a.cid[j] == rid && j != t);
 }
 
-template <class T, int BM, int BN>
-__global__ __launch_bounds__(256) void softmax_lse_kernel(Args a) {
-  __shared__ __align__(16) char lds[2 * (BM + BN) * kRowBytes];
-  constexpr int NI = BN / 64, MJ = BM / 64;
+template <class T, class B>
+__global__ __launch_bounds__(B::THREADS) void softmax_lse_kernel(Args a) {
+  __shared__ __align__(16) char b0[B::BYTES];
+  __shared__ __align__(16) char b1[B::BYTES];
+  constexpr int NI = B::NI, MJ = B::MJ;
   const int tl = xcd_tile(blockIdx.x, gridDim.x);
-  const int m0 = tl / a.gn * BM, tn = tl % a.gn, n0 = tn * BN;
-  f32x16 acc[NI][MJ];
-  tile_product<T, false, false, BM, BN>(acc, lds, a.X, a.W, a.s, m0, n0, 0, a.s.K);  // ends with a barrier
-  float2* red = reinterpret_cast<float2*>(lds);  // [2][BM]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5, wm = wave & 1, wn = wave >> 1;
+  const int m0 = tl / a.gn * B::BM, tn = tl % a.gn, n0 = tn * B::BN;
+  B blk;
+  blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
+  auto& acc = blk.acc;
+  const int r = blk.r, h = blk.h, wm = blk.wm, wn = blk.wn;
+  __syncthreads();
+  float2* red = reinterpret_cast<float2*>(b0);  // [WN][BM]
 #pragma unroll
   for (int j = 0; j < MJ; ++j) {
     const int ml = (wm * MJ + j) * 32 + r, m = m0 + ml;
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(256) void softmax_lse_kernel(Args a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int n = n0 + (wn * NI + i) * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-        const float v = logit2(a, acc[i][j][e], n, t, rid);
+        const float v = left_out(a, n, t, rid) ? -INFINITY : acc[i][j][e] * a.scale2;
         acc[i][j][e] = v;
         mx = fmaxf(mx, v);
         if (in && n == t) a.tlogit[m] = v;
@@ -76,14 +78,18 @@ __global__ __launch_bounds__(256) void softmax_lse_kernel(Args a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(acc[i][j][e] - base);
     sum += __shfl_xor(sum, 32, 64);
-    if (h == 0) red[wn * BM + ml] = make_float2(mx, sum);
+    if (h == 0) red[wn * B::BM + ml] = make_float2(mx, sum);
   }
   __syncthreads();
-  if (threadIdx.x < BM && m0 + (int)threadIdx.x < a.s.M) {
-    const float2 p = red[threadIdx.x], q = red[BM + threadIdx.x];
-    const float mx = fmaxf(p.x, q.x), base = mx == -INFINITY ? 0.f : mx;
-    const float sum = p.y * __builtin_amdgcn_exp2f(p.x - base) + q.y * __builtin_amdgcn_exp2f(q.x - base);
-    a.part[(long long)tn * a.s.M + m0 + threadIdx.x] = make_float2(mx, sum);
+  for (int ml = threadIdx.x; ml < B::BM && m0 + ml < a.s.M; ml += B::THREADS) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < B::WN; ++k) mx = fmaxf(mx, red[k * B::BM + ml].x);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < B::WN; ++k) sum = fmaf(red[k * B::BM + ml].y, __builtin_amdgcn_exp2f(red[k * B::BM + ml].x - base), sum);
+    a.part[(long long)tn * a.s.M + m0 + ml] = make_float2(mx, sum);
   }
 }
 
@@ -120,15 +126,17 @@ __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restr
 }
 
 // G of a piece of the candidates, [M, ldg] in T; columns behind the last candidate are zero
-template <class T, int BM, int BN>
-__global__ __launch_bounds__(256) void softmax_grad_kernel(Args a) {
-  __shared__ __align__(16) char lds[2 * (BM + BN) * kRowBytes];
-  constexpr int NI = BN / 64, MJ = BM / 64;
+template <class T, class B>
+__global__ __launch_bounds__(B::THREADS) void softmax_grad_kernel(Args a) {
+  __shared__ __align__(16) char b0[B::BYTES];
+  __shared__ __align__(16) char b1[B::BYTES];
+  constexpr int NI = B::NI, MJ = B::MJ;
   const int tl = xcd_tile(blockIdx.x, gridDim.x);
-  const int m0 = tl / a.gn * BM, n0 = tl % a.gn * BN;
-  f32x16 acc[NI][MJ];
-  tile_product<T, false, false, BM, BN>(acc, lds, a.X, a.W, a.s, m0, n0, 0, a.s.K);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5, wm = wave & 1, wn = wave >> 1;
+  const int m0 = tl / a.gn * B::BM, n0 = tl % a.gn * B::BN;
+  B blk;
+  blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
+  auto& acc = blk.acc;
+  const int r = blk.r, h = blk.h, wm = blk.wm, wn = blk.wn;
   T* __restrict__ G = static_cast<T*>(a.G);
   const float up = __is_same(T, _Float16) ? kF16Up / *a.cmax : 1.f;
 #pragma unroll
@@ -147,8 +155,7 @@ __global__ __launch_bounds__(256) void softmax_grad_kernel(Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int n = a.v0 + nl + e;
-          const float v = logit2(a, acc[i][j][4 * q + e], n, t, rid);
-          const float p = v == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v - lse2);
+          const float p = left_out(a, n, t, rid) ? 0.f : __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + e], a.scale2, -lse2));
           g[e] = off || n >= a.V ? 0.f : c * (n == t ? p - 1.f : p);
         }
         if (nl < a.ldg) *reinterpret_cast<typename Type<T>::quad*>(G + m * a.ldg + nl) = to_quad<T>(g);
@@ -274,8 +281,8 @@ extern "C" int tt_softmax_loss(const void* x, int64_t ldx, const void* w, int64_
   TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
   rc = with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
-    if (b == 128) hipLaunchKernelGGL((softmax_lse_kernel<T, 128, 128>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((softmax_lse_kernel<T, 64, 64>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    if (b == 128) hipLaunchKernelGGL((softmax_lse_kernel<T, Mid>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((softmax_lse_kernel<T, Small>), dim3((unsigned)grid), dim3(256), 0, st, a);
     TT_CHECK_LAUNCH();
     return (int)TT_OK;
   });
@@ -328,13 +335,13 @@ extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t
     a.W = Operand{static_cast<const char*>(W.p) + v0 * W.ld * width, W.ld};
     a.s = Shape{(int)N, vc, D, D};
     const int b = tile_of(N, p.piece);
-    a.gn = (int)((p.piece + b - 1) / b);
+    a.gn = (vc + b - 1) / b;  // every tile starts at a candidate of the piece; the last one zero-fills behind it
     const long long grid = ((N + b - 1) / b) * (long long)a.gn;
     TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
     rc = with_type(dtype, [&](auto tag) {
       using T = decltype(tag);
-      if (b == 128) hipLaunchKernelGGL((softmax_grad_kernel<T, 128, 128>), dim3((unsigned)grid), dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((softmax_grad_kernel<T, 64, 64>), dim3((unsigned)grid), dim3(256), 0, st, a);
+      if (b == 128) hipLaunchKernelGGL((softmax_grad_kernel<T, Mid>), dim3((unsigned)grid), dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((softmax_grad_kernel<T, Small>), dim3((unsigned)grid), dim3(256), 0, st, a);
       TT_CHECK_LAUNCH();
       return (int)TT_OK;
     });
