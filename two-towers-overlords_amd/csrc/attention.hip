@@ -25,29 +25,6 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Eight 16-bit rows x four columns (or four float rows x four columns), one 8- / 16-byte load per row, to four 16-byte
-// chunks of consecutive rows: two v_perm_b32 make the pairs of two columns, the rest is register naming.
-template <class T> struct KsUnit;
-template <> struct KsUnit<float> {
-  f32x4 v[4];
-  __device__ __forceinline__ u32x4 column(int c) const {
-    f32x4 o = {v[0][c], v[1][c], v[2][c], v[3][c]};
-    return __builtin_bit_cast(u32x4, o);
-  }
-};
-struct KsUnit16 {
-  u32x2 v[8];
-  __device__ __forceinline__ u32x4 column(int c) const {
-    const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;  // high / low halves of (row k + 1, row k)
-    u32x4 o;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = __builtin_amdgcn_perm(v[2 * j + 1][c >> 1], v[2 * j][c >> 1], sel);
-    return o;
-  }
-};
-template <> struct KsUnit<__bf16> : KsUnit16 {};
-template <> struct KsUnit<_Float16> : KsUnit16 {};
-
 struct Args {
   const void *q, *k, *v, *o, *dout;
   long long qt, qh, kt, kh, vt, vh, ot, oh, dot, doh;  // element strides per token and head
@@ -122,77 +99,94 @@ struct Dim {
   static constexpr int KPF = Type<T>::KPF;
   static constexpr int TILE = kRowBytes / (int)sizeof(T);     // rows of a tile: 64 (16-bit) or 32 (float)
   static constexpr int SUB = TILE / 32;                       // accumulator tiles of a tile
+  static constexpr int PER = 4 / SUB;                         // fragments of an accumulator tile, as the second product's operand
   static constexpr int CH = DP / KPF;                         // 16-byte chunks of a row
   static constexpr int G = CH / 2;                            // matrix instructions' groups along the head
-  static constexpr int GT = 4;                                // groups along a tile's rows
   static constexpr int DT = DP / 32;                          // accumulator tiles along the head
-  static constexpr int ROWS = ((CH + 7) / 8) * TILE * kRowBytes;  // bytes of a row image
-  static constexpr int COLS = DP * kRowBytes;                     // bytes of a transposed image
+  static constexpr int PITCH = CH < 8 ? CH * 16 : kRowBytes;  // bytes of a row in a block; a block is 128 bytes wide, or the head
+  static constexpr int CPB = PITCH / 16;
+  static constexpr int BYTES = TILE * CH * 16;                // of a tile's image
+  static constexpr int RPG = 1024 / PITCH;                    // rows that a wave fills with one instruction
+  static constexpr int GROUPS = BYTES / 1024;
 };
 
-// row image: TILE rows of the head's chunks, 128-byte column blocks
+__device__ __constant__ uint32_t kZeros[4] = {0, 0, 0, 0};  // what a lane reads for a row that is not there
+
+// The image of a tile of TILE rows of one head, as it lies in memory: read along the rows (the first products) and across
+// them (the second ones).  64-byte rows are twisted by bits 2..3 of the row, which has the same effect as `twist`.
 template <class T, int DP>
-__device__ __forceinline__ u32x4 head_frag(const char* __restrict__ img, int row, int chunk) {
-  return row_frag(img + (chunk >> 3) * (Dim<T, DP>::TILE * kRowBytes), row, chunk & 7);
-}
+struct Image {
+  using D = Dim<T, DP>;
+  static __device__ __forceinline__ int tw(int row) { return D::CPB == 8 ? twist(row) : (row >> 2) & 3; }
+  static __device__ __forceinline__ const char* at(const char* img, int row, int chunk) {
+    return img + (chunk / D::CPB) * (D::TILE * D::PITCH) + row * D::PITCH + ((chunk % D::CPB) ^ tw(row)) * 16;
+  }
+  static __device__ __forceinline__ u32x4 row(const char* img, int r, int chunk) { return *reinterpret_cast<const u32x4*>(at(img, r, chunk)); }
+  // rows [2 KPF g + KPF h, + KPF) of column 32 t + (lane & 31)
+  static __device__ __forceinline__ u32x4 col(const char* img, int g, int t, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+      const int c = 32 * t + (lane & 31);
+      u32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t*>(at(img, 8 * g + 4 * h + j, c >> 2) + (c & 3) * 4);
+      return v;
+    } else {
+      const int j = lane & 15, c = 32 * t + (lane & 16) + 4 * (j & 3), k = 16 * g + 8 * h + (j >> 2), half = (c & 4) * 2;
+      const u32x2 lo = tr_read(at(img, k, c >> 3) + half), hi = tr_read(at(img, k + 4, c >> 3) + half);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+  }
+};
 
-// Staging of a tile of rows [r0, r0 + TILE) of one head into a row image and / or a transposed image.  Rows at or behind
-// `end`, and rows the key mask takes out (`keep` non-null), arrive as zeros: 0 * NaN must not reach a sum.
-template <class T, int DP, int NT>
-struct RowStage {
+// Fills images of tiles of one head.  Rows whose bit of `vis` is clear (behind the document's end, or taken out by the key
+// mask) and columns behind the head arrive as zeros: 0 * NaN must not reach a sum.
+template <class T, int DP, int WAVES>
+struct Filler {
   using D = Dim<T, DP>;
-  static constexpr int N = (D::TILE * D::CH + NT - 1) / NT;
-  u32x4 c[N];
-  __device__ __forceinline__ void load(const T* __restrict__ p, long long ld, int r0, int end, int Dh, int tid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int f = tid + i * NT, row = f / D::CH, ch = f % D::CH;
-      const bool ok = f < D::TILE * D::CH && r0 + row < end && ch * D::KPF < Dh;
-      c[i] = u32x4{0, 0, 0, 0};
-      if (ok) c[i] = *reinterpret_cast<const u32x4*>(p + (r0 + row) * ld + ch * D::KPF);
-    }
+  static constexpr int N = (D::GROUPS + WAVES - 1) / WAVES;
+  const char* p;      // the head's rows from the document's start
+  long long ld;       // bytes between rows
+  bool whole;         // the head fills its padded width
+
+  __device__ __forceinline__ void init(const void* base, long long token_stride, int Dh) {
+    p = static_cast<const char*>(base);
+    ld = token_stride * (long long)sizeof(T);
+    whole = Dh == DP;
   }
-  __device__ __forceinline__ void store(char* __restrict__ img, int tid) const {
+  __device__ __forceinline__ void operator()(char* __restrict__ img, int r0, unsigned long long vis, int Dh, int wave, int lane) const {
+    const char* __restrict__ src = p + r0 * ld;
+    const bool all = whole && vis == (D::TILE == 64 ? ~0ull : 0xffffffffull);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int f = tid + i * NT, row = f / D::CH, ch = f % D::CH;
-      if (f < D::TILE * D::CH)
-        *reinterpret_cast<u32x4*>(img + (ch >> 3) * (D::TILE * kRowBytes) + swz(row, ch & 7)) = c[i];
+      const int g = i * WAVES + wave;
+      if (D::GROUPS % WAVES != 0 && g >= D::GROUPS) break;
+      const int lin = g * D::RPG + lane / D::CPB, blk = lin / D::TILE, row = lin % D::TILE;
+      const int ch = blk * D::CPB + ((lane % D::CPB) ^ Image<T, DP>::tw(row));
+      const char* s = src + (uint32_t)(row * (uint32_t)ld) + ch * 16;
+      if (!all && !(((vis >> row) & 1) && ch * D::KPF < Dh)) s = reinterpret_cast<const char*>(kZeros);
+      lds_fill(s, img + g * 1024);
     }
   }
 };
-template <class T, int DP, int NT>
-struct ColStage {
-  using D = Dim<T, DP>;
-  static constexpr int U = 8 * (DP / 4), N = (U + NT - 1) / NT;  // units of KPF rows x 4 columns
-  KsUnit<T> u[N];
-  __device__ __forceinline__ void load(const T* __restrict__ p, long long ld, int r0, int end, int Dh,
-                                       const unsigned char* __restrict__ keep, int tid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int f = tid + i * NT, kg = f / (DP / 4), cq = f % (DP / 4);
-#pragma unroll
-      for (int j = 0; j < D::KPF; ++j) {
-        using V = decltype(u[i].v[0] + u[i].v[0]);
-        const int row = r0 + kg * D::KPF + j;
-        bool ok = f < U && row < end && 4 * cq < Dh;
-        if (keep && ok) ok = keep[row] != 0;
-        u[i].v[j] = V(0);
-        if (ok) u[i].v[j] = *reinterpret_cast<const V*>(p + row * ld + 4 * cq);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(char* __restrict__ img, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int f = tid + i * NT, kg = f / (DP / 4), cq = f % (DP / 4);
-      if (f < U) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(img + swz(4 * cq + j, kg)) = u[i].column(j);
-      }
-    }
-  }
-};
+
+// Which of the tile's rows [r0, r0 + TILE) hold keys: the document's length and the key mask, whose bytes (`kb`, one per
+// lane) were asked for a tile earlier.
+template <class T>
+__device__ __forceinline__ unsigned long long visible(int r0, int len, bool masked, unsigned kb, int lane) {
+  constexpr int TILE = kRowBytes / (int)sizeof(T);
+  if (masked) return __ballot(lane < TILE && r0 + lane < len && kb != 0);
+  const int n = len - r0;
+  return n >= TILE ? (TILE == 64 ? ~0ull : 0xffffffffull) : (n <= 0 ? 0ull : (1ull << n) - 1);
+}
+// this lane's 16 rows of accumulator tile t, as bits row_of(e, 0): `vis` and, where the query sees only the first `seen` rows, those
+template <class T>
+__device__ __forceinline__ uint32_t lane_bits(unsigned long long vis, int t, int seen, int h) {
+  uint32_t w = (uint32_t)(vis >> (32 * t));
+  const int n = seen - 32 * t;
+  w &= n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+  return w >> ((sizeof(T) == 2 ? 8 : 4) * h);
+}
 
 // this lane's fragments of ONE row (its column of the accumulator): chunks 2 g + h
 template <class T, int DP>
@@ -205,10 +199,11 @@ __device__ __forceinline__ void load_own(u32x4* __restrict__ f, const T* __restr
   }
 }
 
+// tanh(x r); 16-bit operands: 1 - 2 / (1 + exp 2 x r), good to 2^-22 absolute, +-1 far out
 template <class T>
-__device__ __forceinline__ float tanh_(float x) {
-  if constexpr (sizeof(T) == 4) return tanhf(x);
-  return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * x));  // +-1 far out
+__device__ __forceinline__ float tanh_(float x, float r) {
+  if constexpr (sizeof(T) == 4) return tanhf(x * r);
+  return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * kLog2e * r))), 1.f);
 }
 
 // Scores of one 32x32 tile, in place, from raw products: to units in which p = exp2(s * c - ...) with c = unit(a).  `d` gets
@@ -221,7 +216,7 @@ __device__ __forceinline__ void shape_scores(f32x16& s, f32x16& d, const Args& a
     const float r = a.scale / a.cap;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float t = tanh_<T>(s[i] * r);
+      const float t = tanh_<T>(s[i], r);
       s[i] = a.cap * t;
       if (GRAD) d[i] = fmaf(-t, t, 1.f);
     }
@@ -230,8 +225,9 @@ __device__ __forceinline__ void shape_scores(f32x16& s, f32x16& d, const Args& a
     for (int i = 0; i < 16; ++i) s[i] *= a.scale;
   }
   if (a.slopes) {
+    const float at = (float)(dist0 - (sizeof(T) == 2 ? 8 : 4) * h);  // exact: positions are below 2^24 apart
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope, fabsf((float)(dist0 - row_of<T>(i, h))), s[i]);
+    for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope, fabsf(at - (float)row_of<T>(i, 0)), s[i]);
   }
 }
 
@@ -243,11 +239,13 @@ __device__ __forceinline__ int key_end(const Args& a, int prefix, int i1, int le
 
 // ------------------------------------------------------------------------------------------------ forward
 template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void attention_fwd_kernel(Args a, int slots) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 4 : DP == 64 ? 3 : 2))) void attention_fwd_kernel(Args a, int slots) {
   using D = Dim<T, DP>;
-  constexpr int NT = 64 * WAVES, BM = 32 * WAVES;
-  __shared__ __align__(16) char kimg[D::ROWS];
-  __shared__ __align__(16) char vimg[D::COLS];
+  constexpr int BM = 32 * WAVES;
+  __shared__ __align__(16) char k0img[D::BYTES];
+  __shared__ __align__(16) char v0img[D::BYTES];
+  __shared__ __align__(16) char k1img[D::BYTES];
+  __shared__ __align__(16) char v1img[D::BYTES];
   const int id = xcd_tile(blockIdx.x, gridDim.x);
   const int head = id % a.H, slot = id / a.H;
   const Where w = locate(a.cu, a.docs, a.T, slot, BM);
@@ -286,82 +284,85 @@ __global__ __launch_bounds__(64 * WAVES) void attention_fwd_kernel(Args a, int s
     for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  RowStage<T, DP, NT> ks;
-  ColStage<T, DP, NT> vs;
-  ks.load(kp, a.kt, 0, w.len, a.Dh, tid);
-  vs.load(vp, a.vt, 0, w.len, a.Dh, keep, tid);
-  for (int k0 = 0; k0 < kend; k0 += D::TILE) {
-    ks.store(kimg, tid);
-    vs.store(vimg, tid);
-    __syncthreads();
+  Filler<T, DP, WAVES> fk, fv;
+  fk.init(kp, a.kt, a.Dh);
+  fv.init(vp, a.vt, a.Dh);
+  auto mask_byte = [&](int r0) -> unsigned { return keep && lane < D::TILE && r0 + lane < w.len ? keep[r0 + lane] : 0u; };
+  unsigned kb = mask_byte(0);
+  unsigned long long vis = visible<T>(0, w.len, keep, kb, lane);
+  fk(k0img, 0, vis, a.Dh, wave, lane);
+  fv(v0img, 0, vis, a.Dh, wave, lane);
+  kb = mask_byte(D::TILE);
+  const float jump = 8.f / c;  // a row's maximum is followed once it is 2^8 behind: sums stay exact enough, rescaling is rare
+
+  auto tile = [&](int k0, const char* __restrict__ kimg, const char* __restrict__ vimg, char* __restrict__ kn, char* __restrict__ vn) {
+    stage_wait();
+    const unsigned long long now = vis;
     if (k0 + D::TILE < kend) {
-      ks.load(kp, a.kt, k0 + D::TILE, w.len, a.Dh, tid);
-      vs.load(vp, a.vt, k0 + D::TILE, w.len, a.Dh, keep, tid);
+      vis = visible<T>(k0 + D::TILE, w.len, keep, kb, lane);
+      fk(kn, k0 + D::TILE, vis, a.Dh, wave, lane);
+      fv(vn, k0 + D::TILE, vis, a.Dh, wave, lane);
+      kb = mask_byte(k0 + 2 * D::TILE);
     }
-    if (k0 < wend && i0 + wave * 32 < w.len) {
-      f32x16 s[D::SUB];
-      const int rem = wend - k0;
+    if (k0 >= wend || i0 + wave * 32 >= w.len) return;
+    f32x16 s[D::SUB];
+    const int rem = wend - k0;
+    const bool masked = now != (D::TILE == 64 ? ~0ull : 0xffffffffull) ||
+                        (limited && k0 + D::TILE > i0 + wave * 32 + 1 && k0 + D::TILE > prefix);
+    float mx = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < D::SUB; ++t) {
-        f32x16 acc;
+    for (int t = 0; t < D::SUB; ++t) {
+      f32x16 acc;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+      for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+      if (32 * t < rem) {  // uniform: not the half of a tile that nobody here sees
 #pragma unroll
-        for (int g = 0; g < D::G; ++g) mma<T>(acc, head_frag<T, DP>(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
-        s[t] = acc;
-      }
-      unsigned long long vis = 0;
-      {
-        const int kk = k0 + lane;
-        bool v = kk < w.len && lane < D::TILE;
-        if (keep && v) v = keep[kk] != 0;
-        vis = __ballot(v);
-      }
-      const unsigned long long all = D::TILE == 64 ? ~0ull : 0xffffffffull;
-      const bool masked = vis != all || (limited && k0 + D::TILE > i0 + wave * 32 && k0 + D::TILE > prefix);
-      float mx = m;
-#pragma unroll
-      for (int t = 0; t < D::SUB; ++t) {
+        for (int g = 0; g < D::G; ++g) mma<T>(acc, Image<T, DP>::row(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
         f32x16 unused;
-        shape_scores<T, false>(s[t], unused, a, slope, i - (k0 + 32 * t), h);
+        shape_scores<T, false>(acc, unused, a, slope, i - (k0 + 32 * t), h);
         if (masked) {
+          const uint32_t bits = lane_bits<T>(now, t, seen - k0, h);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int kk = 32 * t + row_of<T>(e, h);
-            if (!((vis >> kk) & 1) || k0 + kk >= seen) s[t][e] = -INFINITY;
-          }
+          for (int e = 0; e < 16; ++e) acc[e] = bits & (1u << row_of<T>(e, 0)) ? acc[e] : -INFINITY;
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[e]);
       }
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mc = mx == -INFINITY ? 0.f : mx * c;
-      if (__any(mx > m)) {
-        const float f = __builtin_amdgcn_exp2f(fmaf(m, c, -mc));
-        l *= f;
+      s[t] = acc;
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    if (__any(mx > m + jump || m == -INFINITY)) {
+      mx = fmaxf(mx, m);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * c);
+      l *= f;
 #pragma unroll
-        for (int t = 0; t < D::DT; ++t)
+      for (int t = 0; t < D::DT; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[t][e] *= f;
-        m = mx;
+        for (int e = 0; e < 16; ++e) o[t][e] *= f;
+      m = mx;
+    }
+    const float mc = m == -INFINITY ? 0.f : m * c;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < D::SUB; ++t) {
+      if (32 * t >= rem) break;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -mc));
+        sum[e & 3] += s[t][e];
       }
 #pragma unroll
-      for (int t = 0; t < D::SUB; ++t)
+      for (int g = 0; g < D::PER; ++g) {
+        const u32x4 pf = acc_frag<T>(s[t], g);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -mc));
-          l += s[t][e];
-        }
-#pragma unroll
-      for (int g = 0; g < D::GT; ++g) {
-        constexpr int PER = D::GT / D::SUB;
-        if (32 * (g / PER) >= rem) break;  // uniform: the second half of a tile behind the last key
-        const u32x4 pf = acc_frag<T>(s[g / PER], g % PER);
-#pragma unroll
-        for (int t = 0; t < D::DT; ++t) mma<T>(o[t], row_frag(vimg, 32 * t + r, 2 * g + h), pf);
+        for (int u = 0; u < D::DT; ++u) mma<T>(o[u], Image<T, DP>::col(vimg, t * D::PER + g, u, lane), pf);
       }
     }
-    __syncthreads();
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  };
+  for (int k0 = 0; k0 < kend; k0 += 2 * D::TILE) {
+    tile(k0, k0img, v0img, k1img, v1img);
+    if (k0 + D::TILE < kend) tile(k0 + D::TILE, k1img, v1img, k0img, v0img);
   }
   l += __shfl_xor(l, 32, 64);
   if (!live) return;
@@ -380,12 +381,13 @@ __global__ __launch_bounds__(64 * WAVES) void attention_fwd_kernel(Args a, int s
 // ------------------------------------------------------------------------------------------------ dq, delta
 // dS = P (dO V^T - delta) d,  dq_i = scale sum_j dS_ij k_j,  delta_i = dO_i . o_i
 template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void attention_dq_kernel(Args a, int slots) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 3 : DP == 64 || sizeof(T) == 2 ? 2 : 1))) void attention_dq_kernel(Args a, int slots) {
   using D = Dim<T, DP>;
-  constexpr int NT = 64 * WAVES, BM = 32 * WAVES;
-  __shared__ __align__(16) char kimg[D::ROWS];
-  __shared__ __align__(16) char vimg[D::ROWS];
-  __shared__ __align__(16) char ktim[D::COLS];
+  constexpr int BM = 32 * WAVES;
+  __shared__ __align__(16) char k0img[D::BYTES];
+  __shared__ __align__(16) char v0img[D::BYTES];
+  __shared__ __align__(16) char k1img[D::BYTES];
+  __shared__ __align__(16) char v1img[D::BYTES];
   const int id = xcd_tile(blockIdx.x, gridDim.x);
   const int head = id % a.H, slot = id / a.H;
   const Where w = locate(a.cu, a.docs, a.T, slot, BM);
@@ -440,65 +442,60 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dq_kernel(Args a, int sl
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
 
-  RowStage<T, DP, NT> ks, vs;
-  ColStage<T, DP, NT> kc;
-  ks.load(kp, a.kt, 0, w.len, a.Dh, tid);
-  vs.load(vp, a.vt, 0, w.len, a.Dh, tid);
-  kc.load(kp, a.kt, 0, w.len, a.Dh, keep, tid);
-  for (int k0 = 0; k0 < kend; k0 += D::TILE) {
-    ks.store(kimg, tid);
-    vs.store(vimg, tid);
-    kc.store(ktim, tid);
-    __syncthreads();
+  Filler<T, DP, WAVES> fk, fv;
+  fk.init(kp, a.kt, a.Dh);
+  fv.init(vp, a.vt, a.Dh);
+  auto mask_byte = [&](int r0) -> unsigned { return keep && lane < D::TILE && r0 + lane < w.len ? keep[r0 + lane] : 0u; };
+  unsigned kb = mask_byte(0);
+  unsigned long long vis = visible<T>(0, w.len, keep, kb, lane);
+  fk(k0img, 0, vis, a.Dh, wave, lane);
+  fv(v0img, 0, vis, a.Dh, wave, lane);
+  kb = mask_byte(D::TILE);
+
+  auto tile = [&](int k0, const char* __restrict__ kimg, const char* __restrict__ vimg, char* __restrict__ kn, char* __restrict__ vn) {
+    stage_wait();
+    const unsigned long long now = vis;
     if (k0 + D::TILE < kend) {
-      ks.load(kp, a.kt, k0 + D::TILE, w.len, a.Dh, tid);
-      vs.load(vp, a.vt, k0 + D::TILE, w.len, a.Dh, tid);
-      kc.load(kp, a.kt, k0 + D::TILE, w.len, a.Dh, keep, tid);
+      vis = visible<T>(k0 + D::TILE, w.len, keep, kb, lane);
+      fk(kn, k0 + D::TILE, vis, a.Dh, wave, lane);
+      fv(vn, k0 + D::TILE, vis, a.Dh, wave, lane);
+      kb = mask_byte(k0 + 2 * D::TILE);
     }
-    if (k0 < wend && i0 + wave * 32 < w.len) {
-      const int kk0 = k0 + lane;
-      bool v = kk0 < w.len && lane < D::TILE;
-      if (keep && v) v = keep[kk0] != 0;
-      const unsigned long long vis = __ballot(v);
-      const unsigned long long all = D::TILE == 64 ? ~0ull : 0xffffffffull;
-      const bool masked = vis != all || (limited && k0 + D::TILE > i0 + wave * 32 && k0 + D::TILE > prefix);
-      const int rem = wend - k0;
+    if (k0 >= wend || i0 + wave * 32 >= w.len) return;
+    const bool masked = now != (D::TILE == 64 ? ~0ull : 0xffffffffull) ||
+                        (limited && k0 + D::TILE > i0 + wave * 32 + 1 && k0 + D::TILE > prefix);
+    const int rem = wend - k0;
 #pragma unroll
-      for (int t = 0; t < D::SUB; ++t) {
-        if (32 * t >= rem) break;
-        f32x16 s, dp, d;
+    for (int t = 0; t < D::SUB; ++t) {
+      if (32 * t >= rem) break;
+      f32x16 s, dp, d;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+      for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
 #pragma unroll
-        for (int g = 0; g < D::G; ++g) {
-          mma<T>(s, head_frag<T, DP>(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
-          mma<T>(dp, head_frag<T, DP>(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
-        }
-        shape_scores<T, true>(s, d, a, slope, i - (k0 + 32 * t), h);
+      for (int g = 0; g < D::G; ++g) {
+        mma<T>(s, Image<T, DP>::row(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
+        mma<T>(dp, Image<T, DP>::row(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
+      }
+      shape_scores<T, true>(s, d, a, slope, i - (k0 + 32 * t), h);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse2));
-          float ds = p * (dp[e] - delta);
-          if (a.cap > 0.f) ds *= d[e];
-          s[e] = ds;
-        }
-        if (masked) {
+      for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse2)) * (dp[e] - delta);
+      if (a.cap > 0.f) s *= d;
+      if (masked) {
+        const uint32_t bits = lane_bits<T>(now, t, seen - k0, h);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int kk = 32 * t + row_of<T>(e, h);
-            if (!((vis >> kk) & 1) || k0 + kk >= seen) s[e] = 0.f;
-          }
-        }
-        constexpr int PER = D::GT / D::SUB;
+        for (int e = 0; e < 16; ++e) s[e] = bits & (1u << row_of<T>(e, 0)) ? s[e] : 0.f;
+      }
 #pragma unroll
-        for (int g = 0; g < PER; ++g) {
-          const u32x4 f = acc_frag<T>(s, g);
+      for (int g = 0; g < D::PER; ++g) {
+        const u32x4 f = acc_frag<T>(s, g);
 #pragma unroll
-          for (int u = 0; u < D::DT; ++u) mma<T>(acc[u], row_frag(ktim, 32 * u + r, 2 * (t * PER + g) + h), f);
-        }
+        for (int u = 0; u < D::DT; ++u) mma<T>(acc[u], Image<T, DP>::col(kimg, t * D::PER + g, u, lane), f);
       }
     }
-    __syncthreads();
+  };
+  for (int k0 = 0; k0 < kend; k0 += 2 * D::TILE) {
+    tile(k0, k0img, v0img, k1img, v1img);
+    if (k0 + D::TILE < kend) tile(k0 + D::TILE, k1img, v1img, k0img, v0img);
   }
   if (!live) return;
 #pragma unroll
@@ -515,14 +512,15 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dq_kernel(Args a, int sl
 // A wave owns 32 keys (columns) and walks the queries, for every query head that shares the key head:
 // dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i
 template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void attention_dkv_kernel(Args a, int slots) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64 && sizeof(T) == 2 ? 2 : 1))) void attention_dkv_kernel(Args a, int slots) {
   using D = Dim<T, DP>;
-  constexpr int NT = 64 * WAVES, BM = 32 * WAVES;
-  __shared__ __align__(16) char qimg[D::ROWS];
-  __shared__ __align__(16) char dimg[D::ROWS];
-  __shared__ __align__(16) char qtim[D::COLS];
-  __shared__ __align__(16) char dtim[D::COLS];
-  __shared__ __align__(16) float stat[2][D::TILE];
+  constexpr int BM = 32 * WAVES;
+  __shared__ __align__(16) char q0img[D::BYTES];
+  __shared__ __align__(16) char d0img[D::BYTES];
+  __shared__ __align__(16) char q1img[D::BYTES];
+  __shared__ __align__(16) char d1img[D::BYTES];
+  __shared__ __align__(16) float stat0[2 * D::TILE];
+  __shared__ __align__(16) float stat1[2 * D::TILE];
   const int id = xcd_tile(blockIdx.x, gridDim.x);
   const int kvh = id % a.Hkv, slot = id / a.Hkv;
   const Where w = locate(a.cu, a.docs, a.T, slot, BM);
@@ -558,72 +556,89 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv_kernel(Args a, int s
 #pragma unroll
     for (int e = 0; e < 16; ++e) ak[t][e] = av[t][e] = 0.f;
 
-  for (int hq = 0; hq < rep; ++hq) {
-    const int head = kvh * rep + hq;
-    const T* __restrict__ qp = static_cast<const T*>(a.q) + w.start * a.qt + head * a.qh;
-    const T* __restrict__ dp_ = static_cast<const T*>(a.dout) + w.start * a.dot + head * a.doh;
-    const float* __restrict__ lse = a.lse + (long long)head * a.T + w.start;
-    const float* __restrict__ del = a.delta + (long long)head * a.T + w.start;
-    const float slope = a.slopes ? a.slopes[head] : 0.f;
-    for (int q0 = bfirst; q0 < w.len; q0 += D::TILE) {
-      {
-        RowStage<T, DP, NT> s;
-        s.load(qp, a.qt, q0, w.len, a.Dh, tid);
-        s.store(qimg, tid);
-        s.load(dp_, a.dot, q0, w.len, a.Dh, tid);
-        s.store(dimg, tid);
+  // tiles of queries, head after head of the group: one pipeline
+  const int per = bfirst < w.len ? (w.len - bfirst + D::TILE - 1) / D::TILE : 0, total = per * rep;
+  const char* const qb = static_cast<const char*>(a.q) + (w.start * a.qt + (long long)kvh * rep * a.qh) * (long long)sizeof(T);
+  const char* const db = static_cast<const char*>(a.dout) + (w.start * a.dot + (long long)kvh * rep * a.doh) * (long long)sizeof(T);
+  float st[2];  // lse and delta of query (tid) of the tile being filled
+  auto issue = [&](int n, char* __restrict__ qi, char* __restrict__ di) {
+    const int hq = n / per, q0 = bfirst + (n - hq * per) * D::TILE;
+    const unsigned long long vis = visible<T>(q0, w.len, false, 0, lane);
+    Filler<T, DP, WAVES> f;
+    f.init(qb + hq * a.qh * (long long)sizeof(T), a.qt, a.Dh);
+    f(qi, q0, vis, a.Dh, wave, lane);
+    f.init(db + hq * a.doh * (long long)sizeof(T), a.dot, a.Dh);
+    f(di, q0, vis, a.Dh, wave, lane);
+    st[0] = -INFINITY;
+    st[1] = 0.f;
+    if (tid < D::TILE && q0 + tid < w.len) {
+      const long long at = (long long)(kvh * rep + hq) * a.T + w.start + q0 + tid;
+      st[0] = a.lse[at];
+      st[1] = a.delta[at];
+    }
+  };
+  auto put = [&](float* __restrict__ s) {  // before the barrier that publishes the tile
+    if (tid < D::TILE) {
+      s[tid] = st[0] == -INFINITY ? INFINITY : st[0] * kLog2e;  // a row that sees nothing, or none: p = 0
+      s[D::TILE + tid] = st[1];
+    }
+  };
+  auto tile = [&](int n, const char* __restrict__ qimg, const char* __restrict__ dimg, float* __restrict__ stat,
+                  char* __restrict__ qn, char* __restrict__ dn) {
+    put(stat);
+    stage_wait();
+    if (n + 1 < total) issue(n + 1, qn, dn);
+    const int hq = n / per, q0 = bfirst + (n - hq * per) * D::TILE;
+    if (q0 + D::TILE <= wfirst || j0 + wave * 32 >= w.len) return;
+    const float slope = a.slopes ? a.slopes[kvh * rep + hq] : 0.f;
+    const bool masked = limited && q0 < j0 + wave * 32 + 31 && j0 + wave * 32 + 31 >= prefix;
+#pragma unroll
+    for (int t = 0; t < D::SUB; ++t) {
+      if (q0 + 32 * t >= w.len) break;
+      f32x16 s, dp, d;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+      for (int g = 0; g < D::G; ++g) {
+        mma<T>(s, Image<T, DP>::row(qimg, 32 * t + fold<T>(r), 2 * g + h), kf[g]);
+        mma<T>(dp, Image<T, DP>::row(dimg, 32 * t + fold<T>(r), 2 * g + h), vf[g]);
       }
-      {
-        ColStage<T, DP, NT> s;
-        s.load(qp, a.qt, q0, w.len, a.Dh, nullptr, tid);
-        s.store(qtim, tid);
-        s.load(dp_, a.dot, q0, w.len, a.Dh, nullptr, tid);
-        s.store(dtim, tid);
+      shape_scores<T, true>(s, d, a, slope, j - (q0 + 32 * t), h);
+      f32x16 ls, de;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        ls[e] = stat[32 * t + row_of<T>(e, h)];
+        de[e] = stat[D::TILE + 32 * t + row_of<T>(e, h)];
       }
-      if (tid < D::TILE) {
-        const float t = q0 + tid < w.len ? lse[q0 + tid] : -INFINITY;
-        stat[0][tid] = t == -INFINITY ? INFINITY : t * kLog2e;  // a row that sees nothing, or none: p = 0
-        stat[1][tid] = q0 + tid < w.len ? del[q0 + tid] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -ls[e]));
+        dp[e] = s[e] * (dp[e] - de[e]);
       }
-      __syncthreads();
-      if (q0 + D::TILE > wfirst && j0 + wave * 32 < w.len) {
-        const bool masked = limited && q0 < j0 + wave * 32 + 31 && j0 + wave * 32 + 31 >= prefix;
+      if (a.cap > 0.f) dp *= d;
+      if (masked) {
 #pragma unroll
-        for (int t = 0; t < D::SUB; ++t) {
-          if (q0 + 32 * t >= w.len) break;
-          f32x16 s, dp, d;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-#pragma unroll
-          for (int g = 0; g < D::G; ++g) {
-            mma<T>(s, head_frag<T, DP>(qimg, 32 * t + fold<T>(r), 2 * g + h), kf[g]);
-            mma<T>(dp, head_frag<T, DP>(dimg, 32 * t + fold<T>(r), 2 * g + h), vf[g]);
-          }
-          shape_scores<T, true>(s, d, a, slope, j - (q0 + 32 * t), h);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int qq = 32 * t + row_of<T>(e, h);
-            float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, -stat[0][qq]));
-            if (masked && q0 + qq < first) p = 0.f;
-            float ds = p * (dp[e] - stat[1][qq]);
-            if (a.cap > 0.f) ds *= d[e];
-            s[e] = p;
-            dp[e] = ds;
-          }
-          constexpr int PER = D::GT / D::SUB;
-#pragma unroll
-          for (int g = 0; g < PER; ++g) {
-            const u32x4 pf = acc_frag<T>(s, g), sf = acc_frag<T>(dp, g);
-#pragma unroll
-            for (int u = 0; u < D::DT; ++u) {
-              mma<T>(av[u], row_frag(dtim, 32 * u + r, 2 * (t * PER + g) + h), pf);
-              mma<T>(ak[u], row_frag(qtim, 32 * u + r, 2 * (t * PER + g) + h), sf);
-            }
-          }
+        for (int e = 0; e < 16; ++e) {
+          const bool sees = q0 + 32 * t + row_of<T>(e, h) >= first;
+          s[e] = sees ? s[e] : 0.f;
+          dp[e] = sees ? dp[e] : 0.f;
         }
       }
-      __syncthreads();
+#pragma unroll
+      for (int g = 0; g < D::PER; ++g) {
+        const u32x4 pf = acc_frag<T>(s, g), sf = acc_frag<T>(dp, g);
+#pragma unroll
+        for (int u = 0; u < D::DT; ++u) {
+          mma<T>(av[u], Image<T, DP>::col(dimg, t * D::PER + g, u, lane), pf);
+          mma<T>(ak[u], Image<T, DP>::col(qimg, t * D::PER + g, u, lane), sf);
+        }
+      }
     }
+  };
+  if (total > 0) issue(0, q0img, d0img);
+  for (int n = 0; n < total; n += 2) {
+    tile(n, q0img, d0img, stat0, q1img, d1img);
+    if (n + 1 < total) tile(n + 1, q1img, d1img, stat1, q0img, d0img);
   }
   if (!in) return;
 #pragma unroll
@@ -690,7 +705,9 @@ int with_shape(int dtype, int Dh, F&& f) {
 bool view_ok(const tt_head_view& v, int width, bool required) {
   if (!v.data) return !required;
   const int kpf = 16 / width;
-  return tt_aligned16(v.data) && v.token_stride % kpf == 0 && v.head_stride % kpf == 0;
+  // (the last bound keeps a tile's 32-bit offsets in range)
+  return tt_aligned16(v.data) && v.token_stride % kpf == 0 && v.head_stride % kpf == 0 && v.token_stride >= 0 &&
+         v.token_stride < (1 << 22);
 }
 
 int check(const tt_attention_args* p) {

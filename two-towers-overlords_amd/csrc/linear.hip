@@ -81,40 +81,88 @@ struct FwdArgs {
   int act, vec, gn;  // gn: tiles along N
 };
 
+// The pre-activation as it is kept: a positive z below fp16's range must not become 0, relu'(z) is 1 there.
+template <class T>
+__device__ __forceinline__ f32x4 kept(f32x4 v, int act) {
+  if (__is_same(T, _Float16) && act == TT_ACT_RELU) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = v[c] > 0.f ? fmaxf(v[c], 5.9604645e-8f) : v[c];
+  }
+  return v;
+}
+
+// whole quads, aligned: the loads of an accumulator row are issued together
+template <class T, int ACT, class B>
+__device__ __forceinline__ void epilogue(B& blk, const FwdArgs& a, int m0, int n0) {
+  typedef typename Type<T>::quad quad;
+  const T* __restrict__ bias = static_cast<const T*>(a.bias);
+  const int N = a.s.N, nb = n0 + blk.wn * B::NI * 32 + 4 * blk.h;
+  quad bq[B::NI][4];
+#pragma unroll
+  for (int i = 0; i < B::NI; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = nb + 32 * i + 8 * q;
+      bq[i][q] = quad(0);
+      if (bias && n < N) bq[i][q] = *reinterpret_cast<const quad*>(bias + n);
+    }
+#pragma unroll
+  for (int j = 0; j < B::MJ; ++j) {
+    const int m = m0 + (blk.wm * B::MJ + j) * 32 + blk.r;
+    const bool row = m < a.s.M;
+    const T* __restrict__ res = static_cast<const T*>(a.res) + m * a.ldr + nb;
+    T* __restrict__ y = static_cast<T*>(a.y) + m * a.ldy + nb;
+    T* __restrict__ z = static_cast<T*>(a.z) + (long long)m * N + nb;
+    quad rq[B::NI][4];
+    if (a.res) {
+#pragma unroll
+      for (int i = 0; i < B::NI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          rq[i][q] = quad(0);
+          if (row && nb + 32 * i + 8 * q < N) rq[i][q] = *reinterpret_cast<const quad*>(res + 32 * i + 8 * q);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < B::NI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool in = row && nb + 32 * i + 8 * q < N;
+        f32x4 v = from_quad<T>(bq[i][q]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] += blk.acc[i][j][4 * q + c];
+        if (a.z && in) *reinterpret_cast<quad*>(z + 32 * i + 8 * q) = to_quad<T>(kept<T>(v, ACT));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = act_<ACT, sizeof(T) == 2>(v[c]);
+        if (a.res) v += from_quad<T>(rq[i][q]);
+        if (in) *reinterpret_cast<quad*>(y + 32 * i + 8 * q) = to_quad<T>(v);
+      }
+  }
+}
+
 template <class T, class B>
-__global__ __launch_bounds__(B::THREADS) void linear_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void linear_fwd_kernel(FwdArgs a) {
   __shared__ __align__(16) char b0[B::BYTES];
   __shared__ __align__(16) char b1[B::BYTES];
   const int t = xcd_tile(blockIdx.x, gridDim.x);
   const int m0 = t / a.gn * B::BM, n0 = t % a.gn * B::BN;
   B blk;
   blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
-  const T* __restrict__ bias = static_cast<const T*>(a.bias);
-  const T* __restrict__ res = static_cast<const T*>(a.res);
-  T* __restrict__ y = static_cast<T*>(a.y);
-  T* __restrict__ z = static_cast<T*>(a.z);
-  const int M = a.s.M, N = a.s.N;
-  const bool vec = a.vec;
-  with_act(a.act, [&](auto tag) {
-    constexpr int ACT = decltype(tag)::value;
+  if (!a.vec) {  // columns or strides that are not whole quads: element by element
+    T* __restrict__ z = static_cast<T*>(a.z);
     blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
-      if (m >= M) return;
-      if (bias) v += load_quad<T>(bias, 0, 0, n, N, vec);
-      if (z) {
-        f32x4 k = v;
-        if constexpr (ACT == TT_ACT_RELU && __is_same(T, _Float16)) {
-          // a positive z below fp16's range must not be kept as 0: relu'(z) is 1 there
-#pragma unroll
-          for (int c = 0; c < 4; ++c) k[c] = v[c] > 0.f ? fmaxf(v[c], 5.9604645e-8f) : v[c];
-        }
-        store_quad<T>(z, N, m, n, N, vec, k);
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = act_<ACT, sizeof(T) == 2>(v[c]);
-      if (res) v += load_quad<T>(res, a.ldr, m, n, N, vec);
-      store_quad<T>(y, a.ldy, m, n, N, vec, v);
+      if (m >= a.s.M || n >= a.s.N) return;
+      if (a.bias) v += load_quad<T>(static_cast<const T*>(a.bias), 0, 0, n, a.s.N, false);
+      if (z) store_quad<T>(z, a.s.N, m, n, a.s.N, false, kept<T>(v, a.act));
+      with_act(a.act, [&](auto tag) {
+        for (int c = 0; c < 4; ++c) v[c] = act_<decltype(tag)::value, sizeof(T) == 2>(v[c]);
+      });
+      if (a.res) v += load_quad<T>(static_cast<const T*>(a.res), a.ldr, m, n, a.s.N, false);
+      store_quad<T>(static_cast<T*>(a.y), a.ldy, m, n, a.s.N, false, v);
     });
-  });
+    return;
+  }
+  with_act(a.act, [&](auto tag) { epilogue<T, decltype(tag)::value>(blk, a, m0, n0); });
 }
 
 // dz = dy act'(z) (written when dz != null, row stride ldz) and, per block of rows, the column sums of dz.
@@ -193,7 +241,7 @@ struct GradArgs {
   int gm, gn, vec;
 };
 template <class T, bool XKS, class B>
-__global__ __launch_bounds__(B::THREADS) void grad_product_kernel(GradArgs a) {
+__global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void grad_product_kernel(GradArgs a) {
   __shared__ __align__(16) char b0[B::BYTES];
   __shared__ __align__(16) char b1[B::BYTES];
   const int tiles = a.gm * a.gn;

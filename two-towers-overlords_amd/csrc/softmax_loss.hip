@@ -42,7 +42,7 @@ __device__ __forceinline__ bool left_out(const Args& a, int j, long long t, long
 }
 
 template <class T, class B>
-__global__ __launch_bounds__(B::THREADS) void softmax_lse_kernel(Args a) {
+__global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void softmax_lse_kernel(Args a) {
   __shared__ __align__(16) char b0[B::BYTES];
   __shared__ __align__(16) char b1[B::BYTES];
   constexpr int NI = B::NI, MJ = B::MJ;
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restr
 
 // G of a piece of the candidates, [M, ldg] in T; columns behind the last candidate are zero
 template <class T, class B>
-__global__ __launch_bounds__(B::THREADS) void softmax_grad_kernel(Args a) {
+__global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void softmax_grad_kernel(Args a) {
   __shared__ __align__(16) char b0[B::BYTES];
   __shared__ __align__(16) char b1[B::BYTES];
   constexpr int NI = B::NI, MJ = B::MJ;
