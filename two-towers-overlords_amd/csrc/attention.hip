@@ -206,29 +206,42 @@ __device__ __forceinline__ float tanh_(float x, float r) {
   return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * kLog2e * r))), 1.f);
 }
 
-// Scores of one 32x32 tile, in place, from raw products: to units in which p = exp2(s * c - ...) with c = unit(a).  `d` gets
-// d s / d (scale q.k), needed by the backward pass only.  dist0 = (query position) - (position of the tile's row 0) for
-// tiles whose rows are keys; its negative serves tiles whose rows are queries.
+// Scores of one 32x32 tile from raw products, in units in which p = exp2(s * c - ...) with c = unit(a): capped (or, where only
+// a distance bias follows, scaled), then the bias.  dist0 = (query position) - (position of the tile's row 0) for tiles
+// whose rows are keys; its negative serves tiles whose rows are queries.  By value: references kept these in scratch memory.
 __device__ __forceinline__ float unit(const Args& a) { return (a.cap > 0.f || a.slopes) ? kLog2e : a.scale * kLog2e; }
-template <class T, bool GRAD>
-__device__ __forceinline__ void shape_scores(f32x16& s, f32x16& d, const Args& a, float slope, int dist0, int h) {
+template <class T>
+__device__ __forceinline__ f32x16 capped(f32x16 s, const Args& a) {
   if (a.cap > 0.f) {
     const float r = a.scale / a.cap;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float t = tanh_<T>(s[i], r);
-      s[i] = a.cap * t;
-      if (GRAD) d[i] = fmaf(-t, t, 1.f);
-    }
+    for (int i = 0; i < 16; ++i) s[i] = a.cap * tanh_<T>(s[i], r);
   } else if (a.slopes) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] *= a.scale;
   }
+  return s;
+}
+template <class T>
+__device__ __forceinline__ f32x16 biased(f32x16 s, const Args& a, float slope, int dist0, int h) {
   if (a.slopes) {
     const float at = (float)(dist0 - (sizeof(T) == 2 ? 8 : 4) * h);  // exact: positions are below 2^24 apart
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope, fabsf(at - (float)row_of<T>(i, 0)), s[i]);
   }
+  return s;
+}
+// d x capped score / d (scale q.k) = x (1 - (score / cap)^2)
+__device__ __forceinline__ f32x16 through_cap(f32x16 x, f32x16 s, const Args& a) {
+  if (a.cap > 0.f) {
+    const float r = 1.f / a.cap;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float t = s[i] * r;
+      x[i] *= fmaf(-t, t, 1.f);
+    }
+  }
+  return x;
 }
 
 // number of keys (from the document's start) that some query of [i0, i1) sees, and the first from which masking is needed
@@ -318,8 +331,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
       if (32 * t < rem) {  // uniform: not the half of a tile that nobody here sees
 #pragma unroll
         for (int g = 0; g < D::G; ++g) mma<T>(acc, Image<T, DP>::row(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
-        f32x16 unused;
-        shape_scores<T, false>(acc, unused, a, slope, i - (k0 + 32 * t), h);
+        acc = biased<T>(capped<T>(acc, a), a, slope, i - (k0 + 32 * t), h);
         if (masked) {
           const uint32_t bits = lane_bits<T>(now, t, seen - k0, h);
 #pragma unroll
@@ -468,7 +480,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 #pragma unroll
     for (int t = 0; t < D::SUB; ++t) {
       if (32 * t >= rem) break;
-      f32x16 s, dp, d;
+      f32x16 s, dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
 #pragma unroll
@@ -476,10 +488,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         mma<T>(s, Image<T, DP>::row(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
         mma<T>(dp, Image<T, DP>::row(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
       }
-      shape_scores<T, true>(s, d, a, slope, i - (k0 + 32 * t), h);
+      const f32x16 sc = capped<T>(s, a);
+      s = biased<T>(sc, a, slope, i - (k0 + 32 * t), h);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse2)) * (dp[e] - delta);
-      if (a.cap > 0.f) s *= d;
+      s = through_cap(s, sc, a);
       if (masked) {
         const uint32_t bits = lane_bits<T>(now, t, seen - k0, h);
 #pragma unroll
@@ -512,7 +525,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 // A wave owns 32 keys (columns) and walks the queries, for every query head that shares the key head:
 // dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i
 template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? (sizeof(T) == 2 ? 3 : 2) : DP == 64 && sizeof(T) == 2 ? 2 : 1))) void attention_dkv_kernel(Args a, int slots) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 2 : DP == 64 && sizeof(T) == 2 ? 2 : 1))) void attention_dkv_kernel(Args a, int slots) {
   using D = Dim<T, DP>;
   constexpr int BM = 32 * WAVES;
   __shared__ __align__(16) char q0img[D::BYTES];
@@ -595,7 +608,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 #pragma unroll
     for (int t = 0; t < D::SUB; ++t) {
       if (q0 + 32 * t >= w.len) break;
-      f32x16 s, dp, d;
+      f32x16 s, dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
 #pragma unroll
@@ -603,7 +616,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         mma<T>(s, Image<T, DP>::row(qimg, 32 * t + fold<T>(r), 2 * g + h), kf[g]);
         mma<T>(dp, Image<T, DP>::row(dimg, 32 * t + fold<T>(r), 2 * g + h), vf[g]);
       }
-      shape_scores<T, true>(s, d, a, slope, j - (q0 + 32 * t), h);
+      const f32x16 sc = capped<T>(s, a);
+      s = biased<T>(sc, a, slope, j - (q0 + 32 * t), h);
       f32x16 ls, de;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -615,7 +629,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -ls[e]));
         dp[e] = s[e] * (dp[e] - de[e]);
       }
-      if (a.cap > 0.f) dp *= d;
+      dp = through_cap(dp, sc, a);
       if (masked) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
