@@ -34,9 +34,20 @@ struct Args {
   const int *cu, *prefix;
   const float* slopes;
   const unsigned char* keep;
-  int T, docs, H, Hkv, Dh, causal;
+  int T, docs, H, Hkv, Dh, causal, spread;
   float scale, cap;
 };
+
+// Head and tile slot of this workgroup.  Short documents: consecutive slots, all heads of each, on one XCD, whose L2 then holds
+// the rows they share.  Long ones (spread): neighbours go round the XCDs, which evens out documents of different lengths and
+// the triangle of a causal mask; `last_first`: the tiles with the longest rows of keys first.
+__device__ __forceinline__ void place(const Args& a, int heads, bool last_first, int& head, int& slot) {
+  int id = blockIdx.x;
+  if (!a.spread) id = xcd_tile(id, gridDim.x);
+  else if (last_first) id = gridDim.x - 1 - id;
+  head = id % heads;
+  slot = id / heads;
+}
 
 struct Where {
   int doc, start, len, tile;
@@ -199,37 +210,82 @@ __device__ __forceinline__ void load_own(u32x4* __restrict__ f, const T* __restr
   }
 }
 
-// tanh(x r); 16-bit operands: 1 - 2 / (1 + exp 2 x r), good to 2^-22 absolute, +-1 far out
-template <class T>
-__device__ __forceinline__ float tanh_(float x, float r) {
-  if constexpr (sizeof(T) == 4) return tanhf(x * r);
-  return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * kLog2e * r))), 1.f);
+// Scores from raw products, in units in which p = exp2(s * c - ...): raw products where there is no cap (c = scale log2 e, the
+// bias's slope divided by the scale), natural units behind a cap.  By value: references kept these in scratch memory.
+struct Units {
+  float c, slope;
+};
+__device__ __forceinline__ Units units(const Args& a, int head) {
+  Units u;
+  const float slope = a.slopes ? a.slopes[head] : 0.f;
+  u.c = a.cap > 0.f ? kLog2e : a.scale * kLog2e;
+  u.slope = a.cap > 0.f ? slope : slope / a.scale;
+  return u;
 }
-
-// Scores of one 32x32 tile from raw products, in units in which p = exp2(s * c - ...) with c = unit(a): capped (or, where only
-// a distance bias follows, scaled), then the bias.  dist0 = (query position) - (position of the tile's row 0) for tiles
-// whose rows are keys; its negative serves tiles whose rows are queries.  By value: references kept these in scratch memory.
-__device__ __forceinline__ float unit(const Args& a) { return (a.cap > 0.f || a.slopes) ? kLog2e : a.scale * kLog2e; }
+// cap tanh(s scale / cap).  16-bit operands: where no score of the tile is beyond 0.35 cap, the series to x^9 (the next term is
+// below 10^-7); else 1 - 2 / (1 + exp 2x), good to 2^-22 absolute and +-1 far out.  float: the accurate function.
 template <class T>
 __device__ __forceinline__ f32x16 capped(f32x16 s, const Args& a) {
-  if (a.cap > 0.f) {
-    const float r = a.scale / a.cap;
+  if (!(a.cap > 0.f)) return s;
+  const float r = a.scale / a.cap;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = a.cap * tanh_<T>(s[i], r);
-  } else if (a.slopes) {
+    for (int i = 0; i < 16; ++i) s[i] = a.cap * tanhf(s[i] * r);
+    return s;
+  }
+  float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] *= a.scale;
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(s[i]));
+  if (!__any(top * r > 0.35f)) {
+    const float r2 = r * r, k9 = 62.f / 2835.f * r2 * r2 * r2 * r2 * a.scale, k7 = -17.f / 315.f * r2 * r2 * r2 * a.scale,
+                k5 = 2.f / 15.f * r2 * r2 * a.scale, k3 = -1.f / 3.f * r2 * a.scale;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float u = s[i] * s[i];
+      s[i] *= fmaf(u, fmaf(u, fmaf(u, fmaf(u, k9, k7), k5), k3), a.scale);
+    }
+  } else {
+    const float e2 = 2.f * kLog2e * r;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      s[i] = fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[i] * e2)), a.cap);
   }
   return s;
 }
+// The distance bias of accumulator tile t, -slope |at - row| with row = 32 t + row_of(e, 0) and `at` the lane's own position
+// less the tile's (and the lane half's rows).  side > 0 / < 0: the whole tile lies on one side of the wave's own positions, and
+// the bias is linear: the part that depends on the row is added here, the lane's own part (`own`) is left to the exponent.
+struct Bias {
+  float slope, at, own;
+  int side;
+};
 template <class T>
-__device__ __forceinline__ f32x16 biased(f32x16 s, const Args& a, float slope, int dist0, int h) {
+__device__ __forceinline__ Bias bias_of(const Args& a, const Units& u, int first, int pos, int r0, int h) {  // first: the wave's first position
+  Bias b{u.slope, 0.f, 0.f, 2};
   if (a.slopes) {
-    const float at = (float)(dist0 - (sizeof(T) == 2 ? 8 : 4) * h);  // exact: positions are below 2^24 apart
+    b.at = (float)(pos - r0 - (sizeof(T) == 2 ? 8 : 4) * h);  // exact: positions are below 2^24 apart
+    b.side = first >= r0 + kRowBytes / (int)sizeof(T) - 1 ? 1 : (first + 31 <= r0 ? -1 : 0);
+    if (b.side) b.own = -(float)b.side * b.slope * b.at;
+  }
+  return b;
+}
+template <class T>
+__device__ __forceinline__ f32x16 biased(f32x16 s, const Bias& b, int t) {
+  if (b.side == 2) return s;
+  if (b.side) {
+    const float k = b.side > 0 ? b.slope : -b.slope;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope, fabsf(at - (float)row_of<T>(i, 0)), s[i]);
+    for (int i = 0; i < 16; ++i) s[i] = fmaf(k, (float)(32 * t + row_of<T>(i, 0)), s[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = fmaf(-b.slope, fabsf(b.at - (float)(32 * t + row_of<T>(i, 0))), s[i]);
   }
   return s;
+}
+// x where bit `bit` of w is set, else `other` (two instructions, no condition code)
+__device__ __forceinline__ float pick(uint32_t w, int bit, float x, float other) {
+  const int m = (int)(w << (31 - bit)) >> 31;
+  return __builtin_bit_cast(float, (__builtin_bit_cast(int, x) & m) | (__builtin_bit_cast(int, other) & ~m));
 }
 // d x capped score / d (scale q.k) = x (1 - (score / cap)^2)
 __device__ __forceinline__ f32x16 through_cap(f32x16 x, f32x16 s, const Args& a) {
@@ -259,8 +315,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   __shared__ __align__(16) char v0img[D::BYTES];
   __shared__ __align__(16) char k1img[D::BYTES];
   __shared__ __align__(16) char v1img[D::BYTES];
-  const int id = xcd_tile(blockIdx.x, gridDim.x);
-  const int head = id % a.H, slot = id / a.H;
+  int head, slot;
+  place(a, a.H, true, head, slot);
   const Where w = locate(a.cu, a.docs, a.T, slot, BM);
   const int i0 = w.tile * BM;
   if (i0 < 0 || i0 >= w.len) return;
@@ -285,8 +341,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   const int kend = key_end(a, prefix, min(i0 + BM, w.len), w.len);
   const int wend = key_end(a, prefix, min(i0 + wave * 32 + 32, w.len), w.len);  // this wave's own end
   const int seen = limited ? max(i + 1, prefix) : w.len;                       // this query's
-  const float slope = a.slopes ? a.slopes[head] : 0.f;
-  const float c = unit(a);
+  const Units un = units(a, head);
+  const float c = un.c;
 
   u32x4 qf[D::G];
   load_own<T, DP>(qf, static_cast<const T*>(a.q) + tok * a.qt + head * a.qh, live, a.Dh, h);
@@ -322,6 +378,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     const int rem = wend - k0;
     const bool masked = now != (D::TILE == 64 ? ~0ull : 0xffffffffull) ||
                         (limited && k0 + D::TILE > i0 + wave * 32 + 1 && k0 + D::TILE > prefix);
+    const Bias bias = bias_of<T>(a, un, i0 + wave * 32, i, k0, h);
     float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < D::SUB; ++t) {
@@ -331,17 +388,18 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
       if (32 * t < rem) {  // uniform: not the half of a tile that nobody here sees
 #pragma unroll
         for (int g = 0; g < D::G; ++g) mma<T>(acc, Image<T, DP>::row(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
-        acc = biased<T>(capped<T>(acc, a), a, slope, i - (k0 + 32 * t), h);
+        acc = biased<T>(capped<T>(acc, a), bias, t);
         if (masked) {
           const uint32_t bits = lane_bits<T>(now, t, seen - k0, h);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[e] = bits & (1u << row_of<T>(e, 0)) ? acc[e] : -INFINITY;
+          for (int e = 0; e < 16; ++e) acc[e] = pick(bits, row_of<T>(e, 0), acc[e], -INFINITY);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[e]);
       }
       s[t] = acc;
     }
+    mx += bias.own;  // the lane halves' own parts differ by their rows
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     if (__any(mx > m + jump || m == -INFINITY)) {
       mx = fmaxf(mx, m);
@@ -353,14 +411,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         for (int e = 0; e < 16; ++e) o[t][e] *= f;
       m = mx;
     }
-    const float mc = m == -INFINITY ? 0.f : m * c;
+    const float mc = fmaf(bias.own, c, m == -INFINITY ? 0.f : -m * c);
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < D::SUB; ++t) {
       if (32 * t >= rem) break;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, -mc));
+        s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, mc));
         sum[e & 3] += s[t][e];
       }
 #pragma unroll
@@ -400,8 +458,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   __shared__ __align__(16) char v0img[D::BYTES];
   __shared__ __align__(16) char k1img[D::BYTES];
   __shared__ __align__(16) char v1img[D::BYTES];
-  const int id = xcd_tile(blockIdx.x, gridDim.x);
-  const int head = id % a.H, slot = id / a.H;
+  int head, slot;
+  place(a, a.H, true, head, slot);
   const Where w = locate(a.cu, a.docs, a.T, slot, BM);
   const int i0 = w.tile * BM;
   if (i0 < 0 || i0 >= w.len) return;
@@ -424,8 +482,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   const int kend = key_end(a, prefix, min(i0 + BM, w.len), w.len);
   const int wend = key_end(a, prefix, min(i0 + wave * 32 + 32, w.len), w.len);
   const int seen = limited ? max(i + 1, prefix) : w.len;
-  const float slope = a.slopes ? a.slopes[head] : 0.f;
-  const float c = unit(a);
+  const Units un = units(a, head);
+  const float c = un.c;
 
   u32x4 qf[D::G], df[D::G];
   load_own<T, DP>(qf, static_cast<const T*>(a.q) + tok * a.qt + head * a.qh, live, a.Dh, h);
@@ -477,6 +535,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     const bool masked = now != (D::TILE == 64 ? ~0ull : 0xffffffffull) ||
                         (limited && k0 + D::TILE > i0 + wave * 32 + 1 && k0 + D::TILE > prefix);
     const int rem = wend - k0;
+    const Bias bias = bias_of<T>(a, un, i0 + wave * 32, i, k0, h);
+    const float off = fmaf(bias.own, c, -lse2);
 #pragma unroll
     for (int t = 0; t < D::SUB; ++t) {
       if (32 * t >= rem) break;
@@ -489,14 +549,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         mma<T>(dp, Image<T, DP>::row(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
       }
       const f32x16 sc = capped<T>(s, a);
-      s = biased<T>(sc, a, slope, i - (k0 + 32 * t), h);
+      s = biased<T>(sc, bias, t);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse2)) * (dp[e] - delta);
+      for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, off)) * (dp[e] - delta);
       s = through_cap(s, sc, a);
       if (masked) {
         const uint32_t bits = lane_bits<T>(now, t, seen - k0, h);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = bits & (1u << row_of<T>(e, 0)) ? s[e] : 0.f;
+        for (int e = 0; e < 16; ++e) s[e] = pick(bits, row_of<T>(e, 0), s[e], 0.f);
       }
 #pragma unroll
       for (int g = 0; g < D::PER; ++g) {
@@ -534,8 +594,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   __shared__ __align__(16) char d1img[D::BYTES];
   __shared__ __align__(16) float stat0[2 * D::TILE];
   __shared__ __align__(16) float stat1[2 * D::TILE];
-  const int id = xcd_tile(blockIdx.x, gridDim.x);
-  const int kvh = id % a.Hkv, slot = id / a.Hkv;
+  int kvh, slot;
+  place(a, a.Hkv, false, kvh, slot);
   const Where w = locate(a.cu, a.docs, a.T, slot, BM);
   const int j0 = w.tile * BM;
   if (j0 < 0 || j0 >= w.len) return;
@@ -558,7 +618,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   const int first = !limited || j < prefix ? 0 : j;
   const int wfirst = !limited || j0 + wave * 32 < prefix ? 0 : j0 + wave * 32;
   const int bfirst = (!limited || j0 < prefix ? 0 : j0) / D::TILE * D::TILE;
-  const float c = unit(a);
+  const float c = units(a, 0).c;
 
   u32x4 kf[D::G], vf[D::G];
   load_own<T, DP>(kf, static_cast<const T*>(a.k) + tok * a.kt + kvh * a.kh, live, a.Dh, h);
@@ -603,7 +663,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     if (n + 1 < total) issue(n + 1, qn, dn);
     const int hq = n / per, q0 = bfirst + (n - hq * per) * D::TILE;
     if (q0 + D::TILE <= wfirst || j0 + wave * 32 >= w.len) return;
-    const float slope = a.slopes ? a.slopes[kvh * rep + hq] : 0.f;
+    const Bias bias = bias_of<T>(a, units(a, kvh * rep + hq), j0 + wave * 32, j, q0, h);
+    const float off = bias.own * c;
     const bool masked = limited && q0 < j0 + wave * 32 + 31 && j0 + wave * 32 + 31 >= prefix;
 #pragma unroll
     for (int t = 0; t < D::SUB; ++t) {
@@ -617,7 +678,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         mma<T>(dp, Image<T, DP>::row(dimg, 32 * t + fold<T>(r), 2 * g + h), vf[g]);
       }
       const f32x16 sc = capped<T>(s, a);
-      s = biased<T>(sc, a, slope, j - (q0 + 32 * t), h);
+      s = biased<T>(sc, bias, t);
       f32x16 ls, de;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -626,16 +687,16 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -ls[e]));
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, off) - ls[e]);
         dp[e] = s[e] * (dp[e] - de[e]);
       }
       dp = through_cap(dp, sc, a);
       if (masked) {
+        const uint32_t bits = ~lane_bits<T>(~0ull, t, first - q0, h);  // queries from `first` on
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const bool sees = q0 + 32 * t + row_of<T>(e, h) >= first;
-          s[e] = sees ? s[e] : 0.f;
-          dp[e] = sees ? dp[e] : 0.f;
+          s[e] = pick(bits, row_of<T>(e, 0), s[e], 0.f);
+          dp[e] = pick(bits, row_of<T>(e, 0), dp[e], 0.f);
         }
       }
 #pragma unroll
@@ -699,7 +760,10 @@ int launch_bwd(const Args& a, int waves, hipStream_t st) {
 }
 
 // workgroups of 128 rows where the documents are long enough to fill them, of 64 rows for short ones
-int pick_waves(long long T, int docs) { return T >= 128LL * docs ? 4 : 2; }
+#ifndef WAVES_RULE
+#define WAVES_RULE T >= 128LL * docs ? 4 : 2
+#endif
+int pick_waves(long long T, int docs) { return WAVES_RULE; }
 
 template <class F>
 int with_shape(int dtype, int Dh, F&& f) {
@@ -747,6 +811,10 @@ Args make_args(const tt_attention_args* p) {
   a.lse = p->lse; a.delta = p->delta; a.cu = p->cu_seqlens; a.prefix = p->prefix; a.slopes = p->slopes; a.keep = p->key_mask;
   a.T = (int)p->T; a.docs = p->docs; a.H = p->heads; a.Hkv = p->kv_heads; a.Dh = p->head_dim; a.causal = p->causal;
   a.scale = p->scale; a.cap = p->softcap;
+#ifndef SPREAD
+#define SPREAD p->T >= 256LL * p->docs
+#endif
+  a.spread = SPREAD;
   return a;
 }
 
