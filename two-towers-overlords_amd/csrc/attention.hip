@@ -34,7 +34,7 @@ struct Args {
   const int *cu, *prefix;
   const float* slopes;
   const unsigned char* keep;
-  int T, docs, H, Hkv, Dh, causal, spread;
+  int T, docs, H, Hkv, Dh, causal, spread, sorted;
   float scale, cap;
 };
 
@@ -44,7 +44,7 @@ struct Args {
 __device__ __forceinline__ void place(const Args& a, int heads, bool last_first, int& head, int& slot) {
   int id = blockIdx.x;
   if (!a.spread) id = xcd_tile(id, gridDim.x);
-  else if (last_first) id = gridDim.x - 1 - id;
+  else if (last_first && !a.sorted) id = gridDim.x - 1 - id;
   head = id % heads;
   slot = id / heads;
 }
@@ -75,6 +75,42 @@ __device__ __forceinline__ Where locate(const int* __restrict__ cu, int docs, in
   const int e = w.tail ? T : max(at(w.doc + 1), w.start);
   w.len = e - w.start;
   w.tile = t - (w.start / bm + w.doc);
+  return w;
+}
+
+// The same with the tiles sorted by their place in their document, for at most 64 documents: the longest rows of a triangle
+// first, whatever the documents' lengths.  last_first: the last tiles (they see the most keys), else the first ones (their keys
+// are seen by the most queries).  Lane b holds document b's tile count; a ballot counts the documents that reach a tile.
+__device__ __forceinline__ Where locate_sorted(const int* __restrict__ cu, int docs, int T, int rank, int bm, bool last_first) {
+  const int lane = threadIdx.x & 63;
+  auto at = [&](int b) { return min(max(cu[b], 0), T); };
+  const int s = lane < docs ? at(lane) : 0, e = lane < docs ? max(at(lane + 1), s) : 0, tiles = (e - s + bm - 1) / bm;
+  int top = tiles;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+  top = __builtin_amdgcn_readfirstlane(top);
+  Where w;
+  w.tail = false;
+  for (int i = 0; i < top; ++i) {
+    const int k = last_first ? top - 1 - i : i;
+    unsigned long long m = __ballot(tiles > k);
+    const int n = __builtin_popcountll(m);
+    if (rank >= n) {
+      rank -= n;
+      continue;
+    }
+    while (rank-- > 0) m &= m - 1;
+    w.doc = __builtin_ctzll(m);
+    w.start = __builtin_amdgcn_readlane(s, w.doc);
+    w.len = __builtin_amdgcn_readlane(e, w.doc) - w.start;
+    w.tile = k;
+    return w;
+  }
+  w.tail = true;
+  w.doc = docs;
+  w.start = at(docs);
+  w.len = T - w.start;
+  w.tile = rank;
   return w;
 }
 
@@ -259,10 +295,10 @@ struct Bias {
   float slope, at, own;
   int side;
 };
-template <class T>
+template <class T, bool PLAIN>
 __device__ __forceinline__ Bias bias_of(const Args& a, const Units& u, int first, int pos, int r0, int h) {  // first: the wave's first position
   Bias b{u.slope, 0.f, 0.f, 2};
-  if (a.slopes) {
+  if (!PLAIN && a.slopes) {
     b.at = (float)(pos - r0 - (sizeof(T) == 2 ? 8 : 4) * h);  // exact: positions are below 2^24 apart
     b.side = first >= r0 + kRowBytes / (int)sizeof(T) - 1 ? 1 : (first + 31 <= r0 ? -1 : 0);
     if (b.side) b.own = -(float)b.side * b.slope * b.at;
@@ -307,8 +343,8 @@ __device__ __forceinline__ int key_end(const Args& a, int prefix, int i1, int le
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 4 : DP == 64 ? 3 : 2))) void attention_fwd_kernel(Args a, int slots) {
+template <class T, int DP, int WAVES, bool PLAIN>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 4 : DP == 64 ? 3 : 2))) void attention_fwd_kernel(Args a) {
   using D = Dim<T, DP>;
   constexpr int BM = 32 * WAVES;
   __shared__ __align__(16) char k0img[D::BYTES];
@@ -317,7 +353,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   __shared__ __align__(16) char v1img[D::BYTES];
   int head, slot;
   place(a, a.H, true, head, slot);
-  const Where w = locate(a.cu, a.docs, a.T, slot, BM);
+  const Where w = a.sorted ? locate_sorted(a.cu, a.docs, a.T, slot, BM, true) : locate(a.cu, a.docs, a.T, slot, BM);
   const int i0 = w.tile * BM;
   if (i0 < 0 || i0 >= w.len) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
@@ -378,7 +414,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     const int rem = wend - k0;
     const bool masked = now != (D::TILE == 64 ? ~0ull : 0xffffffffull) ||
                         (limited && k0 + D::TILE > i0 + wave * 32 + 1 && k0 + D::TILE > prefix);
-    const Bias bias = bias_of<T>(a, un, i0 + wave * 32, i, k0, h);
+    const Bias bias = bias_of<T, PLAIN>(a, un, i0 + wave * 32, i, k0, h);
     float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < D::SUB; ++t) {
@@ -388,7 +424,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
       if (32 * t < rem) {  // uniform: not the half of a tile that nobody here sees
 #pragma unroll
         for (int g = 0; g < D::G; ++g) mma<T>(acc, Image<T, DP>::row(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
-        acc = biased<T>(capped<T>(acc, a), bias, t);
+        if constexpr (!PLAIN) acc = biased<T>(capped<T>(acc, a), bias, t);
         if (masked) {
           const uint32_t bits = lane_bits<T>(now, t, seen - k0, h);
 #pragma unroll
@@ -450,8 +486,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 
 // ------------------------------------------------------------------------------------------------ dq, delta
 // dS = P (dO V^T - delta) d,  dq_i = scale sum_j dS_ij k_j,  delta_i = dO_i . o_i
-template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 3 : DP == 64 || sizeof(T) == 2 ? 2 : 1))) void attention_dq_kernel(Args a, int slots) {
+template <class T, int DP, int WAVES, bool PLAIN>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 3 : DP == 64 || sizeof(T) == 2 ? 2 : 1))) void attention_dq_kernel(Args a) {
   using D = Dim<T, DP>;
   constexpr int BM = 32 * WAVES;
   __shared__ __align__(16) char k0img[D::BYTES];
@@ -460,7 +496,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   __shared__ __align__(16) char v1img[D::BYTES];
   int head, slot;
   place(a, a.H, true, head, slot);
-  const Where w = locate(a.cu, a.docs, a.T, slot, BM);
+  const Where w = a.sorted ? locate_sorted(a.cu, a.docs, a.T, slot, BM, true) : locate(a.cu, a.docs, a.T, slot, BM);
   const int i0 = w.tile * BM;
   if (i0 < 0 || i0 >= w.len) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
@@ -535,7 +571,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     const bool masked = now != (D::TILE == 64 ? ~0ull : 0xffffffffull) ||
                         (limited && k0 + D::TILE > i0 + wave * 32 + 1 && k0 + D::TILE > prefix);
     const int rem = wend - k0;
-    const Bias bias = bias_of<T>(a, un, i0 + wave * 32, i, k0, h);
+    const Bias bias = bias_of<T, PLAIN>(a, un, i0 + wave * 32, i, k0, h);
     const float off = fmaf(bias.own, c, -lse2);
 #pragma unroll
     for (int t = 0; t < D::SUB; ++t) {
@@ -548,11 +584,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         mma<T>(s, Image<T, DP>::row(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
         mma<T>(dp, Image<T, DP>::row(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
       }
-      const f32x16 sc = capped<T>(s, a);
-      s = biased<T>(sc, bias, t);
+      f32x16 sc;
+      if constexpr (!PLAIN) {
+        sc = capped<T>(s, a);
+        s = biased<T>(sc, bias, t);
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, off)) * (dp[e] - delta);
-      s = through_cap(s, sc, a);
+      if constexpr (!PLAIN) s = through_cap(s, sc, a);
       if (masked) {
         const uint32_t bits = lane_bits<T>(now, t, seen - k0, h);
 #pragma unroll
@@ -584,8 +623,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 // ------------------------------------------------------------------------------------------------ dk, dv
 // A wave owns 32 keys (columns) and walks the queries, for every query head that shares the key head:
 // dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i
-template <class T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 2 : DP == 64 && sizeof(T) == 2 ? 2 : 1))) void attention_dkv_kernel(Args a, int slots) {
+template <class T, int DP, int WAVES, bool PLAIN>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 || (DP == 64 && sizeof(T) == 2) ? 2 : 1))) void attention_dkv_kernel(Args a) {
   using D = Dim<T, DP>;
   constexpr int BM = 32 * WAVES;
   __shared__ __align__(16) char q0img[D::BYTES];
@@ -596,7 +635,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   __shared__ __align__(16) float stat1[2 * D::TILE];
   int kvh, slot;
   place(a, a.Hkv, false, kvh, slot);
-  const Where w = locate(a.cu, a.docs, a.T, slot, BM);
+  const Where w = a.sorted ? locate_sorted(a.cu, a.docs, a.T, slot, BM, false) : locate(a.cu, a.docs, a.T, slot, BM);
   const int j0 = w.tile * BM;
   if (j0 < 0 || j0 >= w.len) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
@@ -663,7 +702,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     if (n + 1 < total) issue(n + 1, qn, dn);
     const int hq = n / per, q0 = bfirst + (n - hq * per) * D::TILE;
     if (q0 + D::TILE <= wfirst || j0 + wave * 32 >= w.len) return;
-    const Bias bias = bias_of<T>(a, units(a, kvh * rep + hq), j0 + wave * 32, j, q0, h);
+    const Bias bias = bias_of<T, PLAIN>(a, units(a, kvh * rep + hq), j0 + wave * 32, j, q0, h);
     const float off = bias.own * c;
     const bool masked = limited && q0 < j0 + wave * 32 + 31 && j0 + wave * 32 + 31 >= prefix;
 #pragma unroll
@@ -677,8 +716,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         mma<T>(s, Image<T, DP>::row(qimg, 32 * t + fold<T>(r), 2 * g + h), kf[g]);
         mma<T>(dp, Image<T, DP>::row(dimg, 32 * t + fold<T>(r), 2 * g + h), vf[g]);
       }
-      const f32x16 sc = capped<T>(s, a);
-      s = biased<T>(sc, bias, t);
+      f32x16 sc;
+      if constexpr (!PLAIN) {
+        sc = capped<T>(s, a);
+        s = biased<T>(sc, bias, t);
+      }
       f32x16 ls, de;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -690,7 +732,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, off) - ls[e]);
         dp[e] = s[e] * (dp[e] - de[e]);
       }
-      dp = through_cap(dp, sc, a);
+      if constexpr (!PLAIN) dp = through_cap(dp, sc, a);
       if (masked) {
         const uint32_t bits = ~lane_bits<T>(~0ull, t, first - q0, h);  // queries from `first` on
 #pragma unroll
@@ -732,28 +774,18 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     }
 }
 
-template <class T, int DP>
-int launch_fwd(const Args& a, int waves, hipStream_t st) {
-  const long long slots = (long long)a.T / (32 * waves) + a.docs + 1, grid = slots * a.H;
-  TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
-  if (waves == 4) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, 4>), dim3((unsigned)grid), dim3(256), 0, st, a, (int)slots);
-  else hipLaunchKernelGGL((attention_fwd_kernel<T, DP, 2>), dim3((unsigned)grid), dim3(128), 0, st, a, (int)slots);
-  TT_CHECK_LAUNCH();
-  return TT_OK;
-}
-template <class T, int DP>
-int launch_bwd(const Args& a, int waves, hipStream_t st) {
-  const long long slots = (long long)a.T / (32 * waves) + a.docs + 1;
+// PLAIN: neither cap nor bias, the encoder's own case: fewer registers and branches
+template <class T, int DP, int WAVES, bool PLAIN>
+int launch(const Args& a, bool backward, hipStream_t st) {
+  const long long slots = (long long)a.T / (32 * WAVES) + a.docs + 1;
   TT_REQUIRE(slots * a.H <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
-  const dim3 gq((unsigned)(slots * a.H)), gk((unsigned)(slots * a.Hkv));
-  if (waves == 4) {
-    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 4>), gq, dim3(256), 0, st, a, (int)slots);
-    TT_CHECK_LAUNCH();
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 4>), gk, dim3(256), 0, st, a, (int)slots);
+  const dim3 gq((unsigned)(slots * a.H)), gk((unsigned)(slots * a.Hkv)), bl(64 * WAVES);
+  if (!backward) {
+    hipLaunchKernelGGL((attention_fwd_kernel<T, DP, WAVES, PLAIN>), gq, bl, 0, st, a);
   } else {
-    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 2>), gq, dim3(128), 0, st, a, (int)slots);
+    hipLaunchKernelGGL((attention_dq_kernel<T, DP, WAVES, PLAIN>), gq, bl, 0, st, a);
     TT_CHECK_LAUNCH();
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 2>), gk, dim3(128), 0, st, a, (int)slots);
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, WAVES, PLAIN>), gk, bl, 0, st, a);
   }
   TT_CHECK_LAUNCH();
   return TT_OK;
@@ -815,7 +847,23 @@ Args make_args(const tt_attention_args* p) {
 #define SPREAD p->T >= 256LL * p->docs
 #endif
   a.spread = SPREAD;
+#ifndef SORTED
+#define SORTED (a.spread && p->docs <= 64 && (p->causal || p->prefix))
+#endif
+  a.sorted = SORTED;
   return a;
+}
+
+int run(const tt_attention_args* p, bool backward, hipStream_t st) {
+  const Args a = make_args(p);
+  const int waves = pick_waves(p->T, p->docs);
+  const bool plain = !(a.cap > 0.f) && !a.slopes;
+  return with_shape(p->dtype, p->head_dim, [&](auto t, auto dp) {
+    using T = decltype(t);
+    constexpr int DP = decltype(dp)::value;
+    if (plain) return waves == 4 ? launch<T, DP, 4, true>(a, backward, st) : launch<T, DP, 2, true>(a, backward, st);
+    return waves == 4 ? launch<T, DP, 4, false>(a, backward, st) : launch<T, DP, 2, false>(a, backward, st);
+  });
 }
 
 }  // namespace
@@ -828,11 +876,7 @@ extern "C" int tt_packed_attention(const tt_attention_args* p, tt_stream_t strea
   const int width = dtype_bytes(p->dtype);
   TT_REQUIRE(view_ok(p->q, width, true) && view_ok(p->k, width, true) && view_ok(p->v, width, true) && view_ok(p->out, width, true),
              TT_ERR_ALIGNMENT);
-  const Args a = make_args(p);
-  const int waves = pick_waves(p->T, p->docs);
-  return with_shape(p->dtype, p->head_dim, [&](auto t, auto dp) {
-    return launch_fwd<decltype(t), decltype(dp)::value>(a, waves, static_cast<hipStream_t>(stream));
-  });
+  return run(p, false, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int tt_packed_attention_bwd(const tt_attention_args* p, tt_stream_t stream) {
@@ -847,9 +891,5 @@ extern "C" int tt_packed_attention_bwd(const tt_attention_args* p, tt_stream_t s
                  view_ok(p->out, width, true) && view_ok(p->dout, width, true) && view_ok(p->dq, width, true) &&
                  view_ok(p->dk, width, true) && view_ok(p->dv, width, true),
              TT_ERR_ALIGNMENT);
-  const Args a = make_args(p);
-  const int waves = pick_waves(p->T, p->docs);
-  return with_shape(p->dtype, p->head_dim, [&](auto t, auto dp) {
-    return launch_bwd<decltype(t), decltype(dp)::value>(a, waves, static_cast<hipStream_t>(stream));
-  });
+  return run(p, true, static_cast<hipStream_t>(stream));
 }
