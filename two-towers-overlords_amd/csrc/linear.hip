@@ -6,6 +6,7 @@
 //             dW = dz^T x                                   both operands K-strided, contraction over the rows split
 //
 // Replaces the nn.Linear (+ activation, + residual add) calls of the frozen encoder of backend/model.py:51-52.
+#include <type_traits>
 #include "mfma_tile.h"
 
 using namespace ttm;
@@ -78,7 +79,7 @@ struct FwdArgs {
   const void *bias, *res;
   void *y, *z;
   long long ldr, ldy;
-  int act, vec, gn;  // gn: tiles along N
+  int act, vec, gm, gn;  // tiles along M and N
 };
 
 // The pre-activation as it is kept: a positive z below fp16's range must not become 0, relu'(z) is 1 there.
@@ -144,8 +145,10 @@ template <class T, class B>
 __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void linear_fwd_kernel(FwdArgs a) {
   __shared__ __align__(16) char b0[B::BYTES];
   __shared__ __align__(16) char b1[B::BYTES];
-  const int t = xcd_tile(blockIdx.x, gridDim.x);
-  const int m0 = t / a.gn * B::BM, n0 = t % a.gn * B::BN;
+  int m0, n0;
+  tile_at(xcd_tile(blockIdx.x, gridDim.x), a.gm, a.gn, m0, n0);
+  m0 *= B::BM;
+  n0 *= B::BN;
   B blk;
   blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
   if (!a.vec) {  // columns or strides that are not whole quads: element by element
@@ -247,7 +250,10 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   const int tiles = a.gm * a.gn;
   const int id = xcd_tile(blockIdx.x, gridDim.x);
   const int z = id / tiles, t = id - z * tiles;
-  const int m0 = t / a.gn * B::BM, n0 = t % a.gn * B::BN;
+  int m0, n0;
+  tile_at(t, a.gm, a.gn, m0, n0);
+  m0 *= B::BM;
+  n0 *= B::BN;
   B blk;
   const int kbeg = z * a.s.kper;
   blk.template product<T, XKS, true>(b0, b1, a.g.X, a.g.Y, a.s, m0, n0, kbeg, min(a.s.K, kbeg + a.s.kper));
@@ -270,9 +276,6 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
     });
   }
 }
-
-// 128x128 tiles once they fill the chip, else 64x64
-bool big_tiles(long long M, long long N, long long splits) { return ((M + 127) / 128) * ((N + 127) / 128) * splits >= 256; }
 
 template <class F>
 int with_type(int dtype, F&& f) {
@@ -322,7 +325,7 @@ int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
   const int bk = kRowBytes / dtype_bytes(dtype);
   a.s = Shape{g.M, g.N, g.K, (int)(pad_to((g.K + g.nsplit - 1) / g.nsplit, bk))};
   a.vec = g.slab ? (g.N % 4 == 0 && quad_ok(g.slab, g.N, 4)) : (g.N % 4 == 0 && quad_ok(g.out, g.ldo, dtype_bytes(dtype)));
-  const int b = big_tiles(g.M, g.N, g.nsplit) ? 128 : 64;
+  const int b = pick_tile(g.M, g.N, g.nsplit, dtype);
   a.gm = (g.M + b - 1) / b;
   a.gn = (g.N + b - 1) / b;
   const long long grid = (long long)a.gm * a.gn * g.nsplit;
@@ -330,16 +333,13 @@ int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
   TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
   return with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
-    const dim3 gr((unsigned)grid), bl(256);
-    if (g.xks) {
-      if (b == 128) hipLaunchKernelGGL((grad_product_kernel<T, true, Mid>), gr, bl, 0, st, a);
-      else hipLaunchKernelGGL((grad_product_kernel<T, true, Small>), gr, bl, 0, st, a);
-    } else {
-      if (b == 128) hipLaunchKernelGGL((grad_product_kernel<T, false, Mid>), gr, bl, 0, st, a);
-      else hipLaunchKernelGGL((grad_product_kernel<T, false, Small>), gr, bl, 0, st, a);
-    }
-    TT_CHECK_LAUNCH();
-    return (int)TT_OK;
+    return with_block<T>(b, [&](auto* shape) {
+      using B = std::remove_pointer_t<decltype(shape)>;
+      if (g.xks) hipLaunchKernelGGL((grad_product_kernel<T, true, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
+      else hipLaunchKernelGGL((grad_product_kernel<T, false, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
+      TT_CHECK_LAUNCH();
+      return (int)TT_OK;
+    });
   });
 }
 
@@ -383,16 +383,19 @@ extern "C" int tt_linear_act(const void* x, int64_t ldx, const void* w, int64_t 
   a.s = Shape{(int)M, N, K, K};
   a.bias = bias; a.res = residual; a.y = y; a.z = preact; a.ldr = ldr; a.ldy = ldy; a.act = act;
   a.vec = N % 4 == 0 && quad_ok(bias, 0, width) && quad_ok(residual, ldr, width) && quad_ok(y, ldy, width) && quad_ok(preact, N, width);
-  const int b = big_tiles(M, N, 1) ? 128 : 64;
+  const int b = pick_tile(M, N, 1, dtype);
+  a.gm = (int)((M + b - 1) / b);
   a.gn = (N + b - 1) / b;
-  const long long grid = ((M + b - 1) / b) * (long long)a.gn;
+  const long long grid = (long long)a.gm * a.gn;
   TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
   return with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
-    if (b == 128) hipLaunchKernelGGL((linear_fwd_kernel<T, Mid>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((linear_fwd_kernel<T, Small>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    TT_CHECK_LAUNCH();
-    return (int)TT_OK;
+    return with_block<T>(b, [&](auto* shape) {
+      using B = std::remove_pointer_t<decltype(shape)>;
+      hipLaunchKernelGGL((linear_fwd_kernel<T, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
+      TT_CHECK_LAUNCH();
+      return (int)TT_OK;
+    });
   });
 }
 

@@ -172,6 +172,15 @@ __device__ __forceinline__ int xcd_tile(int id, int total) {
   return x * q + min(x, r) + (id >> 3);
 }
 
+constexpr int kBand = 4;
+// Row and column of tile t of a grid of gm x gn: bands of four rows, column by column, so that the tiles in flight on an XCD
+// share both operands' panels (32 tiles of one row would share one; bf16 8192 cubed, 128-wide tiles: 1236 -> 1112 us).
+__device__ __forceinline__ void tile_at(int t, int gm, int gn, int& m, int& n) {
+  const int band = t / (kBand * gn), first = band * kBand, rows = min(kBand, gm - first), in = t - band * kBand * gn;
+  n = in / rows;
+  m = first + in - n * rows;
+}
+
 struct Shape {
   int M, N, K;      // output [M, N] (N contiguous), contraction K.  A K-contiguous operand is readable, and zero, up to the
                     // next multiple of KPF behind K; a K-strided one has K rows, readable to the next multiple of KPF columns
@@ -242,17 +251,22 @@ struct Block {
     auto step = [&](int t, char* __restrict__ cur, char* __restrict__ nxt, auto& c) {
       stage_wait();
       if (t + 1 < steps) issue(t + 1, nxt);
+      // the next group's fragments are asked for before this group's products
+      u32x4 fy[2][NI], fx[2][MJ];
+      auto get = [&](int g) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) fy[g & 1][i] = TY::get(cur + BM * kRowBytes, (wn * NI + i) * 32, g, lane);
+#pragma unroll
+        for (int j = 0; j < MJ; ++j) fx[g & 1][j] = TX::get(cur, (wm * MJ + j) * 32, g, lane);
+      };
+      get(0);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        u32x4 fy[NI], fx[MJ];
-#pragma unroll
-        for (int i = 0; i < NI; ++i) fy[i] = TY::get(cur + BM * kRowBytes, (wn * NI + i) * 32, g, lane);
-#pragma unroll
-        for (int j = 0; j < MJ; ++j) fx[j] = TX::get(cur, (wm * MJ + j) * 32, g, lane);
+        if (g < 3) get(g + 1);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-          for (int j = 0; j < MJ; ++j) mma<T>(c[i][j], fy[i], fx[j]);
+          for (int j = 0; j < MJ; ++j) mma<T>(c[i][j], fy[g & 1][i], fx[g & 1][j]);
       }
     };
     issue(0, b0);
@@ -287,6 +301,31 @@ struct Block {
 };
 using Small = Block<64, 64, 2, 2>;
 using Mid = Block<128, 128, 2, 2>;
+using Large = Block<256, 256, 4, 2>;
+
+// Edge of the output tile, 64, 128 or 256, for a product of M x N outputs in `splits` parts: the least estimated time, in units
+// of a compute unit's work.  A round of tiles takes as long as the tiles that share a compute unit; `rate` is what a tile
+// shape reaches of the best one's on full rounds: bf16 8192 cubed 460 / 998 / 1120 TFLOP/s, float 16384 x 4096 x 1024 120 / 131;
+// float has no registers for the largest.
+inline int pick_tile(long long M, long long N, long long splits, int dtype) {
+  static const struct { int edge, share; float rate16, rate32; } kinds[] = {{64, 4, 0.42f, 0.92f}, {128, 2, 0.9f, 1.f}, {256, 1, 1.f, 0.f}};
+  int best = 64;
+  double least = 1e300;
+  for (const auto& k : kinds) {
+    if (dtype == TT_F32 && k.rate32 == 0.f) continue;
+    const long long tiles = ((M + k.edge - 1) / k.edge) * ((N + k.edge - 1) / k.edge) * splits;
+    const double rounds = (double)((tiles + 256 * k.share - 1) / (256 * k.share));
+    // the last round's compute units share their tiles only as far as there are any
+    const long long last = tiles - (long long)(rounds - 1) * 256 * k.share;
+    const double share = rounds - 1 + (double)((last + 255) / 256) / k.share;
+    const double t = share * k.share * k.edge * k.edge / (dtype == TT_F32 ? k.rate32 : k.rate16);
+    if (t < least) {
+      least = t;
+      best = k.edge;
+    }
+  }
+  return best;
+}
 
 // one row's quad at columns [n, n + 4) of a row-major matrix; `vec`: whole quads are in range and aligned
 template <class T>
@@ -330,6 +369,14 @@ inline bool packed_ok(const void* p, long long ld, long long cols, int dtype) {
 inline size_t pack_bytes(const void* p, long long ld, long long rows, long long cols, int dtype) {
   if (packed_ok(p, ld, cols, dtype)) return 0;
   return align256((size_t)rows * (size_t)pad_to(cols, 16 / dtype_bytes(dtype)) * dtype_bytes(dtype));
+}
+
+// f(block) with the block shape of a tile edge that pick_tile gave for T
+template <class T, class F>
+int with_block(int edge, F&& f) {
+  if constexpr (sizeof(T) == 2)
+    if (edge == 256) return f(static_cast<Large*>(nullptr));
+  return edge == 64 ? f(static_cast<Small*>(nullptr)) : f(static_cast<Mid*>(nullptr));
 }
 
 }  // namespace ttm

@@ -27,7 +27,7 @@ struct Args {
   Shape s;               // M rows, N candidates (all of them, or a piece), K features
   const long long *target, *rid, *cid;
   long long ignore;
-  int v0, V, gn;         // first candidate of the piece; candidates in all; tiles along N
+  int v0, V, gm, gn;     // first candidate of the piece; candidates in all; tiles along the rows and the candidates
   float scale2;          // scale * log2 e
   float2* part;          // [gn, M] (maximum, sum) of a tile's candidates
   float* tlogit;         // [M] the target's logit, base 2
@@ -46,8 +46,9 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   __shared__ __align__(16) char b0[B::BYTES];
   __shared__ __align__(16) char b1[B::BYTES];
   constexpr int NI = B::NI, MJ = B::MJ;
-  const int tl = xcd_tile(blockIdx.x, gridDim.x);
-  const int m0 = tl / a.gn * B::BM, tn = tl % a.gn, n0 = tn * B::BN;
+  int tm, tn;
+  tile_at(xcd_tile(blockIdx.x, gridDim.x), a.gm, a.gn, tm, tn);
+  const int m0 = tm * B::BM, n0 = tn * B::BN;
   B blk;
   blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
   auto& acc = blk.acc;
@@ -131,8 +132,9 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   __shared__ __align__(16) char b0[B::BYTES];
   __shared__ __align__(16) char b1[B::BYTES];
   constexpr int NI = B::NI, MJ = B::MJ;
-  const int tl = xcd_tile(blockIdx.x, gridDim.x);
-  const int m0 = tl / a.gn * B::BM, n0 = tl % a.gn * B::BN;
+  int tm, tn;
+  tile_at(xcd_tile(blockIdx.x, gridDim.x), a.gm, a.gn, tm, tn);
+  const int m0 = tm * B::BM, n0 = tn * B::BN;
   B blk;
   blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
   auto& acc = blk.acc;
@@ -191,8 +193,6 @@ int with_type(int dtype, F&& f) {
   }
 }
 
-int tile_of(long long M, long long N) { return ((M + 127) / 128) * ((N + 127) / 128) >= 256 ? 128 : 64; }
-
 struct Plan {
   int gn, fwd_tile;
   long long piece;      // candidates of a piece (a multiple of 128)
@@ -203,7 +203,7 @@ constexpr long long kPieceBytes = 256LL << 20;  // of G: what the Infinity Cache
 Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long M, int V, int D, int dtype) {
   Plan p{};
   const int width = dtype_bytes(dtype);
-  p.fwd_tile = tile_of(M, V);
+  p.fwd_tile = pick_tile(M, V, 1, dtype);
   p.gn = (V + p.fwd_tile - 1) / p.fwd_tile;
   p.x = pack_bytes(x, ldx, M, D, dtype);
   p.w = pack_bytes(w, ldw, V, D, dtype);
@@ -277,14 +277,17 @@ extern "C" int tt_softmax_loss(const void* x, int64_t ldx, const void* w, int64_
   a.target = (const long long*)target; a.rid = (const long long*)row_ids; a.cid = (const long long*)cand_ids;
   a.ignore = ignore_index; a.V = V; a.gn = p.gn; a.scale2 = scale * kLog2e;
   const int b = p.fwd_tile;
-  const long long grid = ((N + b - 1) / b) * (long long)p.gn;
+  a.gm = (int)((N + b - 1) / b);
+  const long long grid = (long long)a.gm * p.gn;
   TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
   rc = with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
-    if (b == 128) hipLaunchKernelGGL((softmax_lse_kernel<T, Mid>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((softmax_lse_kernel<T, Small>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    TT_CHECK_LAUNCH();
-    return (int)TT_OK;
+    return with_block<T>(b, [&](auto* shape) {
+      using B = std::remove_pointer_t<decltype(shape)>;
+      hipLaunchKernelGGL((softmax_lse_kernel<T, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
+      TT_CHECK_LAUNCH();
+      return (int)TT_OK;
+    });
   });
   if (rc != TT_OK) return rc;
   hipLaunchKernelGGL(softmax_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, a.part, a.tlogit, a.target, a.ignore,
@@ -334,16 +337,19 @@ extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t
     a.v0 = (int)v0;
     a.W = Operand{static_cast<const char*>(W.p) + v0 * W.ld * width, W.ld};
     a.s = Shape{(int)N, vc, D, D};
-    const int b = tile_of(N, p.piece);
+    const int b = pick_tile(N, vc, 1, dtype);
     a.gn = (vc + b - 1) / b;  // every tile starts at a candidate of the piece; the last one zero-fills behind it
-    const long long grid = ((N + b - 1) / b) * (long long)a.gn;
+    a.gm = (int)((N + b - 1) / b);
+    const long long grid = (long long)a.gm * a.gn;
     TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
     rc = with_type(dtype, [&](auto tag) {
       using T = decltype(tag);
-      if (b == 128) hipLaunchKernelGGL((softmax_grad_kernel<T, Mid>), dim3((unsigned)grid), dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((softmax_grad_kernel<T, Small>), dim3((unsigned)grid), dim3(256), 0, st, a);
-      TT_CHECK_LAUNCH();
-      return (int)TT_OK;
+      return with_block<T>(b, [&](auto* shape) {
+        using B = std::remove_pointer_t<decltype(shape)>;
+        hipLaunchKernelGGL((softmax_grad_kernel<T, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
+        TT_CHECK_LAUNCH();
+        return (int)TT_OK;
+      });
     });
     if (rc != TT_OK) return rc;
     if (dx) {
