@@ -92,53 +92,43 @@ __device__ __forceinline__ f32x4 kept(f32x4 v, int act) {
   return v;
 }
 
-// whole quads, aligned: the loads of an accumulator row are issued together
+// whole 16-byte chunks, aligned
 template <class T, int ACT, class B>
-__device__ __forceinline__ void epilogue(B& blk, const FwdArgs& a, int m0, int n0) {
-  typedef typename Type<T>::quad quad;
-  const T* __restrict__ bias = static_cast<const T*>(a.bias);
-  const int N = a.s.N, nb = n0 + blk.wn * B::NI * 32 + 4 * blk.h;
-  quad bq[B::NI][4];
+__device__ __forceinline__ void epilogue(B& blk, const FwdArgs& a, char* __restrict__ b0, char* __restrict__ b1, int m0, int n0) {
+  using R = typename B::template Rows<T>;
+  const int n = blk.template row_col<T>(n0), M = a.s.M;
+  const bool col = n < a.s.N;
+  const T* __restrict__ res = static_cast<const T*>(a.res);
+  Chunk<T> bias;
+  bias.zero();
+  if (a.bias && col) bias.load(static_cast<const T*>(a.bias) + n);
+  Chunk<T> rq[R::STEPS];
+  blk.template for_rows<T>(
+      b0, b1, m0, n0,
+      [&](int j) {  // the residual of 32 rows at once
+        if (!res) return;
 #pragma unroll
-  for (int i = 0; i < B::NI; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int n = nb + 32 * i + 8 * q;
-      bq[i][q] = quad(0);
-      if (bias && n < N) bq[i][q] = *reinterpret_cast<const quad*>(bias + n);
-    }
-#pragma unroll
-  for (int j = 0; j < B::MJ; ++j) {
-    const int m = m0 + (blk.wm * B::MJ + j) * 32 + blk.r;
-    const bool row = m < a.s.M;
-    const T* __restrict__ res = static_cast<const T*>(a.res) + m * a.ldr + nb;
-    T* __restrict__ y = static_cast<T*>(a.y) + m * a.ldy + nb;
-    T* __restrict__ z = static_cast<T*>(a.z) + (long long)m * N + nb;
-    quad rq[B::NI][4];
-    if (a.res) {
-#pragma unroll
-      for (int i = 0; i < B::NI; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          rq[i][q] = quad(0);
-          if (row && nb + 32 * i + 8 * q < N) rq[i][q] = *reinterpret_cast<const quad*>(res + 32 * i + 8 * q);
+        for (int s = 0; s < R::STEPS; ++s) {
+          const int m = blk.template row_at<T>(m0, j, s);
+          rq[s].zero();
+          if (m < M && col) rq[s].load(res + m * a.ldr + n);
         }
-    }
+      },
+      [&](int j, int s, int m, int, f32x4 (&v)[R::Q]) {
+        const bool in = m < M && col;
+        Chunk<T> z, y;
 #pragma unroll
-    for (int i = 0; i < B::NI; ++i)
+        for (int q = 0; q < R::Q; ++q) {
+          v[q] += from_quad<T>(bias.q[q]);
+          z.q[q] = to_quad<T>(kept<T>(v[q], ACT));
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const bool in = row && nb + 32 * i + 8 * q < N;
-        f32x4 v = from_quad<T>(bq[i][q]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] += blk.acc[i][j][4 * q + c];
-        if (a.z && in) *reinterpret_cast<quad*>(z + 32 * i + 8 * q) = to_quad<T>(kept<T>(v, ACT));
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = act_<ACT, sizeof(T) == 2>(v[c]);
-        if (a.res) v += from_quad<T>(rq[i][q]);
-        if (in) *reinterpret_cast<quad*>(y + 32 * i + 8 * q) = to_quad<T>(v);
-      }
-  }
+          for (int c = 0; c < 4; ++c) v[q][c] = act_<ACT, sizeof(T) == 2>(v[q][c]);
+          if (res) v[q] += from_quad<T>(rq[s].q[q]);
+          y.q[q] = to_quad<T>(v[q]);
+        }
+        if (a.z && in) z.store(static_cast<T*>(a.z) + (long long)m * a.s.N + n);
+        if (in) y.store(static_cast<T*>(a.y) + m * a.ldy + n);
+      });
 }
 
 template <class T, class B>
@@ -151,7 +141,7 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   n0 *= B::BN;
   B blk;
   blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
-  if (!a.vec) {  // columns or strides that are not whole quads: element by element
+  if (!a.vec) {  // columns or strides that are not whole chunks: element by element
     T* __restrict__ z = static_cast<T*>(a.z);
     blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
       if (m >= a.s.M || n >= a.s.N) return;
@@ -165,11 +155,11 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
     });
     return;
   }
-  with_act(a.act, [&](auto tag) { epilogue<T, decltype(tag)::value>(blk, a, m0, n0); });
+  with_act(a.act, [&](auto tag) { epilogue<T, decltype(tag)::value>(blk, a, b0, b1, m0, n0); });
 }
 
-// dz = dy act'(z) (written when dz != null, row stride ldz) and, per block of rows, the column sums of dz.
-// 256 threads = 64 quads of columns x 4 rows; grid (ceil(N / 256), row blocks).
+// dz = dy act'(z) (written when dz != null, row stride ldz) and, per block of rows, the column sums of dz.  Memory-bound.
+// 256 threads = 64 chunks of KPF columns x 4 rows; grid (ceil(N / (64 KPF)), row blocks).
 struct DzArgs {
   const void *dy, *z;
   void* dz;
@@ -178,39 +168,64 @@ struct DzArgs {
   int M, N, rows, act, vec;
 };
 template <class T>
+__device__ __forceinline__ Chunk<T> load_chunk(const T* __restrict__ p, long long ld, int m, int n, int N, bool vec) {
+  Chunk<T> c;
+  if (vec) {
+    c.load(p + m * ld + n);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Type<T>::KPF; ++i) c.q[i >> 2][i & 3] = n + i < N ? p[m * ld + n + i] : (T)0.f;
+  }
+  return c;
+}
+template <class T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
-  __shared__ f32x4 red[4][64];
+  constexpr int Q = Chunk<T>::Q, KPF = Type<T>::KPF;
+  __shared__ f32x4 red[4][64][Q];
   const int q = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int n = (blockIdx.x * 64 + q) * 4;
+  const int n = (blockIdx.x * 64 + q) * KPF;
   const int m1 = min(a.M, (int)(blockIdx.y + 1) * a.rows);
   const T* __restrict__ dy = static_cast<const T*>(a.dy);
   const T* __restrict__ z = static_cast<const T*>(a.z);
   T* __restrict__ dz = static_cast<T*>(a.dz);
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  f32x4 sum[Q];
+#pragma unroll
+  for (int i = 0; i < Q; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const bool vec = a.vec;
   if (n < a.N) {
     with_act(a.act, [&](auto tag) {
       constexpr int ACT = decltype(tag)::value;
+#pragma unroll 2
       for (int m = blockIdx.y * a.rows + w; m < m1; m += 4) {
-        f32x4 v = load_quad<T>(dy, a.lddy, m, n, a.N, vec);
-        if constexpr (ACT != TT_ACT_NONE) {
-          const f32x4 zz = load_quad<T>(z, a.N, m, n, a.N, vec);
+        Chunk<T> c = load_chunk<T>(dy, a.lddy, m, n, a.N, vec), zc = c;
+        if constexpr (ACT != TT_ACT_NONE) zc = load_chunk<T>(z, a.N, m, n, a.N, vec);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) v[c] *= dact_<ACT, sizeof(T) == 2>(zz[c]);
+        for (int i = 0; i < Q; ++i) {
+          f32x4 v = from_quad<T>(c.q[i]);
+          if constexpr (ACT != TT_ACT_NONE) {
+            const f32x4 zz = from_quad<T>(zc.q[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= dact_<ACT, sizeof(T) == 2>(zz[e]);
+          }
+          sum[i] += v;
+          c.q[i] = to_quad<T>(v);
         }
-        if (dz) *reinterpret_cast<typename Type<T>::quad*>(dz + m * a.ldz + n) = to_quad<T>(v);  // ldz covers whole quads
-        sum += v;
+        if (dz) c.store(dz + m * a.ldz + n);  // ldz covers whole chunks; columns behind N get 0 * act'(0)
       }
     });
   }
   if (!a.part) return;
-  red[w][q] = sum;
+#pragma unroll
+  for (int i = 0; i < Q; ++i) red[w][q][i] = sum[i];
   __syncthreads();
   if (w == 0 && n < a.N) {
-    const f32x4 s = (red[0][q] + red[1][q]) + (red[2][q] + red[3][q]);
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (n + c < a.N) a.part[(long long)blockIdx.y * a.N + n + c] = s[c];
+    for (int i = 0; i < Q; ++i) {
+      const f32x4 s = (red[0][q][i] + red[1][q][i]) + (red[2][q][i] + red[3][q][i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + 4 * i + e < a.N) a.part[(long long)blockIdx.y * a.N + n + 4 * i + e] = s[e];
+    }
   }
 }
 
@@ -259,22 +274,54 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   blk.template product<T, XKS, true>(b0, b1, a.g.X, a.g.Y, a.s, m0, n0, kbeg, min(a.s.K, kbeg + a.s.kper));
   const int M = a.s.M, N = a.s.N;
   const bool vec = a.vec;
+  const float alpha = a.g.alpha_dev ? a.g.alpha * *a.g.alpha_dev : a.g.alpha;
   if (a.g.slab) {
     float* __restrict__ c = a.g.slab + (long long)z * M * N;
     const bool more = a.g.accumulate;
-    blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
-      if (m >= M) return;
-      if (more) v += load_quad<float>(c, N, m, n, N, vec);
-      store_quad<float>(c, N, m, n, N, vec, v);
-    });
-  } else {
-    T* __restrict__ c = static_cast<T*>(a.g.out);
-    const float alpha = a.g.alpha_dev ? a.g.alpha * *a.g.alpha_dev : a.g.alpha;
-    const long long ldo = a.g.ldo;
-    blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
-      if (m < M) store_quad<T>(c, ldo, m, n, N, vec, v * alpha);
-    });
+    if (!vec) {
+      blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
+        if (m >= M) return;
+        if (more) v += load_quad<float>(c, N, m, n, N, false);
+        store_quad<float>(c, N, m, n, N, false, v);
+      });
+      return;
+    }
+    using R = typename B::template Rows<float>;
+    f32x4 old[R::STEPS];
+    const int n = blk.template row_col<float>(n0);
+    blk.template for_rows<float>(
+        b0, b1, m0, n0,
+        [&](int j) {
+          if (!more) return;
+#pragma unroll
+          for (int s = 0; s < R::STEPS; ++s) {
+            const int m = blk.template row_at<float>(m0, j, s);
+            if (m < M && n < N) old[s] = *reinterpret_cast<const f32x4*>(c + (long long)m * N + n);
+          }
+        },
+        [&](int j, int s, int m, int, f32x4 (&v)[R::Q]) {
+          if (more) v[0] += old[s];
+          if (m < M && n < N) *reinterpret_cast<f32x4*>(c + (long long)m * N + n) = v[0];
+        });
+    return;
   }
+  T* __restrict__ c = static_cast<T*>(a.g.out);
+  const long long ldo = a.g.ldo;
+  if (!vec) {
+    blk.for_quads(m0, n0, [&](int m, int n, f32x4 v) {
+      if (m < M) store_quad<T>(c, ldo, m, n, N, false, v * alpha);
+    });
+    return;
+  }
+  using R = typename B::template Rows<T>;
+  blk.template for_rows<T>(
+      b0, b1, m0, n0, [](int) {},
+      [&](int j, int s, int m, int n, f32x4 (&v)[R::Q]) {
+        Chunk<T> o;
+#pragma unroll
+        for (int q = 0; q < R::Q; ++q) o.q[q] = to_quad<T>(v[q] * alpha);
+        if (m < M && n < N) o.store(c + m * ldo + n);
+      });
 }
 
 template <class F>
@@ -287,7 +334,8 @@ int with_type(int dtype, F&& f) {
   }
 }
 bool known_dtype(int d) { return d == TT_F32 || d == TT_BF16 || d == TT_F16; }
-bool quad_ok(const void* p, long long ld, int width) { return !p || ((reinterpret_cast<uintptr_t>(p) % (4 * width)) == 0 && ld % 4 == 0); }
+// rows of 16-byte chunks
+bool chunk_ok(const void* p, long long ld, int width) { return !p || (tt_aligned16(p) && ld % (16 / width) == 0); }
 
 }  // namespace
 
@@ -324,7 +372,7 @@ int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
   a.g = g;
   const int bk = kRowBytes / dtype_bytes(dtype);
   a.s = Shape{g.M, g.N, g.K, (int)(pad_to((g.K + g.nsplit - 1) / g.nsplit, bk))};
-  a.vec = g.slab ? (g.N % 4 == 0 && quad_ok(g.slab, g.N, 4)) : (g.N % 4 == 0 && quad_ok(g.out, g.ldo, dtype_bytes(dtype)));
+  a.vec = g.slab ? g.N % 4 == 0 : chunk_ok(g.out, g.ldo, dtype_bytes(dtype)) && g.N % (16 / dtype_bytes(dtype)) == 0;
   const int b = pick_tile(g.M, g.N, g.nsplit, dtype);
   a.gm = (g.M + b - 1) / b;
   a.gn = (g.N + b - 1) / b;
@@ -382,7 +430,7 @@ extern "C" int tt_linear_act(const void* x, int64_t ldx, const void* w, int64_t 
   }
   a.s = Shape{(int)M, N, K, K};
   a.bias = bias; a.res = residual; a.y = y; a.z = preact; a.ldr = ldr; a.ldy = ldy; a.act = act;
-  a.vec = N % 4 == 0 && quad_ok(bias, 0, width) && quad_ok(residual, ldr, width) && quad_ok(y, ldy, width) && quad_ok(preact, N, width);
+  a.vec = N % (16 / width) == 0 && chunk_ok(bias, 0, width) && chunk_ok(residual, ldr, width) && chunk_ok(y, ldy, width) && chunk_ok(preact, N, width);
   const int b = pick_tile(M, N, 1, dtype);
   a.gm = (int)((M + b - 1) / b);
   a.gn = (N + b - 1) / b;
@@ -413,7 +461,7 @@ BwdPlan bwd_plan(const void* dy, int64_t lddy, const void* x, int64_t ldx, const
   p.own_dz = act != TT_ACT_NONE || !packed_ok(dy, lddy, N, dtype);
   p.ldz = p.own_dz ? pad_to(N, 16 / width) : lddy;
   p.splits = need_dw ? tt_grad_splits(N, K, M) : 1;
-  const long long gx = (N + 255) / 256;
+  const long long gx = (N + 1024 / width - 1) / (1024 / width);
   long long rb = (1024 + gx - 1) / gx;
   if (rb > (M + 15) / 16) rb = (M + 15) / 16;
   if (rb < 1) rb = 1;
@@ -466,17 +514,13 @@ extern "C" int tt_linear_act_bwd(const void* dy, int64_t lddy, const void* x, in
   const bool products = dx || dw;
   const bool write_dz = p.own_dz && products;
   if (write_dz || dbias) {
-    if (write_dz && p.ldz != N) {  // the zero columns behind N are part of the operand
-      rc = tt_launch_pack(dy, lddy, dz, p.ldz, M, N, width, st);
-      if (rc != TT_OK) return rc;
-    }
     DzArgs a{};
     a.dy = dy; a.z = preact; a.dz = write_dz ? dz : nullptr; a.part = dbias ? part : nullptr;
     a.lddy = lddy; a.ldz = p.ldz; a.M = (int)M; a.N = N; a.rows = p.rows; a.act = act;
-    a.vec = N % 4 == 0 && quad_ok(dy, lddy, width) && quad_ok(act == TT_ACT_NONE ? nullptr : preact, N, width);
+    a.vec = N % (16 / width) == 0 && chunk_ok(dy, lddy, width) && chunk_ok(act == TT_ACT_NONE ? nullptr : preact, N, width);
     rc = with_type(dtype, [&](auto tag) {
       using T = decltype(tag);
-      hipLaunchKernelGGL(linear_dz_kernel<T>, dim3((N + 255) / 256, p.row_blocks), dim3(256), 0, st, a);
+      hipLaunchKernelGGL(linear_dz_kernel<T>, dim3((N + 1024 / width - 1) / (1024 / width), p.row_blocks), dim3(256), 0, st, a);
       TT_CHECK_LAUNCH();
       return (int)TT_OK;
     });

@@ -109,6 +109,9 @@ __device__ __forceinline__ void lds_fill(const char* src, char* dst) {
 // This wave's outstanding fills have landed and its LDS accesses are done; then the whole workgroup's.
 __device__ __forceinline__ void stage_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// LDS as a wave's own scratch: what its lanes wrote is there for all of them
+__device__ __forceinline__ void wave_lds_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // ---- a product's operand in global memory ------------------------------------------------------------------
 // `p` is 16-byte aligned, `ld` a multiple of KPF elements, and so is the contiguous extent (callers pack what is not).
 // K-contiguous (KS = false): element (row, k) at p[row * ld + k].  K-strided (KS = true): element (row, k) at p[k * ld + row].
@@ -298,6 +301,51 @@ struct Block {
           fn(m0 + (wm * MJ + j) * 32 + r, n0 + (wn * NI + i) * 32 + 8 * a + 4 * h, v);
         }
   }
+
+  // Rows of the output instead: the accumulators of 32 rows at a time go through the wave's own part of LDS and come back as
+  // KPF consecutive columns per lane, so that 16 lanes read and write 256 consecutive bytes of a row (a quad per lane and row
+  // touched 16 bytes of 32 rows at a time).  fn(j, step, m, n, v): v holds KPF / 4 quads; n does not depend on j and step.
+  // The 16-byte chunk of a row is XORed with the row: no bank conflicts either way.  pre(j): before the rows of j.
+  template <class T>
+  struct Rows {
+    static constexpr int W = NI * 32, Q = Type<T>::KPF / 4, LPR = W / Type<T>::KPF, RPS = 64 / LPR, STEPS = 32 / RPS;
+  };
+  template <class T>
+  __device__ __forceinline__ int row_col(int n0) const { return n0 + wn * Rows<T>::W + (lane % Rows<T>::LPR) * Type<T>::KPF; }
+  template <class T>
+  __device__ __forceinline__ int row_at(int m0, int j, int step) const {
+    return m0 + (wm * MJ + j) * 32 + step * Rows<T>::RPS + lane / Rows<T>::LPR;
+  }
+  template <class T, class P, class F>
+  __device__ __forceinline__ void for_rows(char* __restrict__ b0, char* __restrict__ b1, int m0, int n0, P&& pre, F&& fn) {
+    using R = Rows<T>;
+    constexpr int AREA = 32 * R::W * 4, PER = BYTES / AREA;
+    static_assert(PER * 2 >= WAVES, "an area per wave");
+    __syncthreads();  // everyone is done with the operands
+    char* const area = wave < PER ? b0 + wave * AREA : b1 + (wave - PER) * AREA;
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) {
+      pre(j);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 v = {acc[i][j][4 * a], acc[i][j][4 * a + 1], acc[i][j][4 * a + 2], acc[i][j][4 * a + 3]};
+          *reinterpret_cast<f32x4*>(area + r * (R::W * 4) + (((i * 8 + 2 * a + h) ^ (r & 7)) * 16)) = v;
+        }
+      wave_lds_sync();
+#pragma unroll
+      for (int s = 0; s < R::STEPS; ++s) {
+        const int row = s * R::RPS + lane / R::LPR;
+        f32x4 v[R::Q];
+#pragma unroll
+        for (int q = 0; q < R::Q; ++q)
+          v[q] = *reinterpret_cast<const f32x4*>(area + row * (R::W * 4) + ((((lane % R::LPR) * R::Q + q) ^ (row & 7)) * 16));
+        fn(j, s, row_at<T>(m0, j, s), row_col<T>(n0), v);
+      }
+      wave_lds_sync();
+    }
+  }
 };
 using Small = Block<64, 64, 2, 2>;
 using Mid = Block<128, 128, 2, 2>;
@@ -353,6 +401,26 @@ __device__ __forceinline__ f32x4 load_quad(const T* __restrict__ p, long long ld
   }
   return v;
 }
+
+// KPF consecutive columns (16 bytes) of a row
+template <class T>
+struct Chunk {
+  static constexpr int Q = Type<T>::KPF / 4;
+  typename Type<T>::quad q[Q];
+  __device__ __forceinline__ void load(const T* __restrict__ p) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+    __builtin_memcpy(q, &v, 16);
+  }
+  __device__ __forceinline__ void store(T* __restrict__ p) const {
+    u32x4 v;
+    __builtin_memcpy(&v, q, 16);
+    *reinterpret_cast<u32x4*>(p) = v;
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) q[i] = typename Type<T>::quad(0);
+  }
+};
 
 // ---- host side ----------------------------------------------------------------------------------------------
 inline long long pad_to(long long n, int m) { return (n + m - 1) / m * m; }

@@ -38,7 +38,9 @@ struct Args {
 
 // Is candidate j left out of the row's sum (its own group, or behind the last)?
 __device__ __forceinline__ bool left_out(const Args& a, int j, long long t, long long rid) {
-  return j >= a.V || (a.rid && a.cid[j] == rid && j != t);
+  bool out = j >= a.V;
+  if (a.rid) out |= (a.cid[min(j, a.V - 1)] == rid) & (j != t);
+  return out;
 }
 
 template <class T, class B>
@@ -55,29 +57,42 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   const int r = blk.r, h = blk.h, wm = blk.wm, wn = blk.wn;
   __syncthreads();
   float2* red = reinterpret_cast<float2*>(b0);  // [WN][BM]
+  const int nw = n0 + wn * NI * 32;             // the wave's first candidate
+  const bool plain = !a.rid && nw + NI * 32 <= a.V;
 #pragma unroll
   for (int j = 0; j < MJ; ++j) {
     const int ml = (wm * MJ + j) * 32 + r, m = m0 + ml;
     const bool in = m < a.s.M;
-    const long long t = in ? a.target[m] : -1, rid = in && a.rid ? a.rid[m] : 0;
+    const long long t = in ? a.target[m] : -1;
+    const long long at = t - nw;
+    if (__any(at >= 0 && at < NI * 32)) {  // some row's target is among these candidates
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (at == i * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) a.tlogit[m] = acc[i][j][e] * a.scale2;
+    }
+    if (!plain) {
+      const long long rid = in && a.rid ? a.rid[m] : 0;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (left_out(a, nw + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3), t, rid)) acc[i][j][e] = -INFINITY;
+    }
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int n = n0 + (wn * NI + i) * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-        const float v = left_out(a, n, t, rid) ? -INFINITY : acc[i][j][e] * a.scale2;
-        acc[i][j][e] = v;
-        mx = fmaxf(mx, v);
-        if (in && n == t) a.tlogit[m] = v;
-      }
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f;
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale2;
+    const float base = mx == -INFINITY ? 0.f : -mx;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(acc[i][j][e] - base);
+      for (int e = 0; e < 16; ++e) part[e & 3] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], a.scale2, base));
+    float sum = (part[0] + part[1]) + (part[2] + part[3]);
     sum += __shfl_xor(sum, 32, 64);
     if (h == 0) red[wn * B::BM + ml] = make_float2(mx, sum);
   }
@@ -131,38 +146,45 @@ template <class T, class B>
 __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void softmax_grad_kernel(Args a) {
   __shared__ __align__(16) char b0[B::BYTES];
   __shared__ __align__(16) char b1[B::BYTES];
-  constexpr int NI = B::NI, MJ = B::MJ;
   int tm, tn;
   tile_at(xcd_tile(blockIdx.x, gridDim.x), a.gm, a.gn, tm, tn);
   const int m0 = tm * B::BM, n0 = tn * B::BN;
   B blk;
   blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
-  auto& acc = blk.acc;
-  const int r = blk.r, h = blk.h, wm = blk.wm, wn = blk.wn;
   T* __restrict__ G = static_cast<T*>(a.G);
   const float up = __is_same(T, _Float16) ? kF16Up / *a.cmax : 1.f;
+  using R = typename B::template Rows<T>;
+  blk.template for_rows<T>(
+      b0, b1, m0, n0, [](int) {},
+      [&](int j, int s, int m, int nl, f32x4 (&v)[R::Q]) {
+        if (m >= a.s.M || nl >= a.ldg) return;
+        const long long t = a.target[m];
+        const float lse2 = a.lse[m] * kLog2e, c = t == a.ignore ? 0.f : (t < 0 || t >= a.V ? NAN : a.coef[m] * up);
+        const int n = a.v0 + nl;
 #pragma unroll
-  for (int j = 0; j < MJ; ++j) {
-    const int m = m0 + (wm * MJ + j) * 32 + r;
-    if (m >= a.s.M) continue;
-    const long long t = a.target[m], rid = a.rid ? a.rid[m] : 0;
-    const bool off = t == a.ignore;
-    const float lse2 = a.lse[m] * kLog2e, c = off ? 0.f : (t < 0 || t >= a.V ? NAN : a.coef[m] * up);
+        for (int q = 0; q < R::Q; ++q)
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+          for (int e = 0; e < 4; ++e) v[q][e] = c * __builtin_amdgcn_exp2f(fmaf(v[q][e], a.scale2, -lse2));
+        if (t >= n && t < n + 4 * R::Q) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int nl = n0 + (wn * NI + i) * 32 + 8 * q + 4 * h;
-        f32x4 g;
+          for (int q = 0; q < R::Q; ++q)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = a.v0 + nl + e;
-          const float p = left_out(a, n, t, rid) ? 0.f : __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * q + e], a.scale2, -lse2));
-          g[e] = off || n >= a.V ? 0.f : c * (n == t ? p - 1.f : p);
+            for (int e = 0; e < 4; ++e)
+              if (n + 4 * q + e == t) v[q][e] -= c;
         }
-        if (nl < a.ldg) *reinterpret_cast<typename Type<T>::quad*>(G + m * a.ldg + nl) = to_quad<T>(g);
-      }
-  }
+        const bool off = t == a.ignore;
+        if (off || a.rid || n + 4 * R::Q > a.V) {
+          const long long rid = a.rid ? a.rid[m] : 0;
+#pragma unroll
+          for (int q = 0; q < R::Q; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[q][e] = (off | left_out(a, n + 4 * q + e, t, rid)) ? 0.f : v[q][e];
+        }
+        Chunk<T> g;
+#pragma unroll
+        for (int q = 0; q < R::Q; ++q) g.q[q] = to_quad<T>(v[q]);
+        g.store(G + m * a.ldg + nl);
+      });
 }
 
 // cmax[0] = max |coef| over the rows that have a target (1 if that is 0 or not finite), cmax[1] = cmax[0] / kF16Up
