@@ -1,0 +1,413 @@
+"""GPU: the encoder operators and the softmax loss as they are used together — a BERT encoder on packed tokens against the
+stock forward, fine-tuning steps through every backward pass, the losses' modules, streams, graphs and long tensors."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+import torch.nn.functional as F
+
+from conftest import load_golden
+
+pytestmark = pytest.mark.gpu
+T = torch.from_numpy
+transformers = pytest.importorskip("transformers")
+
+# one fp32 product of K terms is off by at most (K + 8) 2^-23 of its terms' magnitudes; K <= 128 below: 2^-16
+PRODUCT = (128 + 8) * 2.0 ** -23
+
+
+def tiny_bert(layers=2, hidden=64, heads=2, inter=128, act="gelu", seed=3, positions=160):
+    torch.manual_seed(seed)
+    cfg = transformers.BertConfig(vocab_size=200, hidden_size=hidden, num_hidden_layers=layers, num_attention_heads=heads,
+                                  intermediate_size=inter, max_position_embeddings=positions, hidden_act=act, attn_implementation="eager",
+                                  hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.0)
+    m = transformers.BertModel(cfg).eval()
+    with torch.no_grad():
+        for p in m.parameters():  # weights of a trained model's size, biases that are not zero
+            p.mul_(2.0).add_(torch.randn(p.shape) * 0.02)
+    return m.cuda()
+
+
+def batch(B=9, S=37, seed=0, holes=False):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, 200, (B, S), generator=g)
+    lens = torch.randint(1, S + 1, (B,), generator=g)
+    lens[0] = S
+    mask = (torch.arange(S)[None] < lens[:, None]).long()
+    if holes:
+        mask &= (torch.rand(B, S, generator=g) > 0.3).long()
+        mask[:, 0] = 1
+    return ids.cuda(), mask.cuda()
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_new", "relu", "silu"])
+@pytest.mark.parametrize("hidden,heads", [(32, 4), (64, 2), (96, 1)])
+def test_packed_encoder_equals_the_stock_forward(act, hidden, heads):
+    from two_towers_overlords_amd.encoder import PackedBertEncoder
+
+    m = tiny_bert(hidden=hidden, heads=heads, act=act)
+    ids, mask = batch()
+    with torch.no_grad():
+        got = PackedBertEncoder(m).padded(ids, mask)
+        want = copy.deepcopy(m).double()(input_ids=ids, attention_mask=mask)[0] * mask.unsqueeze(-1)
+    # layer-normalised outputs are of size 1; a layer is 4 products deep on either side of its norms, the norms divide by rows of
+    # about the same size: 2 layers x 8 products x 8 (the norms' and activations' slopes)
+    assert float((got - want).abs().max()) <= 2 * 8 * 8 * PRODUCT
+    assert not bool(got[mask == 0].any())
+
+
+def test_packed_encoder_masks_with_holes_and_token_types():
+    from two_towers_overlords_amd.encoder import PackedBertEncoder
+
+    m = tiny_bert()
+    ids, mask = batch(holes=True)
+    types = torch.randint(0, 2, ids.shape, device="cuda")
+    with torch.no_grad():
+        got = PackedBertEncoder(m).padded(ids, mask, types)
+        want = copy.deepcopy(m).double()(input_ids=ids, attention_mask=mask, token_type_ids=types)[0] * mask.unsqueeze(-1)
+        assert float((got - want).abs().max()) <= 2 * 8 * 8 * PRODUCT
+        full = PackedBertEncoder(m).padded(ids)
+        assert float((full - copy.deepcopy(m).double()(input_ids=ids)[0]).abs().max()) <= 2 * 8 * 8 * PRODUCT
+        mask[3] = 0  # a text without a token: zero rows
+        assert not bool(PackedBertEncoder(m).padded(ids, mask)[3].any())
+        assert PackedBertEncoder(m).padded(ids[:0], mask[:0]).shape == (0, 37, 64)
+
+
+def test_tower_on_the_packed_encoder_matches_the_reference():
+    """The fixture the reference's own tower produced at the MiniLM-L6 shape, with the encoder on packed tokens."""
+    from two_towers_overlords_amd.model import AveragePoolingTower
+
+    g = load_golden("bert_minilm.npz")
+    torch.manual_seed(9)
+    cfg = transformers.BertConfig(vocab_size=30522, hidden_size=384, num_hidden_layers=6, num_attention_heads=12,
+                                  intermediate_size=1536, max_position_embeddings=512)
+    bert = transformers.BertModel(cfg).eval()
+    with torch.no_grad():
+        hidden_cpu = bert(input_ids=T(g["ids"]), attention_mask=T(g["mask"]))[0]
+    if not np.allclose(hidden_cpu.numpy(), g["hidden"], atol=1e-5):
+        pytest.skip("transformers RNG/initialisation differs from the fixture's")
+    t = AveragePoolingTower(projection_dim=64, tokenizer=lambda *a, **k: None, pretrained_model=bert, encoder_mode="bert", encoder_impl="hip")
+    with torch.no_grad():
+        t.projection[0].weight.copy_(T(g["w1"])); t.projection[0].bias.copy_(T(g["b1"]))
+        t.projection[2].weight.copy_(T(g["w2"])); t.projection[2].bias.copy_(T(g["b2"]))
+    t = t.cuda()
+    out = t.encode_ids(T(g["ids"]).cuda(), T(g["mask"]).cuda())
+    assert np.abs(out.detach().cpu().numpy() - g["out"]).max() <= 5e-5  # the bound the stock encoder's GPU forward is held to
+    assert [n for n, p in t.named_parameters() if p.requires_grad] == ["projection.0.weight", "projection.0.bias", "projection.2.weight", "projection.2.bias"]
+
+
+def test_feature_cache_and_autocast_on_the_packed_encoder():
+    from two_towers_overlords_amd.model import TwoTowersModel
+    from two_towers_overlords_amd.training import TripletTrainer
+
+    bert = tiny_bert()
+    ids, mask = batch(B=50, S=30)
+    caches = {}
+    for impl in ("torch", "hip"):
+        model = TwoTowersModel(projection_dim=16, tokenizer=lambda *a, **k: None, pretrained_model=bert, encoder_mode="bert", encoder_impl=impl).cuda()
+        tr = TripletTrainer(model, max_batch=8, max_seq_len=30)
+        caches[impl] = tr.build_feature_cache(ids, mask).clone()
+        if impl == "hip":
+            half = tr.build_feature_cache(ids, mask, encoder_autocast=torch.bfloat16).clone()
+    assert float((caches["torch"] - caches["hip"]).abs().max()) <= 2 * 2 * 8 * 8 * PRODUCT
+    # bf16: every value of the chain is rounded once to 2^-9 relative; 2 layers x 8 roundings, unit rows
+    assert 0 < float((half - caches["hip"]).abs().max()) <= 2 * 8 * 2.0 ** -8
+
+
+
+
+def reference_loss(m, head, ids, mask, qids, temperature):
+    """The same step in 64 bits on the stock forward."""
+    h = m(input_ids=ids, attention_mask=mask)[0] * mask.unsqueeze(-1)
+    x = F.normalize(h.sum(1) / mask.sum(1, keepdim=True), dim=1)
+    e = F.linear(F.relu(F.linear(x, head[0], head[1])), head[2], head[3])
+    q, d = F.normalize(e[: len(e) // 2], dim=1), F.normalize(e[len(e) // 2:], dim=1)
+    l = q @ d.t() / temperature
+    same = (qids[:, None] == qids[None]) & ~torch.eye(len(q), dtype=torch.bool, device=l.device)
+    l = l.masked_fill(same, -float("inf"))
+    return (torch.logsumexp(l, 1) - l.diagonal()).mean()
+
+
+def test_fine_tuning_step_through_every_operator():
+    """Encoder (linear, attention) -> pool -> projection -> in-batch softmax loss -> gradients of every weight."""
+    from two_towers_overlords_amd.model import InBatchSoftmaxLoss, TwoTowersModel
+
+    bert = tiny_bert()
+    ref = copy.deepcopy(bert).double()
+    model = TwoTowersModel(projection_dim=24, tokenizer=lambda *a, **k: None, pretrained_model=bert, encoder_mode="bert",
+                           encoder_impl="hip", train_encoder=True).cuda()
+    model.document_tower.projection.load_state_dict(model.query_tower.projection.state_dict())
+    ids, mask = batch(B=16, S=29, seed=5)
+    qids = torch.tensor([0, 1, 2, 1, 4, 5, 0, 7], device="cuda")
+    loss = InBatchSoftmaxLoss(temperature=0.1)(model.encode_query_ids(ids[:8], mask[:8]), model.encode_document_ids(ids[8:], mask[8:]), qids)
+    loss.backward()
+    head = [p.detach().double().requires_grad_(True) for p in model.query_tower.projection.parameters()]
+    want = reference_loss(ref, head, ids, mask, qids, 0.1)
+    want.backward()
+    depth = 2 * 2 * 8 * 8 * PRODUCT  # forward and backward
+    assert abs(float(loss) - float(want)) <= depth / 0.1
+    got = dict(bert.named_parameters())
+    scale = max(float(p.grad.abs().max()) for p in ref.parameters() if p.grad is not None)
+    checked = 0
+    for name, p in ref.named_parameters():
+        if p.grad is None:
+            assert got[name].grad is None or not bool(got[name].grad.any()), name  # the pooler
+            continue
+        err = float((got[name].grad - p.grad).norm())
+        assert err <= depth * max(float(p.grad.norm()), scale), (name, err, float(p.grad.norm()))
+        checked += 1
+    assert checked >= 30
+    for a, b, c in zip(model.query_tower.projection.parameters(), model.document_tower.projection.parameters(), head):
+        assert float((a.grad + b.grad - c.grad).norm()) <= depth * float(c.grad.norm())
+
+
+def test_train_epoch_fine_tunes_the_encoder_on_the_module_path():
+    from two_towers_overlords_amd.model import TripletLoss, TwoTowersModel
+    from two_towers_overlords_amd.training import TripletTrainer, train_epoch
+
+    bert = tiny_bert()
+    before = {n: p.detach().clone() for n, p in bert.named_parameters()}
+    model = TwoTowersModel(projection_dim=24, tokenizer=lambda *a, **k: None, pretrained_model=bert, encoder_mode="bert",
+                           encoder_impl="hip", train_encoder=True).cuda()
+    opt = torch.optim.Adam([p for p in model.parameters() if p.requires_grad], lr=1e-3)
+    batches = [tuple(batch(B=6, S=20, seed=10 * i + r) for r in range(3)) for i in range(3)]
+    avg = train_epoch(model, batches, TripletLoss(), opt, log_wandb=False)
+    assert np.isfinite(avg)
+    moved = [n for n, p in bert.named_parameters() if not torch.equal(p, before[n])]
+    assert any("attention.self.query" in n for n in moved) and any("word_embeddings" in n for n in moved)
+    with pytest.raises(ValueError, match="train_encoder"):
+        TripletTrainer(model, max_batch=4, max_seq_len=20)
+
+
+def test_encoder_refusals():
+    from two_towers_overlords_amd.encoder import PackedBertEncoder, attention_qkv, linear
+    from two_towers_overlords_amd.model import EmbeddingOnlyEncoder, AveragePoolingTower, InBatchSoftmaxLoss
+
+    tok = lambda *a, **k: None
+    with pytest.raises(ValueError, match="BERT-shaped"):
+        PackedBertEncoder(EmbeddingOnlyEncoder(torch.randn(8, 8)))
+    with pytest.raises(ValueError, match="bert"):
+        AveragePoolingTower(tokenizer=tok, pretrained_model=EmbeddingOnlyEncoder(torch.randn(8, 8)), encoder_mode="embed", encoder_impl="hip")
+    with pytest.raises(ValueError, match="encoder_impl"):
+        AveragePoolingTower(tokenizer=tok, pretrained_model=tiny_bert(), encoder_mode="bert", encoder_impl="triton")
+    with pytest.raises(ValueError, match="train_encoder"):
+        AveragePoolingTower(tokenizer=tok, pretrained_model=tiny_bert(), encoder_mode="bert", train_encoder=True)
+    with pytest.raises(ValueError, match="head size"):
+        PackedBertEncoder(tiny_bert(hidden=60, heads=5))
+    m = tiny_bert()
+    m.config.hidden_act = "tanh"
+    with pytest.raises(ValueError, match="hidden_act"):
+        PackedBertEncoder(m)
+    m = tiny_bert()
+    m.train()
+    PackedBertEncoder(m)(*batch())  # all dropout probabilities are 0
+    m.embeddings.dropout.p = 0.1
+    with pytest.raises(RuntimeError, match="dropout"):
+        PackedBertEncoder(m)(*batch())
+    with pytest.raises(ValueError, match="positions"):
+        PackedBertEncoder(tiny_bert(positions=20))(*batch())
+    with pytest.raises(ValueError, match="residual"):
+        linear(torch.randn(4, 8, device="cuda"), torch.randn(6, 8, device="cuda"), residual=torch.randn(6, device="cuda"))
+    with pytest.raises(ValueError, match="qkv"):
+        attention_qkv(torch.randn(4, 4, 8, device="cuda"), 4, torch.tensor([0, 4], dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError):
+        InBatchSoftmaxLoss()(torch.randn(4, 8, device="cuda"), torch.randn(5, 8, device="cuda"))
+
+
+def test_op_refusals():
+    from two_towers_overlords_amd import ops
+
+    z = lambda *s, **k: torch.zeros(*s, device="cuda", **k)
+    with pytest.raises(TypeError):
+        ops.linear_act(z(4, 8), z(4, 8, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        ops.linear_act(z(4, 8), z(4, 9))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.linear_act(z(4, 8), z(4, 8), residual=z(1, 4).expand(4, 4))
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.linear_act(z(8, 4).t(), z(4, 8))
+    with pytest.raises(ValueError, match="pre-activation"):
+        ops.linear_act_bwd(z(4, 4), z(4, 8), z(4, 8), None, "gelu")
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    q = z(4, 2, 32)
+    for kw in (dict(causal=True, prefix=z(1, dtype=torch.int32)), dict(scale=-1.0), dict(scale=float("inf")), dict(softcap=-1.0), dict(slopes=z(3)),
+               dict(prefix=z(2, dtype=torch.int32)), dict(key_mask=z(5, dtype=torch.bool)), dict(slopes=z(2).requires_grad_(True))):
+        with pytest.raises(ValueError):
+            ops.packed_attention(q, q, q, cu, **kw)
+    for kw in (dict(key_mask=z(4)), dict(prefix=z(1, dtype=torch.int64))):
+        with pytest.raises(TypeError):
+            ops.packed_attention(q, q, q, cu, **kw)
+    with pytest.raises(TypeError):
+        ops.packed_attention(q, q, q, cu.long())
+    with pytest.raises(ValueError, match="multiple"):
+        ops.packed_attention(z(4, 3, 32), q, q, cu)
+    with pytest.raises(ValueError, match="head_dim"):
+        ops.packed_attention(z(4, 2, 12), z(4, 2, 12), z(4, 2, 12), cu)
+    with pytest.raises(ValueError, match="aligned"):
+        ops.packed_attention(z(4, 2, 33)[:, :, 1:], q, q, cu)
+    with pytest.raises(ValueError):
+        ops.packed_attention(q, q, q, cu[:1])
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for kw in (dict(row_ids=t), dict(scale=0.0), dict(row_ids=t, cand_ids=t)):
+        with pytest.raises(ValueError):
+            ops.softmax_loss(z(4, 8), z(5, 8), t, **kw)
+    with pytest.raises(TypeError):
+        ops.softmax_loss(z(4, 8), z(5, 8), t.int())
+    with pytest.raises(ValueError):
+        ops.softmax_loss(z(4, 8), z(5, 9), t)
+
+
+def test_in_batch_softmax_loss_module():
+    from two_towers_overlords_amd.model import InBatchSoftmaxLoss, softmax_loss
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(33, 48, generator=g, device="cuda", requires_grad=True)
+    d = torch.randn(33, 48, generator=g, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 20, (33,), generator=g, device="cuda")
+    for qid in (None, ids):
+        loss = InBatchSoftmaxLoss(0.05)(q, d, qid)
+        gq, gd = torch.autograd.grad(loss * 3.0, (q, d))
+        Q, D = q.detach().double().requires_grad_(True), d.detach().double().requires_grad_(True)
+        l = F.normalize(Q, dim=1) @ F.normalize(D, dim=1).t() / 0.05
+        if qid is not None:
+            l = l.masked_fill((qid[:, None] == qid[None]) & ~torch.eye(33, dtype=torch.bool, device="cuda"), -float("inf"))
+        want = F.cross_entropy(l, torch.arange(33, device="cuda"))
+        wq, wd = torch.autograd.grad(want * 3.0, (Q, D))
+        tol = 20 * (48 + 33 + 16) * 2.0 ** -23  # logits of at most 20, sums of 48 and 33
+        assert abs(float(loss) - float(want)) <= tol
+        assert float((gq - wq).abs().max()) <= tol * float(wq.abs().max()) * 4 and float((gd - wd).abs().max()) <= tol * float(wd.abs().max()) * 4
+    # a sum over rows, each with its own upstream gradient
+    t = torch.randint(0, 33, (33,), generator=g, device="cuda")
+    c = torch.rand(33, generator=g, device="cuda")
+    (gq,) = torch.autograd.grad((softmax_loss(q, d, t) * c).sum(), q)
+    Q = q.detach().double().requires_grad_(True)
+    (wq,) = torch.autograd.grad((F.cross_entropy(Q @ d.detach().double().t(), t, reduction="none") * c).sum(), Q)
+    assert float((gq - wq).abs().max()) <= 40 * (48 + 33 + 16) * 2.0 ** -23 * float(d.abs().max()) * 33
+    assert float(InBatchSoftmaxLoss()(q[:0], d[:0])) == 0.0
+    with pytest.raises(ValueError):
+        InBatchSoftmaxLoss(0.0)
+
+
+def everything(ops, s, out=None):
+    """One call of every entry point on the tensors of `s`."""
+    y, z = ops.linear_act(s["x"], s["w"], s["b"], s["r"], "gelu", save_preact=True)
+    o, lse = ops.packed_attention(s["q"], s["k"], s["v"], s["cu"], slopes=s["slopes"], key_mask=s["keep"])
+    loss, l = ops.softmax_loss(s["x"], s["w"], s["t"], scale=2.0)
+    return [y, *ops.linear_act_bwd(s["r"], s["x"], s["w"], z, "gelu"), o, lse,
+            *ops.packed_attention_bwd(s["do"], s["q"], s["k"], s["v"], o, lse, s["cu"], slopes=s["slopes"], key_mask=s["keep"]),
+            loss, l, *ops.softmax_loss_bwd(s["c"], s["x"], s["w"], s["t"], l, scale=2.0)]
+
+
+def operands(dt, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dt)
+    return dict(x=r(700, 96), w=r(320, 96), b=r(320), r=r(700, 320), q=r(500, 4, 64), k=r(500, 2, 64), v=r(500, 2, 64), do=r(500, 4, 64),
+                cu=torch.tensor([0, 130, 131, 470], dtype=torch.int32, device="cuda"), slopes=torch.rand(4, generator=g, device="cuda"),
+                keep=torch.rand(500, generator=g, device="cuda") > 0.2, t=torch.randint(0, 320, (700,), generator=g, device="cuda"),
+                c=torch.rand(700, generator=g, device="cuda") / 700)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_two_streams_at_once(dt):
+    from two_towers_overlords_amd import ops
+
+    a, b = operands(dt, 1), operands(dt, 2)
+    wa, wb = everything(ops, a), everything(ops, b)
+    torch.cuda.synchronize()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(5):
+        with torch.cuda.stream(sa):
+            ga = everything(ops, a)
+        with torch.cuda.stream(sb):
+            gb = everything(ops, b)
+        outs.append((ga, gb))
+    torch.cuda.synchronize()
+    for ga, gb in outs:
+        assert all(torch.equal(x, y) for x, y in zip(ga, wa)) and all(torch.equal(x, y) for x, y in zip(gb, wb))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_captured_and_replayed(dt):
+    """Two graphs captured one after the other, replayed in turn with new inputs and eager work between: every replay equals
+    the eager call, bit for bit."""
+    from two_towers_overlords_amd import ops
+
+    states = [operands(dt, 1), operands(dt, 2)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for s in states:
+            everything(ops, s)
+    torch.cuda.synchronize()
+    graphs = []
+    for s in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = everything(ops, s)
+        graphs.append((g, out))
+    for it in range(4):
+        fresh = [operands(dt, 10 + 2 * it + i) for i in range(2)]
+        for s, f in zip(states, fresh):
+            for k in s:
+                s[k].copy_(f[k])
+        want = [everything(ops, f) for f in fresh]
+        for (g, out), w in zip(graphs, want):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, w)), it
+        graphs[0][0].replay()  # both in flight on one stream
+        graphs[1][0].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for (g, out), w in zip(graphs, want) for a, b in zip(out, w)), it
+
+
+def test_offsets_beyond_31_bits():
+    from two_towers_overlords_amd import ops
+
+    M, K, N = (1 << 21) + 5, 16, 1040  # 2.18e9 outputs
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+    w, b = torch.randn(N, K, generator=g, device="cuda").bfloat16(), torch.randn(N, generator=g, device="cuda").bfloat16()
+    y = ops.linear_act(x, w, b, None, "gelu")
+    for rows in (slice(0, 70), slice(M - 70, M)):
+        assert torch.equal(y[rows], ops.linear_act(x[rows].contiguous(), w, b, None, "gelu"))
+    dx, _, _ = ops.linear_act_bwd(y, x, w, y, "gelu", bias=False, need_dw=False)
+    assert torch.equal(dx[M - 70:], ops.linear_act_bwd(y[M - 70:].contiguous(), x[M - 70:], w, y[M - 70:].contiguous(), "gelu", bias=False, need_dw=False)[0])
+    del x, y, dx
+    tokens, H, Dh, doc = 1100032, 16, 128, 64  # 2.25e9 elements
+    q = torch.randn(tokens, H, Dh, generator=g, device="cuda", dtype=torch.bfloat16)
+    cu = torch.arange(0, tokens + 1, doc, dtype=torch.int32, device="cuda")
+    o, lse = ops.packed_attention(q, q, q, cu)
+    dq, dk, dv = ops.packed_attention_bwd(q, q, q, q, o, lse, cu)
+    one = torch.tensor([0, doc], dtype=torch.int32, device="cuda")
+    for rows in (slice(0, doc), slice(tokens - doc, tokens)):
+        s = q[rows].contiguous()
+        o1, l1 = ops.packed_attention(s, s, s, one)
+        assert torch.equal(o[rows], o1)
+        for a, c in zip((dq, dk, dv), ops.packed_attention_bwd(s, s, s, s, o1, l1, one)):
+            assert torch.equal(a[rows], c)
+    del q, o, dq, dk, dv
+    V, D = 5_700_001, 384  # 2.19e9 candidate elements
+    w = torch.randn(V, D, generator=g, device="cuda", dtype=torch.bfloat16)
+    x = torch.randn(3, D, generator=g, device="cuda", dtype=torch.bfloat16) * 0.05
+    t = torch.tensor([0, V // 2, V - 1], device="cuda")
+    loss, lse = ops.softmax_loss(x, w, t)
+    l = torch.cat([x.float() @ w[i:i + 1000000].float().t() for i in range(0, V, 1000000)], 1).double()
+    want = torch.logsumexp(l, 1) - l.gather(1, t[:, None]).squeeze(1)
+    assert float((loss - want).abs().max()) <= 64 * (D + 32) * 2.0 ** -23
+    _, dw = ops.softmax_loss_bwd(torch.ones(3, device="cuda"), x, w, t, lse, need_dx=False)
+    tail = slice(V - 1000, V)
+    G = torch.exp(l[:, tail] - torch.logsumexp(l, 1, keepdim=True))
+    G[2, -1] -= 1
+    ref = G.t() @ x.double()
+    assert float((dw[tail] - ref).abs().max()) <= 2.0 ** -7 * float(ref.abs().max())
+
+
+def test_another_current_device_is_left_alone():
+    """The launch follows the tensors' device; with one device: entering and leaving it changes nothing."""
+    from two_towers_overlords_amd import ops
+
+    before = torch.cuda.current_device()
+    everything(ops, operands(torch.float32, 3))
+    assert torch.cuda.current_device() == before

@@ -221,7 +221,7 @@ struct Plan {
   int pieces, sx, sw;   // splits of the two gradient products
   size_t x, w, part, tlogit, cmax, G, dx, dw, fwd, bwd;
 };
-constexpr long long kPieceBytes = 256LL << 20;  // of G: what the Infinity Cache holds
+constexpr long long kPieceBytes = 512LL << 20;  // of G; 8192 rows x 30522 bf16 candidates: 64 MB 1421 us, 128 1279, 256 1272, 512 1217
 Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long M, int V, int D, int dtype) {
   Plan p{};
   const int width = dtype_bytes(dtype);

@@ -23,6 +23,7 @@ import warnings
 from typing import Callable, Optional, Tuple
 
 import torch
+import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import ops
@@ -33,7 +34,8 @@ DEFAULT_MODEL_NAME = "sentence-transformers/all-MiniLM-L6-v2"
 class _ProjectionFn(torch.autograd.Function):
     """Linear(D,P) -> ReLU -> Linear(P,P) (backend/model.py:33-38,59) on the fp32
     MFMA kernels; gradients for the four parameters only (the input comes from the
-    frozen encoder under no_grad, backend/model.py:29-30,51)."""
+    frozen encoder under no_grad, backend/model.py:29-30,51; a trained encoder goes through
+    encoder.linear)."""
 
     @staticmethod
     def forward(ctx, x, w1, b1, w2, b2):
@@ -102,10 +104,18 @@ class AveragePoolingTower(nn.Module):
         tokenizer: Optional[Callable] = None,
         pretrained_model: Optional[nn.Module] = None,
         encoder_mode: Optional[str] = None,
+        encoder_impl: str = "torch",
+        train_encoder: bool = False,
     ):
+        """encoder_impl (`bert` mode): "torch" = the stock PyTorch forward, padded like the reference's; "hip" = the same
+        encoder on packed tokens and this package's kernels (encoder.PackedBertEncoder; equal up to rounding).
+        train_encoder (`bert` mode on "hip"): the encoder's weights are not frozen, and gradients reach them — an
+        extension, backend/model.py:29-30 always freezes them."""
         super().__init__()
         if encoder_mode not in (None, "embed", "bert"):
             raise ValueError("encoder_mode must be 'embed' or 'bert'")
+        if encoder_impl not in ("torch", "hip"):
+            raise ValueError("encoder_impl must be 'torch' or 'hip'")
         if tokenizer is None or pretrained_model is None:
             from transformers import AutoModel, AutoTokenizer  # same loaders as model.py:23-24
 
@@ -116,9 +126,19 @@ class AveragePoolingTower(nn.Module):
         self.tokenizer = tokenizer
         self.pretrained_model = pretrained_model
         self.encoder_mode = encoder_mode
+        self.encoder_impl = encoder_impl
+        self.train_encoder = bool(train_encoder)
+        if (encoder_impl == "hip" or train_encoder) and encoder_mode != "bert":
+            raise ValueError("encoder_impl='hip' and train_encoder are for encoder_mode='bert': `embed` has no encoder to run")
+        if train_encoder and encoder_impl != "hip":
+            raise ValueError("train_encoder needs encoder_impl='hip'")
+        if encoder_impl == "hip":
+            from .encoder import PackedBertEncoder
+
+            PackedBertEncoder(pretrained_model)  # refuses here what it cannot run
         self.embedding_dim = int(_hidden_size(pretrained_model))
         for param in self.pretrained_model.parameters():  # model.py:29-30
-            param.requires_grad = False
+            param.requires_grad = self.train_encoder
         # same container and default init as model.py:33-38, so state_dict keys are
         # projection.0.{weight,bias} / projection.2.{weight,bias}
         self.projection = nn.Sequential(
@@ -195,8 +215,19 @@ class AveragePoolingTower(nn.Module):
         return pm.word_embeddings.weight
 
     def pool_tokens(self, tokens: dict) -> Tensor:
-        """model.py:51-56 -> pooled, normalised [B, D] (no grad)."""
+        """model.py:51-56 -> pooled, normalised [B, D] (no grad, unless the tower trains its encoder)."""
         ids, mask = tokens["input_ids"], tokens.get("attention_mask")
+        if self.encoder_impl == "hip":
+            from .encoder import PackedBertEncoder
+
+            with torch.set_grad_enabled(torch.is_grad_enabled() and self.train_encoder):
+                hidden = PackedBertEncoder(self.pretrained_model).padded(ids, mask, tokens.get("token_type_ids"))
+                if not hidden.requires_grad:
+                    return ops.pool_norm_dense(hidden, None if mask is None else mask.contiguous())
+                # model.py:55-56,63-72, differentiable; tokens that are not attended are zero rows already
+                wt = torch.ones(ids.shape, device=ids.device) if mask is None else mask.float()
+                pooled = (hidden * wt.unsqueeze(-1)).sum(1) / wt.sum(1, keepdim=True).clamp(min=1e-9)
+                return F.normalize(pooled, p=2, dim=1)
         with torch.no_grad():
             if self.encoder_mode == "embed":
                 return ops.gather_pool_norm(self.embedding_table().detach(), ids.contiguous(),
@@ -211,6 +242,10 @@ class AveragePoolingTower(nn.Module):
     def project(self, pooled: Tensor) -> Tensor:
         """model.py:59: the trainable Linear -> ReLU -> Linear on pooled, normalised rows [B, D]."""
         p = self.projection
+        if pooled.requires_grad:  # a trained encoder: the gradient goes on into the pooled rows
+            from .encoder import linear
+
+            return linear(linear(pooled, p[0].weight, p[0].bias, activation="relu"), p[2].weight, p[2].bias)
         return _ProjectionFn.apply(pooled, p[0].weight, p[0].bias, p[2].weight, p[2].bias)
 
     def encode_ids(self, input_ids: Tensor, attention_mask: Optional[Tensor] = None) -> Tensor:
@@ -237,12 +272,15 @@ class TwoTowersModel(nn.Module):
         tokenizer: Optional[Callable] = None,
         pretrained_model: Optional[nn.Module] = None,
         encoder_mode: Optional[str] = None,
+        encoder_impl: str = "torch",
+        train_encoder: bool = False,
     ):
         super().__init__()
-        kw = dict(tokenizer=tokenizer, pretrained_model=pretrained_model, encoder_mode=encoder_mode)
+        kw = dict(tokenizer=tokenizer, pretrained_model=pretrained_model, encoder_mode=encoder_mode, encoder_impl=encoder_impl,
+                  train_encoder=train_encoder)
         self.query_tower = AveragePoolingTower(model_name, projection_dim, **kw)
         if pretrained_model is None:  # loaded from disk: share the frozen weights and tokenizer
-            kw = dict(tokenizer=self.query_tower.tokenizer, pretrained_model=self.query_tower.pretrained_model,
+            kw = dict(kw, tokenizer=self.query_tower.tokenizer, pretrained_model=self.query_tower.pretrained_model,
                       encoder_mode=self.query_tower.encoder_mode)
         self.document_tower = AveragePoolingTower(model_name, projection_dim, **kw)
 
@@ -325,6 +363,54 @@ class InBatchTripletLoss(nn.Module):
     def forward(self, anchor: Tensor, documents: Tensor, query_ids: Optional[Tensor] = None) -> Tensor:
         qid = None if query_ids is None else query_ids.to(torch.int64).contiguous()
         return _InBatchLossFn.apply(anchor, documents, self.margin, qid)
+
+
+class _SoftmaxLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, target, scale, row_ids, cand_ids, ignore_index):
+        loss, lse = ops.softmax_loss(x, w, target, scale, row_ids, cand_ids, ignore_index)
+        ctx.kw = dict(scale=scale, ignore_index=ignore_index)
+        ctx.save_for_backward(x, w, target, lse, row_ids, cand_ids)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, w, target, lse, row_ids, cand_ids = ctx.saved_tensors
+        nx, nw = ctx.needs_input_grad[:2]
+        dx, dw = ops.softmax_loss_bwd(g.contiguous(), x, w, target, lse, row_ids=row_ids, cand_ids=cand_ids, need_dx=nx, need_dw=nw, **ctx.kw)
+        return dx, dw, None, None, None, None, None
+
+
+def softmax_loss(x: Tensor, candidates: Tensor, target: Tensor, *, scale: float = 1.0, row_ids: Optional[Tensor] = None,
+                 cand_ids: Optional[Tensor] = None, ignore_index: int = -100) -> Tensor:
+    """`ops.softmax_loss`, differentiable in x [N, D] and candidates [V, D] -> the rows' losses [N] (float32)."""
+    return _SoftmaxLossFn.apply(x, candidates, target, float(scale), row_ids, cand_ids, int(ignore_index))
+
+
+class InBatchSoftmaxLoss(nn.Module):
+    """Softmax loss over ALL in-batch documents (not in the reference, which samples one negative per item): for query i,
+    document i is the target among every document of the batch,
+        mean_i -log softmax_j(cos(q_i, d_j) / temperature)[i],
+    on cosine similarities like `TripletLoss`; with `query_ids`, other documents of the same query are left out of a query's
+    sum (like data.py:124-128).  The B x B similarities are never stored.  An empty batch gives 0."""
+
+    def __init__(self, temperature: float = 0.05):
+        super().__init__()
+        if not temperature > 0:
+            raise ValueError("temperature must be positive")
+        self.temperature = temperature
+
+    def forward(self, anchor: Tensor, documents: Tensor, query_ids: Optional[Tensor] = None) -> Tensor:
+        if anchor.shape != documents.shape:
+            raise ValueError(f"anchor {tuple(anchor.shape)} and documents {tuple(documents.shape)}: document i belongs to query i")
+        B = anchor.shape[0]
+        q, d = F.normalize(anchor, dim=1, eps=1e-8), F.normalize(documents, dim=1, eps=1e-8)
+        qid = None if query_ids is None else query_ids.to(torch.int64).contiguous()
+        target = torch.arange(B, device=anchor.device)
+        if B == 0:
+            return (q.sum() + d.sum()).float()
+        return softmax_loss(q, d, target, scale=1.0 / self.temperature, row_ids=qid, cand_ids=qid).mean()
 
 
 class EmbeddingOnlyEncoder(nn.Module):

@@ -60,6 +60,9 @@ class TripletTrainer(CalibrationMixin, ExchangeMixin, GraphReplayMixin):
             # between gather and pool): the encoder is not part of the fused step — its pooled outputs are computed
             # once per text by build_feature_cache() (stock PyTorch ops + the dense pool kernel) and the step is fed
             # from that cache; the table is bound only because the engine wants one.
+            if getattr(model.query_tower, "train_encoder", False) or getattr(model.document_tower, "train_encoder", False):
+                raise ValueError("TripletTrainer trains the projections over a frozen encoder; a model built with train_encoder=True "
+                                 "is trained by train_epoch's module path")
             encoder_mode = model.query_tower.encoder_mode
             table = model.query_tower.embedding_table().detach()
             tensors = [p.detach() for p in model.trainable_parameters()]

@@ -582,7 +582,7 @@ def run_training(num_epochs: int = 3, batch_size: int = 1024, learning_rate: flo
                  tokenizer=None, pretrained_model=None, model_name: Optional[str] = None,
                  seed: Optional[int] = None, feature_cache: bool = True, sampler: str = "device",
                  encoder_mode: Optional[str] = None, calibrate: bool = True, three_encodes: bool = False,
-                 encoder_autocast: Optional[str] = None) -> TwoTowersModel:
+                 encoder_autocast: Optional[str] = None, encoder_impl: str = "torch") -> TwoTowersModel:
     """Same keyword surface and defaults as backend/training.py:383-397; builds the
     model / criterion / Adam exactly like :433-436 and runs `num_epochs` epochs on
     the fused engine.  Differences, all outside the hot path: the datasets are passed
@@ -603,7 +603,9 @@ def run_training(num_epochs: int = 3, batch_size: int = 1024, learning_rate: flo
     backend/data.py:132-137's draws under `seed`, at its O(B^2) Python cost per batch.
     `encoder_autocast` ("fp16" | "bf16"; `bert` mode; NOT the parity path): the frozen encoder's one pass per text runs under
     `torch.autocast` — what `use_mixed_precision=True` means for the encoder in the reference's GPU loop (training.py:83);
-    projections, loss and Adam stay fp32.  `use_mixed_precision` itself stays ignored so that a default call is the parity path."""
+    projections, loss and Adam stay fp32.  `encoder_impl="hip"` (`bert` mode) runs the encoder's one pass per text on packed
+    tokens and this package's kernels (encoder.PackedBertEncoder) instead of the stock padded forward; equal up to rounding,
+    with either type.  `use_mixed_precision` itself stays ignored so that a default call is the parity path."""
     from .data import TokenTripletLoader
 
     if train_dataset is None:
@@ -621,7 +623,7 @@ def run_training(num_epochs: int = 3, batch_size: int = 1024, learning_rate: flo
     if model_name is not None:
         kw["model_name"] = model_name
     model = TwoTowersModel(projection_dim=projection_dim, tokenizer=tokenizer, pretrained_model=pretrained_model,
-                           encoder_mode=encoder_mode, **kw)
+                           encoder_mode=encoder_mode, encoder_impl=encoder_impl, **kw)
     model = model.to(device)
     encoder_mode = model.query_tower.encoder_mode
     if max_samples and max_samples > 0 and len(train_dataset) > max_samples:
