@@ -721,16 +721,16 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         sc = capped<T>(s, a);
         s = biased<T>(sc, bias, t);
       }
-      f32x16 ls, de;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        ls[e] = stat[32 * t + row_of<T>(e, h)];
-        de[e] = stat[D::TILE + 32 * t + row_of<T>(e, h)];
-      }
+      for (int q = 0; q < 4; ++q) {  // four rows' lse and delta at a time
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + 32 * t + row_of<T>(4 * q, h));
+        const f32x4 de = *reinterpret_cast<const f32x4*>(stat + D::TILE + 32 * t + row_of<T>(4 * q, h));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, off) - ls[e]);
-        dp[e] = s[e] * (dp[e] - de[e]);
+        for (int i = 0; i < 4; ++i) {
+          const int e = 4 * q + i;
+          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, PLAIN ? -ls[i] : off - ls[i]));
+          dp[e] = s[e] * (dp[e] - de[i]);
+        }
       }
       if constexpr (!PLAIN) dp = through_cap(dp, sc, a);
       if (masked) {

@@ -16,14 +16,31 @@ namespace {
 constexpr float kRsqrt2 = 0.70710678118654752f, kRsqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluC = 0.79788456080286536f, kGeluA = 0.044715f;
 
-// erf.  16-bit results: Abramowitz & Stegun 7.1.26, |error| <= 1.5e-7 — 2^-14 of a bf16 step of 1.
+// Phi(z) = erfc(-z / sqrt 2) / 2 and e = exp(-z^2 / 2), which gelu's derivative needs as well.  erfc(a) = t Q(t) exp(-a^2) with
+// t = 1 / (1 + p a), a = |z| / sqrt 2, no cancellation on the negative side.  16-bit results: Abramowitz & Stegun 7.1.26,
+// |error| <= 1.5e-7, 2^-14 of a bf16 step of 1.  float: p = 0.5 and a polynomial of degree 8 fitted to exp(a^2) erfc(a) / t in the
+// Chebyshev sense on 0 <= a <= 10 (relative error 4e-8); erff cost a quarter of the epilogue's time.
 template <bool FAST>
-__device__ __forceinline__ float erf_(float x) {
-  if constexpr (!FAST) return erff(x);
-  const float a = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * a * a);
-  return copysignf(fmaf(-p, e, 1.f), x);
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float a = fabsf(z) * kRsqrt2;
+  e = __builtin_amdgcn_exp2f(-1.4426950408889634f * (a * a));
+  float q, t;
+  if constexpr (FAST) {
+    t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
+    q = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  } else {
+    t = __builtin_amdgcn_rcpf(fmaf(0.5f, a, 1.f));
+    q = fmaf(t, -0.05906921625137329f, 0.2845761775970459f);
+    q = fmaf(t, q, -0.48720231652259827f);
+    q = fmaf(t, q, 0.27806979417800903f);
+    q = fmaf(t, q, -0.02662738598883152f);
+    q = fmaf(t, q, 0.2026875615119934f);
+    q = fmaf(t, q, 0.24310359358787537f);
+    q = fmaf(t, q, 0.2823753356933594f);
+    q = fmaf(t, q, 0.28208640217781067f);
+  }
+  const float half = 0.5f * (t * q) * e;
+  return z > 0.f ? 1.f - half : half;
 }
 template <bool FAST>
 __device__ __forceinline__ float exp_(float x) {
@@ -37,7 +54,11 @@ __device__ __forceinline__ float inv_(float x) {
 template <int ACT, bool FAST>
 __device__ __forceinline__ float act_(float z) {
   if constexpr (ACT == TT_ACT_RELU) return z < 0.f ? 0.f : z;
-  if constexpr (ACT == TT_ACT_GELU) return 0.5f * z * (1.f + erf_<FAST>(z * kRsqrt2));
+  if constexpr (ACT == TT_ACT_GELU) {
+    float e;
+    const float y = z * normal_cdf<FAST>(z, e);
+    return z < -40.f ? 0.f : y;  // -inf * 0
+  }
   if constexpr (ACT == TT_ACT_GELU_TANH) {  // z / (1 + exp(-2u)) = 0.5 z (1 + tanh u)
     const float u = kGeluC * z * fmaf(kGeluA * z, z, 1.f);
     return z * inv_<FAST>(1.f + exp_<FAST>(-2.f * u));
@@ -51,8 +72,11 @@ __device__ __forceinline__ float dact_(float z) {
   if constexpr (ACT == TT_ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
   if constexpr (ACT == TT_ACT_NONE) return 1.f;
   z = z > 40.f ? 40.f : (z < -40.f ? -40.f : z);
-  if constexpr (ACT == TT_ACT_GELU)
-    return fmaf(z * kRsqrt2Pi, exp_<FAST>(-0.5f * z * z), 0.5f * (1.f + erf_<FAST>(z * kRsqrt2)));
+  if constexpr (ACT == TT_ACT_GELU) {
+    float e;
+    const float p = normal_cdf<FAST>(z, e);
+    return fmaf(z * kRsqrt2Pi, e, p);
+  }
   if constexpr (ACT == TT_ACT_GELU_TANH) {
     const float u = kGeluC * z * fmaf(kGeluA * z, z, 1.f);
     const float s = inv_<FAST>(1.f + exp_<FAST>(-2.f * u));  // (1 + tanh u) / 2;  1 - tanh^2 = 4 s (1 - s)
@@ -156,6 +180,65 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
     return;
   }
   with_act(a.act, [&](auto tag) { epilogue<T, decltype(tag)::value>(blk, a, b0, b1, m0, n0); });
+}
+
+// Few rows (a query's tokens): a tile of 64 x 64 leaves most of the chip idle and walks K alone.  Here a workgroup forms 32 x 32
+// outputs with eight waves, each on every eighth 32-byte pair of chunks of K, its operands straight from memory into registers
+// (up to kFewAhead groups in flight), and the waves' sums meet in LDS, added in wave order.  Weight reads bound it.
+constexpr int kFewWaves = 8, kFewAhead = 6;
+template <class T>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(FwdArgs a) {
+  constexpr int KPF = Type<T>::KPF;
+  __shared__ __align__(16) float red[kFewWaves][32][36];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
+  const int m0 = blockIdx.x / a.gn * 32, n0 = blockIdx.x % a.gn * 32, M = a.s.M, N = a.s.N, K = a.s.K;
+  const T* __restrict__ x = static_cast<const T*>(a.X.p) + min(m0 + r, M - 1) * a.X.ld + h * KPF;
+  const T* __restrict__ w = static_cast<const T*>(a.W.p) + min(n0 + r, N - 1) * a.W.ld + h * KPF;
+  f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  for (int k0 = wave * 2 * KPF; k0 < K; k0 += kFewAhead * kFewWaves * 2 * KPF) {
+    u32x4 fx[kFewAhead], fw[kFewAhead];
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int k = k0 + i * kFewWaves * 2 * KPF;
+      fx[i] = fw[i] = u32x4{0, 0, 0, 0};
+      if (k + h * KPF < K) {  // a chunk that starts inside K is readable, and zero behind it
+        fx[i] = *reinterpret_cast<const u32x4*>(x + k);
+        fw[i] = *reinterpret_cast<const u32x4*>(w + k);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i)
+      if (k0 + i * kFewWaves * 2 * KPF < K) mma<T>(acc, fw[i], fx[i]);  // uniform
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const f32x4 v = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    *reinterpret_cast<f32x4*>(&red[wave][r][8 * q + 4 * h]) = v;
+  }
+  __syncthreads();
+  const int row = threadIdx.x >> 4, c = (threadIdx.x & 15) * 2, m = m0 + row;  // two columns per thread
+  if (m >= M) return;
+  float z[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) {
+    z[0] += red[i][row][c];
+    z[1] += red[i][row][c + 1];
+  }
+  with_act(a.act, [&](auto tag) {
+    constexpr int ACT = decltype(tag)::value;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int n = n0 + c + e;
+      if (n >= N) break;
+      if (a.bias) z[e] += (float)static_cast<const T*>(a.bias)[n];
+      if (a.z) static_cast<T*>(a.z)[(long long)m * N + n] = (T)kept<T>(f32x4{z[e], 0.f, 0.f, 0.f}, ACT)[0];
+      float y = act_<ACT, sizeof(T) == 2>(z[e]);
+      if (a.res) y += (float)static_cast<const T*>(a.res)[m * a.ldr + n];
+      static_cast<T*>(a.y)[m * a.ldy + n] = (T)y;
+    }
+  });
 }
 
 // dz = dy act'(z) (written when dz != null, row stride ldz) and, per block of rows, the column sums of dz.  Memory-bound.
@@ -431,6 +514,18 @@ extern "C" int tt_linear_act(const void* x, int64_t ldx, const void* w, int64_t 
   a.s = Shape{(int)M, N, K, K};
   a.bias = bias; a.res = residual; a.y = y; a.z = preact; a.ldr = ldr; a.ldy = ldy; a.act = act;
   a.vec = N % (16 / width) == 0 && chunk_ok(bias, 0, width) && chunk_ok(residual, ldr, width) && chunk_ok(y, ldy, width) && chunk_ok(preact, N, width);
+  // one round of 32 x 32 workgroups: measured against 64-wide tiles, K = 384 / 1536, N = 1536 / 384, gelu: 11 rows float 11.0 ->
+  // 5.5 us / 30.3 -> 14.6, bf16 4.5 -> 3.6 / 8.6 -> 6.3; at two rounds (N = 1536, 256 rows) 11.6 against 11.2, bf16 4.8 against 5.5
+  if (((M + 31) / 32) * ((N + 31) / 32) <= 256) {
+    a.gm = (int)((M + 31) / 32);
+    a.gn = (N + 31) / 32;
+    return with_type(dtype, [&](auto tag) {
+      using T = decltype(tag);
+      hipLaunchKernelGGL(linear_few_kernel<T>, dim3((unsigned)(a.gm * a.gn)), dim3(64 * kFewWaves), 0, st, a);
+      TT_CHECK_LAUNCH();
+      return (int)TT_OK;
+    });
+  }
   const int b = pick_tile(M, N, 1, dtype);
   a.gm = (int)((M + b - 1) / b);
   a.gn = (N + b - 1) / b;

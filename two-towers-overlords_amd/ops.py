@@ -7,6 +7,7 @@ GPU tensor and the HIP library these functions raise.
 """
 from __future__ import annotations
 
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -30,6 +31,16 @@ class _NoSwitch:
 
 
 _NO_SWITCH = _NoSwitch()
+
+
+def _stream_on(device: torch.device) -> int:
+    """The current stream of `device`, without the Stream object that torch.cuda.current_stream() builds (3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _enter(device: torch.device):
+    """`_on` for a device with an index (a tensor's), without torch.cuda.current_device()'s lazy-init check."""
+    return _NO_SWITCH if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _on(device: torch.device):
@@ -496,11 +507,11 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     ldy = _rows(y, "out", like=x, shape=(M, N))
     z = torch.empty((M, N), dtype=x.dtype, device=x.device) if save_preact and act else None
     if M:
-        with _on(x.device):
+        with _enter(x.device):
             nbytes = _lib.load().tt_linear_act_workspace_bytes(x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K, dt)
             ws = _workspace(nbytes, x.device) if nbytes else None
             call("tt_linear_act", x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(bias), _ptr(residual), ldr, y.data_ptr(), ldy, _ptr(z),
-                 M, N, K, dt, act, _ptr(ws), nbytes, _stream())
+                 M, N, K, dt, act, _ptr(ws), nbytes, _stream_on(x.device))
     return (y, z) if save_preact else y
 
 
@@ -527,40 +538,58 @@ def linear_act_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact: O
     dw = torch.empty((N, K), dtype=x.dtype, device=x.device) if need_dw else None
     db = torch.empty(N, dtype=x.dtype, device=x.device) if bias else None
     if dx is not None or dw is not None or db is not None:
-        with _on(x.device):
+        with _enter(x.device):
             nbytes = _lib.load().tt_linear_act_bwd_workspace_bytes(dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K,
                                                                    dt, act)
             ws = _workspace(nbytes, x.device)
             call("tt_linear_act_bwd", dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(preact) if act else None,
-                 _ptr(dx), _ptr(dw), _ptr(db), M, N, K, dt, act, ws.data_ptr(), nbytes, _stream())
+                 _ptr(dx), _ptr(dw), _ptr(db), M, N, K, dt, act, ws.data_ptr(), nbytes, _stream_on(x.device))
     return dx, dw, db
 
 
-def _head_view(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, shape=None) -> _lib.TTHeadView:
+def _head_view(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, shape=None) -> Tuple[int, int, int]:
+    """(data pointer, token stride, head stride) of a [tokens, heads, head_dim] operand: a tt_head_view."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t)}")
     if not t.is_cuda:
         _req(t, name)
-    if t.dim() != 3 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{name}: expected shape {'[tokens, heads, head_dim]' if shape is None else tuple(shape)}, got {tuple(t.shape)}")
+    ts = t.shape
+    if len(ts) != 3 or (shape is not None and ts != shape):
+        raise ValueError(f"{name}: expected shape {'[tokens, heads, head_dim]' if shape is None else tuple(shape)}, got {tuple(ts)}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise TypeError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
     st, sh, sd = t.stride()
-    st, sh = (0 if t.shape[0] <= 1 else st), (0 if t.shape[1] <= 1 else sh)
-    kpf = 16 // t.element_size()
-    if sd != 1 or st % kpf or sh % kpf or t.data_ptr() % 16:
+    if ts[0] <= 1:
+        st = 0
+    if ts[1] <= 1:
+        sh = 0
+    p = t.data_ptr()
+    size = t.element_size()
+    if sd != 1 or st * size % 16 or sh * size % 16 or p % 16:
         raise ValueError(f"{name}: head_dim must be contiguous, rows and base 16-byte aligned (stride {t.stride()})")
-    return _lib.TTHeadView(t.data_ptr(), st, sh)
+    return p, st, sh
 
 
-def _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask) -> _lib.TTAttentionArgs:
-    a = _lib.TTAttentionArgs()
-    a.dtype = _float_type(q, "q")
-    a.q = _head_view(q, "q")
+_NO_VIEW = (0, 0, 0)
+_ATTENTION_PACK = struct.Struct("=24q6qq6i2f").pack  # tt_attention_args
+
+
+def _attention_call(fn, dt, views, lse, delta, cu_seqlens, mask, T, docs, H, Hkv, Dh) -> None:
+    scale, causal, prefix, softcap, slopes, key_mask = mask
+    flat = [x for v in views for x in v]
+    raw = _ATTENTION_PACK(*flat, lse, delta, cu_seqlens.data_ptr(), _ptr(prefix) or 0, _ptr(slopes) or 0, _ptr(key_mask) or 0, T, docs, H,
+                          Hkv, Dh, dt, 1 if causal else 0, scale, softcap)
+    call(fn, _lib.TTAttentionArgs.from_buffer_copy(raw), _stream_on(cu_seqlens.device))
+
+
+def _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask):
+    """Checks everything but the outputs -> (element type, views of q, k, v, the masks' arguments, T, documents, H, Hkv, Dh)."""
+    dt = _float_type(q, "q")
+    vq = _head_view(q, "q")
     T, H, Dh = q.shape
     Hkv = k.shape[1] if k.dim() == 3 else 0
-    a.k = _head_view(k, "k", like=q, shape=(T, Hkv, Dh))
-    a.v = _head_view(v, "v", like=q, shape=(T, Hkv, Dh))
+    kv_shape = torch.Size((T, Hkv, Dh))
+    vk, vv = _head_view(k, "k", q, kv_shape), _head_view(v, "v", q, kv_shape)
     if H < 1 or Hkv < 1 or H % Hkv:
         raise ValueError(f"packed_attention: {H} query heads are not a multiple of {Hkv} key heads")
     if not 8 <= Dh <= 128 or Dh % 8:
@@ -587,10 +616,7 @@ def _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes,
     scale = Dh ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf") or not 0.0 <= softcap < float("inf"):
         raise ValueError(f"packed_attention: scale must be positive and softcap >= 0, got {scale}, {softcap}")
-    a.T, a.docs, a.heads, a.kv_heads, a.head_dim, a.causal = T, docs, H, Hkv, Dh, int(bool(causal))
-    a.scale, a.softcap = scale, softcap
-    a.cu_seqlens, a.prefix, a.slopes, a.key_mask = cu_seqlens.data_ptr(), _ptr(prefix), _ptr(slopes), _ptr(key_mask)
-    return a
+    return dt, [vq, vk, vv], (scale, causal, prefix, softcap, slopes, key_mask), T, docs, H, Hkv, Dh
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: Optional[float] = None,
@@ -604,13 +630,13 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     scores become softcap * tanh(score / softcap); slopes [H] float32: slopes[h] * |i - j| is subtracted.  A query that sees
     nothing gets 0 (lse -inf).  What masked keys hold does not matter, NaN included.
     The attention of the frozen encoder (backend/model.py:51-52) without its padding."""
-    a = _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((a.heads, a.T), dtype=torch.float32, device=q.device)
-    if a.T:
-        a.out, a.lse = _head_view(out, "out"), lse.data_ptr()
-        with _on(q.device):
-            call("tt_packed_attention", a, _stream())
+    dt, views, mask, T, docs, H, Hkv, Dh = _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask)
+    out = torch.empty((T, H, Dh), dtype=q.dtype, device=q.device)
+    lse = torch.empty((H, T), dtype=torch.float32, device=q.device)
+    if T:
+        views += [(out.data_ptr(), H * Dh, Dh)] + [_NO_VIEW] * 4
+        with _enter(q.device):
+            _attention_call("tt_packed_attention", dt, views, lse.data_ptr(), 0, cu_seqlens, mask, T, docs, H, Hkv, Dh)
     return out, lse
 
 
@@ -621,23 +647,19 @@ def packed_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     """Gradients of `packed_attention` -> (dq, dk, dv), given its arguments and what it returned.  grads: (dq, dk, dv) to write
     into — column blocks of one buffer, say, when q, k, v are; they may not overlap the inputs.  No atomics: the same
     inputs give the same bits."""
-    a = _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask)
-    a.out = _head_view(out, "out", like=q, shape=q.shape)
-    a.dout = _head_view(dout, "dout", like=q, shape=q.shape)
+    dt, views, mask, T, docs, H, Hkv, Dh = _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask)
+    views += [_head_view(out, "out", q, q.shape), _head_view(dout, "dout", q, q.shape)]
     _req(lse, "lse", torch.float32, 2)
-    if tuple(lse.shape) != (a.heads, a.T) or lse.device != q.device:
-        raise ValueError(f"lse: expected shape {(a.heads, a.T)} on {q.device}")
+    if tuple(lse.shape) != (H, T) or lse.device != q.device:
+        raise ValueError(f"lse: expected shape {(H, T)} on {q.device}")
     if grads is None:
         grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     dq, dk, dv = grads
-    a.dq = _head_view(dq, "dq", like=q, shape=q.shape)
-    a.dk = _head_view(dk, "dk", like=q, shape=k.shape)
-    a.dv = _head_view(dv, "dv", like=q, shape=v.shape)
-    if a.T:
-        delta = torch.empty((a.heads, a.T), dtype=torch.float32, device=q.device)
-        a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
-        with _on(q.device):
-            call("tt_packed_attention_bwd", a, _stream())
+    views += [_head_view(dq, "dq", q, q.shape), _head_view(dk, "dk", q, k.shape), _head_view(dv, "dv", q, v.shape)]
+    if T:
+        delta = torch.empty((H, T), dtype=torch.float32, device=q.device)
+        with _enter(q.device):
+            _attention_call("tt_packed_attention_bwd", dt, views, lse.data_ptr(), delta.data_ptr(), cu_seqlens, mask, T, docs, H, Hkv, Dh)
     return dq, dk, dv
 
 
@@ -673,11 +695,11 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, scale: 
     loss = torch.empty(N, dtype=torch.float32, device=x.device)
     lse = torch.empty(N, dtype=torch.float32, device=x.device)
     if N:
-        with _on(x.device):
+        with _enter(x.device):
             nbytes = _lib.load().tt_softmax_loss_workspace_bytes(x.data_ptr(), ldx, w.data_ptr(), ldw, N, V, D, dt)
             ws = _workspace(nbytes, x.device)
             call("tt_softmax_loss", x.data_ptr(), ldx, w.data_ptr(), ldw, target.data_ptr(), _ptr(row_ids), _ptr(cand_ids), N, V, D, dt,
-                 float(scale), int(ignore_index), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes, _stream())
+                 float(scale), int(ignore_index), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes, _stream_on(x.device))
     return loss, lse
 
 
@@ -694,10 +716,10 @@ def softmax_loss_bwd(row_coef: torch.Tensor, x: torch.Tensor, w: torch.Tensor, t
     dx = torch.empty((N, D), dtype=x.dtype, device=x.device) if need_dx else None
     dw = torch.empty((V, D), dtype=x.dtype, device=x.device) if need_dw else None
     if dx is not None or dw is not None:
-        with _on(x.device):
+        with _enter(x.device):
             nbytes = _lib.load().tt_softmax_loss_bwd_workspace_bytes(x.data_ptr(), ldx, w.data_ptr(), ldw, N, V, D, dt)
             ws = _workspace(nbytes, x.device)
             call("tt_softmax_loss_bwd", row_coef.data_ptr(), x.data_ptr(), ldx, w.data_ptr(), ldw, target.data_ptr(), _ptr(row_ids),
                  _ptr(cand_ids), lse.data_ptr(), N, V, D, dt, float(scale), int(ignore_index), _ptr(dx), _ptr(dw), ws.data_ptr(),
-                 nbytes, _stream())
+                 nbytes, _stream_on(x.device))
     return dx, dw
