@@ -19,7 +19,7 @@ using namespace ttm;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.9259629911e-8f;  // log2 e = the sum
 constexpr float kF16Up = 16384.f;
 
 struct Args {
@@ -135,10 +135,11 @@ __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restr
   const float base = mx == -INFINITY ? 0.f : mx;
   sum = 0.f;
   for (int t = 0; t < 16; ++t) sum += red[rl][t].y * __builtin_amdgcn_exp2f(red[rl][t].x - base);
-  const float l2 = mx == -INFINITY && sum == 0.f ? -INFINITY : base + log2f(sum);
-  lse[m] = l2 * kLn2;
+  // in 64 bits, a row each: a row whose target is nearly certain has a loss far below its lse's rounding
+  const double l = log2((double)sum), ln2 = 0.6931471805599453094;
+  lse[m] = mx == -INFINITY && sum == 0.f ? -INFINITY : (float)((base + l) * ln2);
   const long long t = target[m];
-  loss[m] = t == ignore ? 0.f : (t < 0 || t >= V ? NAN : (l2 - tlogit[m]) * kLn2);
+  loss[m] = t == ignore ? 0.f : (t < 0 || t >= V ? NAN : (float)(((double)base - tlogit[m] + l) * ln2));
 }
 
 // G of a piece of the candidates, [M, ldg] in T; columns behind the last candidate are zero
@@ -159,12 +160,14 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
       [&](int j, int s, int m, int nl, f32x4 (&v)[R::Q]) {
         if (m >= a.s.M || nl >= a.ldg) return;
         const long long t = a.target[m];
-        const float lse2 = a.lse[m] * kLog2e, c = t == a.ignore ? 0.f : (t < 0 || t >= a.V ? NAN : a.coef[m] * up);
+        const float lse = a.lse[m], c = t == a.ignore ? 0.f : (t < 0 || t >= a.V ? NAN : a.coef[m] * up);
+        // lse in base 2 as two floats; the second one scales the row
+        const float lse2 = lse * kLog2e, cp = c * __builtin_amdgcn_exp2f(-fmaf(lse, kLog2e, -lse2) - lse * kLog2eLow);
         const int n = a.v0 + nl;
 #pragma unroll
         for (int q = 0; q < R::Q; ++q)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[q][e] = c * __builtin_amdgcn_exp2f(fmaf(v[q][e], a.scale2, -lse2));
+          for (int e = 0; e < 4; ++e) v[q][e] = cp * __builtin_amdgcn_exp2f(fmaf(v[q][e], a.scale2, -lse2));
         if (t >= n && t < n + 4 * R::Q) {
 #pragma unroll
           for (int q = 0; q < R::Q; ++q)
