@@ -534,6 +534,39 @@ def test_softmax_loss_no_rows(ops):
 
 
 def test_softmax_loss_in_several_pieces(ops):
-    """More gradient entries than one piece of the candidates holds: dx is summed over the pieces, dw comes piece by piece."""
+    """More gradient entries than one piece holds: 16-bit types sum dx over pieces of the candidates, float sums dw over pieces
+    of the rows."""
     check_softmax(ops, torch.float32, 4099, 17003, 24, groups=True, ignore=(0, 4098))
+    check_softmax(ops, torch.float32, 4099, 40003, 24, groups=True, ignore=(0, 4098))
+    check_softmax(ops, torch.bfloat16, 4099, 70003, 16)
     check_softmax(ops, torch.float16, 4099, 33001, 24)
+
+
+@pytest.mark.parametrize("scale", [20.0, 60.0])
+def test_softmax_loss_of_nearly_certain_targets_keeps_its_digits(ops, scale):
+    """float: loss and gradient of rows whose target takes all but 1e-6 .. 1e-20 of the probability are good to a relative error,
+    not to the rounding of an lse of 20 or 60."""
+    g = gen(5)
+    w = randn(g, 300, 64)
+    w /= w.norm(dim=1, keepdim=True)
+    x = w[:200] + 0.02 * randn(g, 200, 64)
+    x /= x.norm(dim=1, keepdim=True)
+    t = torch.arange(200, device="cuda")
+    loss, lse = ops.softmax_loss(x, w, t, scale=scale)
+    dx, _ = ops.softmax_loss_bwd(torch.ones(200, device="cuda"), x, w, t, lse, scale=scale)
+    l = x.double() @ w.double().t() * scale
+    d = l - l.gather(1, t[:, None])
+    d.scatter_(1, t[:, None], -math.inf)
+    rest = torch.exp(d).sum(1)  # loss = log(1 + rest)
+    # the differences of two logits carry (64 + F) e scale 2 absolute; the target's own term is 1, and after it come at most 4 + 2
+    # additions in its lane, 1 between lanes, 1 between waves, 5 of tiles and 15 of their lanes: 28 roundings of 2^-24
+    rel = 2 * (64 + F) * E * scale
+    within("loss", loss, torch.log1p(rest), rel * rest + 28 * E / 2 + E * torch.log1p(rest))
+    p = torch.exp(d - torch.log1p(rest)[:, None])
+    p.scatter_(1, t[:, None], 0.0)
+    G = p.clone()
+    G.scatter_(1, t[:, None], -p.sum(1, keepdim=True))
+    DX = G @ w.double() * scale
+    # the row's common factor exp(-lse) carries lse's rounding, 2^-24 of |lse| <= scale + log 300, once
+    rg = rel + E * (scale + 8) + (300 + F) * E
+    within("dx", dx, DX, 4 * rg * scale * (G.abs() @ w.double().abs()) + tiny(torch.float32))

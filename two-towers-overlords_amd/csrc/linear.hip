@@ -455,7 +455,7 @@ int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
   a.g = g;
   const int bk = kRowBytes / dtype_bytes(dtype);
   a.s = Shape{g.M, g.N, g.K, (int)(pad_to((g.K + g.nsplit - 1) / g.nsplit, bk))};
-  a.vec = g.slab ? g.N % 4 == 0 : chunk_ok(g.out, g.ldo, dtype_bytes(dtype)) && g.N % (16 / dtype_bytes(dtype)) == 0;
+  a.vec = g.slab ? g.N % 4 == 0 && tt_aligned16(g.slab) : chunk_ok(g.out, g.ldo, dtype_bytes(dtype)) && g.N % (16 / dtype_bytes(dtype)) == 0;
   const int b = pick_tile(g.M, g.N, g.nsplit, dtype);
   a.gm = (g.M + b - 1) / b;
   a.gn = (g.N + b - 1) / b;

@@ -3,9 +3,13 @@
 //   l_ij = scale x_i.w_j,  lse_i = log sum_j exp l_ij,  loss_i = lse_i - l_i,target
 //   G_ij = c_i (exp(l_ij - lse_i) - [j = target_i]),  dx = scale G w,  dw = scale G^T x
 //
+// float: a target that is nearly certain has G = c (p - 1), of which fp32's lse leaves few digits (5e-6 of dx where the logits reach
+// 20), so G is kept for whole rows and the target's entry is minus the sum of the row's others.
+//
 // Forward: the product's epilogue leaves each row's maximum and sum of a tile's candidates (fp32, base 2); a second launch
-// joins them.  Backward: pieces of the candidates; a piece's G is recomputed from x, w and lse into the workspace, then dw of
-// the piece is final and dx is summed in fp32 over the pieces.  8 N V D operations instead of 6 with stored logits.
+// joins them.  Backward: G is recomputed from x, w and lse into the workspace piece by piece.  16-bit types take pieces of the
+// candidates (dw of a piece is final, dx is summed in fp32 over the pieces), float pieces of the rows (the other way round).
+// 8 N V D operations instead of 6 with stored logits.
 //
 // G is rounded to the operands' type (it feeds matrix instructions).  float and bf16 share fp32's exponent range, so c goes
 // into G; fp16 takes c / max|c| times 2^14, and the products' epilogues take both out again: probabilities keep their
@@ -30,7 +34,9 @@ struct Args {
   int v0, V, gm, gn;     // first candidate of the piece; candidates in all; tiles along the rows and the candidates
   float scale2;          // scale * log2 e
   float2* part;          // [gn, M] (maximum, sum) of a tile's candidates
-  float* tlogit;         // [M] the target's logit, base 2
+  float* others;         // float's backward: [gn * WN, M] sums of G's entries, the target's left out
+  float scale;
+  float* tlogit;         // [M] the target's x.w
   const float *lse, *coef, *cmax;  // backward
   void* G;
   long long ldg;
@@ -70,7 +76,7 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (at == i * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) a.tlogit[m] = acc[i][j][e] * a.scale2;
+          if (at == i * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) a.tlogit[m] = acc[i][j][e];
     }
     if (!plain) {
       const long long rid = in && a.rid ? a.rid[m] : 0;
@@ -112,7 +118,7 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
 // joins the tiles' (maximum, sum) of each row: 16 rows x 16 lanes per workgroup, tiles in a fixed order
 __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restrict__ part, const float* __restrict__ tlogit,
                                                            const long long* __restrict__ target, long long ignore, int M, int V,
-                                                           int gn, float* __restrict__ loss, float* __restrict__ lse) {
+                                                           int gn, float scale2, float* __restrict__ loss, float* __restrict__ lse) {
   __shared__ float2 red[16][17];
   const int rl = threadIdx.x & 15, q = threadIdx.x >> 4, m = blockIdx.x * 16 + rl;
   float mx = -INFINITY, sum = 0.f;
@@ -139,7 +145,7 @@ __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restr
   const double l = log2((double)sum), ln2 = 0.6931471805599453094;
   lse[m] = mx == -INFINITY && sum == 0.f ? -INFINITY : (float)((base + l) * ln2);
   const long long t = target[m];
-  loss[m] = t == ignore ? 0.f : (t < 0 || t >= V ? NAN : (float)(((double)base - tlogit[m] + l) * ln2));
+  loss[m] = t == ignore ? 0.f : (t < 0 || t >= V ? NAN : (float)(((double)base - (double)tlogit[m] * scale2 + l) * ln2));
 }
 
 // G of a piece of the candidates, [M, ldg] in T; columns behind the last candidate are zero
@@ -153,12 +159,13 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   B blk;
   blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
   T* __restrict__ G = static_cast<T*>(a.G);
-  const float up = __is_same(T, _Float16) ? kF16Up / *a.cmax : 1.f;
+  // what a row's coefficient is scaled by in G; the products' alpha takes fp16's out again, and has float's already
+  const float up = __is_same(T, _Float16) ? kF16Up / *a.cmax : (sizeof(T) == 4 ? a.scale : 1.f);
   using R = typename B::template Rows<T>;
   blk.template for_rows<T>(
       b0, b1, m0, n0, [](int) {},
       [&](int j, int s, int m, int nl, f32x4 (&v)[R::Q]) {
-        if (m >= a.s.M || nl >= a.ldg) return;
+        if (m >= a.s.M || nl >= a.ldg) return;  // whole rows of lanes
         const long long t = a.target[m];
         const float lse = a.lse[m], c = t == a.ignore ? 0.f : (t < 0 || t >= a.V ? NAN : a.coef[m] * up);
         // lse in base 2 as two floats; the second one scales the row
@@ -173,7 +180,7 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
           for (int q = 0; q < R::Q; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (n + 4 * q + e == t) v[q][e] -= c;
+              if (n + 4 * q + e == t) v[q][e] = sizeof(T) == 4 ? 0.f : v[q][e] - c;
         }
         const bool off = t == a.ignore;
         if (off || a.rid || n + 4 * R::Q > a.V) {
@@ -183,11 +190,36 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[q][e] = (off | left_out(a, n + 4 * q + e, t, rid)) ? 0.f : v[q][e];
         }
+        if constexpr (sizeof(T) == 4) {
+          float sum = (v[0][0] + v[0][1]) + (v[0][2] + v[0][3]);
+#pragma unroll
+          for (int o = R::LPR / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+          if (blk.lane % R::LPR == 0) a.others[(long long)(tn * B::WN + blk.wn) * a.s.M + m] = sum;
+        }
         Chunk<T> g;
 #pragma unroll
         for (int q = 0; q < R::Q; ++q) g.q[q] = to_quad<T>(v[q]);
         g.store(G + m * a.ldg + nl);
       });
+}
+
+// float: G's target entries, minus the sum of the row's others; 16 rows x 16 lanes per workgroup, parts in a fixed order
+__global__ __launch_bounds__(256) void softmax_target_kernel(const float* __restrict__ others, const long long* __restrict__ target,
+                                                             long long ignore, int M, int V, int parts, float* __restrict__ G,
+                                                             long long ldg) {
+  __shared__ float red[16][17];
+  const int rl = threadIdx.x & 15, q = threadIdx.x >> 4, m = blockIdx.x * 16 + rl;
+  float sum = 0.f;
+  if (m < M)
+    for (int t = q; t < parts; t += 16) sum += others[(long long)t * M + m];
+  red[rl][q] = sum;
+  __syncthreads();
+  if (q != 0 || m >= M) return;
+  const long long t = target[m];
+  if (t == ignore || t < 0 || t >= V) return;
+  sum = 0.f;
+  for (int i = 0; i < 16; ++i) sum += red[rl][i];
+  G[m * ldg + t] = -sum;
 }
 
 // cmax[0] = max |coef| over the rows that have a target (1 if that is 0 or not finite), cmax[1] = cmax[0] / kF16Up
@@ -220,9 +252,10 @@ int with_type(int dtype, F&& f) {
 
 struct Plan {
   int gn, fwd_tile;
-  long long piece;      // candidates of a piece (a multiple of 128)
-  int pieces, sx, sw;   // splits of the two gradient products
-  size_t x, w, part, tlogit, cmax, G, dx, dw, fwd, bwd;
+  long long piece, rows;  // candidates (a multiple of 128) and rows of a piece of G
+  int pieces, blocks;     // pieces of the candidates, pieces of the rows (one of them is 1)
+  int sx, sw;             // splits of the two gradient products
+  size_t x, w, part, tlogit, cmax, G, others, dx, dw, fwd, bwd;
 };
 constexpr long long kPieceBytes = 512LL << 20;  // of G; 8192 rows x 30522 bf16 candidates: 64 MB 1421 us, 128 1279, 256 1272, 512 1217
 Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long M, int V, int D, int dtype) {
@@ -235,18 +268,30 @@ Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long 
   p.part = align256((size_t)p.gn * M * sizeof(float2));
   p.tlogit = align256((size_t)M * 4);
   p.fwd = p.x + p.w + p.part + p.tlogit;
-  const long long cap = kPieceBytes / (M * width) / 128 * 128;
-  const long long vp = pad_to(V, 128), most = cap < 1024 ? 1024 : cap;
-  p.pieces = (int)((vp + most - 1) / most);
-  p.piece = pad_to((vp + p.pieces - 1) / p.pieces, 128);
-  p.pieces = (int)((vp + p.piece - 1) / p.piece);
-  p.sx = tt_grad_splits(M, D, p.piece);
-  p.sw = tt_grad_splits(p.piece, D, M);
+  const long long vp = pad_to(V, 128);
+  p.piece = vp;
+  p.rows = M;
+  p.pieces = p.blocks = 1;
+  if (dtype == TT_F32) {
+    const long long cap = kPieceBytes / (vp * width) / 128 * 128, most = cap < 128 ? 128 : cap;
+    p.blocks = (int)((M + most - 1) / most);
+    p.rows = pad_to((M + p.blocks - 1) / p.blocks, 128);
+    if (p.rows > M) p.rows = M;
+    p.blocks = (int)((M + p.rows - 1) / p.rows);
+    p.others = align256((size_t)((vp + 63) / 64) * 2 * p.rows * 4);  // at least the parts of any tile shape
+  } else {
+    const long long cap = kPieceBytes / (M * width) / 128 * 128, most = cap < 1024 ? 1024 : cap;
+    p.pieces = (int)((vp + most - 1) / most);
+    p.piece = pad_to((vp + p.pieces - 1) / p.pieces, 128);
+    p.pieces = (int)((vp + p.piece - 1) / p.piece);
+  }
+  p.sx = tt_grad_splits(p.rows, D, p.piece);
+  p.sw = p.blocks > 1 ? 1 : tt_grad_splits(p.piece, D, M);  // several blocks of rows add up in dw itself
   p.cmax = 256;
-  p.G = align256((size_t)M * p.piece * width);
-  p.dx = p.pieces > 1 || p.sx > 1 ? align256((size_t)p.sx * M * D * 4) : 0;
+  p.G = align256((size_t)p.rows * p.piece * width);
+  p.dx = p.pieces > 1 || p.sx > 1 ? align256((size_t)p.sx * p.rows * D * 4) : 0;
   p.dw = p.sw > 1 ? align256((size_t)p.sw * p.piece * D * 4) : 0;
-  p.bwd = p.x + p.w + p.cmax + p.G + p.dx + p.dw;
+  p.bwd = p.x + p.w + p.cmax + p.G + p.others + p.dx + p.dw;
   return p;
 }
 
@@ -316,7 +361,7 @@ extern "C" int tt_softmax_loss(const void* x, int64_t ldx, const void* w, int64_
   });
   if (rc != TT_OK) return rc;
   hipLaunchKernelGGL(softmax_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, a.part, a.tlogit, a.target, a.ignore,
-                     (int)N, V, p.gn, loss, lse);
+                     (int)N, V, p.gn, a.scale2, loss, lse);
   TT_CHECK_LAUNCH();
   return TT_OK;
 }
@@ -345,6 +390,7 @@ extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t
   ws += p.w;
   float* cmax = (float*)ws;   ws += p.cmax;
   a.G = ws;                   ws += p.G;
+  a.others = (float*)ws;      ws += p.others;
   float* dxs = (float*)ws;    ws += p.dx;
   float* dws = (float*)ws;
   const float* alpha_dev = nullptr;
@@ -354,17 +400,24 @@ extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t
     TT_CHECK_LAUNCH();
     alpha_dev = cmax + 1;
   }
-  a.target = (const long long*)target; a.rid = (const long long*)row_ids; a.cid = (const long long*)cand_ids;
-  a.ignore = ignore_index; a.V = V; a.scale2 = scale * kLog2e; a.lse = lse; a.coef = row_coef; a.cmax = cmax; a.ldg = p.piece;
-  for (int i = 0; i < p.pieces; ++i) {
-    const long long v0 = i * p.piece;
-    const int vc = (int)(V - v0 < p.piece ? V - v0 : p.piece);
+  const float alpha = dtype == TT_F32 ? 1.f : scale;
+  a.cid = (const long long*)cand_ids;
+  a.ignore = ignore_index; a.V = V; a.scale = scale; a.scale2 = scale * kLog2e; a.cmax = cmax; a.ldg = p.piece;
+  const Operand X = a.X;
+  for (int i = 0; i < p.pieces * p.blocks; ++i) {
+    const long long v0 = p.pieces > 1 ? i * p.piece : 0, r0 = p.blocks > 1 ? i * p.rows : 0;
+    const int vc = (int)(V - v0 < p.piece ? V - v0 : p.piece), rows = (int)(N - r0 < p.rows ? N - r0 : p.rows);
     a.v0 = (int)v0;
     a.W = Operand{static_cast<const char*>(W.p) + v0 * W.ld * width, W.ld};
-    a.s = Shape{(int)N, vc, D, D};
-    const int b = pick_tile(N, vc, 1, dtype);
+    a.X = Operand{static_cast<const char*>(X.p) + r0 * X.ld * width, X.ld};
+    a.target = (const long long*)target + r0;
+    a.rid = row_ids ? (const long long*)row_ids + r0 : nullptr;
+    a.lse = lse + r0;
+    a.coef = row_coef + r0;
+    a.s = Shape{rows, vc, D, D};
+    const int b = pick_tile(rows, vc, 1, dtype);
     a.gn = (vc + b - 1) / b;  // every tile starts at a candidate of the piece; the last one zero-fills behind it
-    a.gm = (int)((N + b - 1) / b);
+    a.gm = (rows + b - 1) / b;
     const long long grid = (long long)a.gm * a.gn;
     TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
     rc = with_type(dtype, [&](auto tag) {
@@ -373,27 +426,36 @@ extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t
         using B = std::remove_pointer_t<decltype(shape)>;
         hipLaunchKernelGGL((softmax_grad_kernel<T, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
         TT_CHECK_LAUNCH();
+        if (sizeof(T) == 4) {
+          hipLaunchKernelGGL(softmax_target_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a.others, a.target, a.ignore,
+                             rows, V, a.gn * B::WN, (float*)a.G, a.ldg);
+          TT_CHECK_LAUNCH();
+        }
         return (int)TT_OK;
       });
     });
     if (rc != TT_OK) return rc;
     if (dx) {
       GradProduct g{};
-      g.X = Operand{a.G, p.piece}; g.Y = a.W; g.M = (int)N; g.N = D; g.K = vc; g.xks = 0; g.nsplit = p.sx;
-      g.alpha = scale; g.alpha_dev = alpha_dev;
-      if (p.dx) { g.slab = dxs; g.accumulate = i > 0; } else { g.out = dx; g.ldo = D; }
+      g.X = Operand{a.G, p.piece}; g.Y = a.W; g.M = rows; g.N = D; g.K = vc; g.xks = 0; g.nsplit = p.sx;
+      g.alpha = alpha; g.alpha_dev = alpha_dev;
+      char* out = static_cast<char*>(dx) + r0 * D * width;
+      if (p.dx) { g.slab = dxs; g.accumulate = v0 > 0; } else { g.out = out; g.ldo = D; }
       if ((rc = tt_launch_grad_product(g, dtype, st)) != TT_OK) return rc;
+      if (p.dx && v0 + p.piece >= V &&
+          (rc = tt_launch_slab_sum(dxs, p.sx, (long long)rows * D, out, dtype, alpha, alpha_dev, st)) != TT_OK)
+        return rc;
     }
     if (dw) {
       GradProduct g{};
-      g.X = Operand{a.G, p.piece}; g.Y = a.X; g.M = vc; g.N = D; g.K = (int)N; g.xks = 1; g.nsplit = p.sw;
-      g.alpha = scale; g.alpha_dev = alpha_dev;
+      g.X = Operand{a.G, p.piece}; g.Y = a.X; g.M = vc; g.N = D; g.K = rows; g.xks = 1; g.nsplit = p.sw;
+      g.alpha = alpha; g.alpha_dev = alpha_dev;
       char* out = static_cast<char*>(dw) + v0 * D * width;
-      if (p.sw > 1) g.slab = dws; else { g.out = out; g.ldo = D; }
+      if (p.blocks > 1) { g.slab = (float*)dw; g.accumulate = i > 0; }
+      else if (p.sw > 1) g.slab = dws; else { g.out = out; g.ldo = D; }
       if ((rc = tt_launch_grad_product(g, dtype, st)) != TT_OK) return rc;
-      if (p.sw > 1 && (rc = tt_launch_slab_sum(dws, p.sw, (long long)vc * D, out, dtype, scale, alpha_dev, st)) != TT_OK) return rc;
+      if (p.sw > 1 && (rc = tt_launch_slab_sum(dws, p.sw, (long long)vc * D, out, dtype, alpha, alpha_dev, st)) != TT_OK) return rc;
     }
   }
-  if (dx && p.dx) return tt_launch_slab_sum(dxs, p.sx, (long long)N * D, dx, dtype, scale, alpha_dev, st);
   return TT_OK;
 }
