@@ -107,6 +107,27 @@ def test_workspaces_hold_no_logits(lib):
     assert lib.tt_softmax_loss_bwd_workspace_bytes(P, D, P, D, N, V, D, 1) < logits / 50
 
 
+def test_sizes_beyond_a_tiles_offsets_are_refused(lib):
+    """A tile's 32-bit offsets reach 256 packed rows of 2^22 elements."""
+    big = 1 << 23
+    assert linear(lib, K=big, ldx=big, ldw=big) == SHAPE and linear(lib, N=big, ldy=big) == SHAPE and linear(lib, M=(1 << 30) + 1) == SHAPE
+    assert lib.tt_linear_act_bwd(P, big, P, 8, P, 8, None, P, P, P, 4, big, 8, 1, 0, P, 1 << 40, None) == SHAPE
+    args = (P, big, P, big, P, None, None, 4, 9, big, 1, 1.0, -100)
+    assert lib.tt_softmax_loss(*args, P, P, P, 1 << 40, None) == SHAPE
+    assert lib.tt_softmax_loss_bwd(P, P, 8, P, 8, P, None, None, P, 4, (1 << 28) + 1, 8, 1, 1.0, -100, P, P, P, 1 << 60, None) == SHAPE
+    assert lib.tt_packed_attention(attention_args(T=(1 << 30) + 1), None) == SHAPE
+    assert lib.tt_packed_attention(attention_args(k=_lib.TTHeadView(P, 1 << 22, 32)), None) == ALIGN
+
+
+@pytest.mark.parametrize("V", [8_400_000, 30_000_000, 1 << 28])
+def test_float_gradient_rows_stay_within_a_tiles_offsets(lib, V):
+    """Rows of float G as long as all candidates: no block of them is larger than a tile's 32-bit offsets reach."""
+    D, N = 8, 1000
+    need = lib.tt_softmax_loss_bwd_workspace_bytes(P, D, P, D, N, V, D, _lib.TT_F32)
+    parts = 2 * ((V + 127) // 128 * 128 // 64)
+    assert 0 < need <= 2 ** 32 * (1 + 1 / 32) + 2 ** 22 and need > 4 * V + parts  # G, its rows' partial sums, dx in parts
+
+
 def test_struct_matches_the_header():
     assert C.sizeof(_lib.TTAttentionArgs) == 280 and C.sizeof(_lib.TTHeadView) == 24
 

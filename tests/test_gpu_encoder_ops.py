@@ -118,6 +118,13 @@ def test_linear_act_and_gradients(ops, dt, M, K, N, act):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(1499, 72, 2296), (72, 1499, 2296), (1499, 2296, 72), (4095, 72, 4088), (72, 4088, 4088), (4095, 4088, 72)])
+def test_linear_act_tile_shapes(ops, dt, M, K, N):
+    """Outputs large enough for 128- and 256-wide tiles, in the forward and in either gradient product, ragged at both edges."""
+    check_linear(ops, dt, M, K, N, "gelu")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("bias,res", [(False, False), (True, False), (False, True)])
 def test_linear_act_without_bias_or_residual(ops, dt, bias, res):
     check_linear(ops, dt, 50, 40, 24, "gelu", bias=bias, res=res)
@@ -379,6 +386,18 @@ def test_attention_long_document(ops, dt):
     check_attention(ops, dt, [1500, 3], 1, 1, 64, causal=True, alibi=True)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("kw", [dict(causal=True), dict(prefix=[300, 0, 700, 5, 64]), dict()], ids=["causal", "prefix", "full"])
+def test_attention_long_documents_in_sorted_order(ops, dt, kw):
+    """Few long documents: their tiles run longest first.  An empty one, one short one and rows behind the last among them."""
+    check_attention(ops, dt, [701, 0, 1030, 64, 300], 2, 1, 64, tail=150, **kw)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_attention_more_long_documents_than_lanes(ops, dt):
+    check_attention(ops, dt, [257 + i % 5 for i in range(67)], 1, 1, 32, causal=True)
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 def test_attention_many_documents(ops, dt):
     """More documents than the 64-wide search takes in one step."""
@@ -483,6 +502,13 @@ def check_softmax(ops, dt, N, V, D, scale=1.0, groups=False, ignore=(), unit=Fal
 def test_softmax_loss_and_gradients(ops, dt, N, V, D):
     check_softmax(ops, dt, N, V, D)
     check_softmax(ops, dt, N, V, D, scale=20.0, unit=True, groups=True, ignore=(0,) if N > 1 else ())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("N,V", [(1499, 2297), (4095, 4089)])
+def test_softmax_loss_tile_shapes(ops, dt, N, V):
+    """128- and 256-wide tiles, ragged at both edges."""
+    check_softmax(ops, dt, N, V, 72, scale=20.0, unit=True, groups=True, ignore=(0, 17, N - 1))
 
 
 @pytest.mark.parametrize("dt", DTYPES)

@@ -215,6 +215,18 @@ def test_encoder_refusals():
         InBatchSoftmaxLoss()(torch.randn(4, 8, device="cuda"), torch.randn(5, 8, device="cuda"))
 
 
+def test_expanded_gradient_outputs_are_refused():
+    from two_towers_overlords_amd import ops
+
+    q = torch.randn(6, 2, 32, device="cuda")
+    cu = torch.tensor([0, 6], dtype=torch.int32, device="cuda")
+    o, lse = ops.packed_attention(q, q, q, cu)
+    one = torch.empty(1, 2, 32, device="cuda").expand(6, 2, 32)
+    for grads in ((one, q, q), (q, one, q), (q, q, one)):
+        with pytest.raises(ValueError, match="expanded"):
+            ops.packed_attention_bwd(o, q, q, q, o, lse, cu, grads=grads)
+
+
 def test_op_refusals():
     from two_towers_overlords_amd import ops
 
@@ -402,6 +414,42 @@ def test_offsets_beyond_31_bits():
     G[2, -1] -= 1
     ref = G.t() @ x.double()
     assert float((dw[tail] - ref).abs().max()) <= 2.0 ** -7 * float(ref.abs().max())
+
+
+def test_float_rows_of_gradients_beyond_32_bits():
+    """128 rows of float gradients of the logits are more than 4 GiB: they go in smaller blocks."""
+    from two_towers_overlords_amd import ops
+
+    N, V, D = 130, 8_400_001, 8
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, w = torch.randn(N, D, generator=g, device="cuda"), torch.randn(V, D, generator=g, device="cuda")
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    t[-1], t[0], t[64] = V - 1, 0, -100
+    c = (torch.rand(N, generator=g, device="cuda") + 0.1) * (t >= 0)
+    loss, lse = ops.softmax_loss(x, w, t)
+    dx, dw = ops.softmax_loss_bwd(c, x, w, t, lse)
+    X = x.double()
+    parts = [w[i:i + 1_000_000].double() for i in range(0, V, 1_000_000)]
+    LSE = torch.logsumexp(torch.stack([torch.logsumexp(X @ p.t(), 1) for p in parts]), 0)
+    E = 2.0 ** -24
+    big = max(float((x.abs() @ p.abs().t().float()).max()) for p in parts)
+    err = (D + 32) * E * big  # of a logit; joined sums of like signs, tile by tile and in 64 bits, add less than 512 + 64 steps
+    assert float((lse - LSE).abs().max()) <= err + 576 * E + E * float(LSE.abs().max())
+    DX, AX = torch.zeros_like(X), torch.zeros_like(X)
+    rel = 2 * err + 700 * E  # of p
+    for i, p in enumerate(parts):
+        G = torch.exp(X @ p.t() - LSE[:, None])
+        at = t - i * 1_000_000
+        here = (at >= 0) & (at < p.shape[0])
+        G[here.nonzero().squeeze(1), at[here]] -= 1
+        G *= c[:, None].double()
+        # a target's entry is minus the sum of the row's others: within rel of that sum
+        DX += G @ p
+        AX += G.abs() @ p.abs()
+        got = dw[i * 1_000_000:(i + 1) * 1_000_000].double()
+        assert bool(((got - G.t() @ X).abs() <= (rel + (N + 32) * E) * (G.abs().t() @ X.abs()) + 1e-30).all()), i
+    # a row of 8.4 million terms is added in at most 32 parts of K / 32 steps of two
+    assert bool(((dx - DX).abs() <= (rel + (V / 32 + 64) * E) * AX).all())
 
 
 def test_another_current_device_is_left_alone():

@@ -416,6 +416,8 @@ int with_type(int dtype, F&& f) {
     default: return TT_ERR_BAD_DTYPE;
   }
 }
+// 2^22 columns: 256 packed rows are within a tile's 32-bit offsets
+bool shape_ok(int64_t M, int N, int K) { return M >= 0 && M <= 1LL << 30 && N >= 1 && N <= 1 << 22 && K >= 1 && K <= 1 << 22; }
 bool known_dtype(int d) { return d == TT_F32 || d == TT_BF16 || d == TT_F16; }
 // rows of 16-byte chunks
 bool chunk_ok(const void* p, long long ld, int width) { return !p || (tt_aligned16(p) && ld % (16 / width) == 0); }
@@ -476,7 +478,7 @@ int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
 
 extern "C" size_t tt_linear_act_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K,
                                                 int dtype) {
-  if (!known_dtype(dtype) || M < 0 || N < 1 || K < 1) return 0;
+  if (!known_dtype(dtype) || !shape_ok(M, N, K)) return 0;
   return pack_bytes(x, ldx, M, K, dtype) + pack_bytes(w, ldw, N, K, dtype);
 }
 
@@ -485,8 +487,7 @@ extern "C" int tt_linear_act(const void* x, int64_t ldx, const void* w, int64_t 
                              void* workspace, size_t workspace_bytes, tt_stream_t stream) {
   TT_REQUIRE(known_dtype(dtype), TT_ERR_BAD_DTYPE);
   TT_REQUIRE(act >= TT_ACT_NONE && act <= TT_ACT_SILU, TT_ERR_UNSUPPORTED);
-  TT_REQUIRE(M >= 0 && M <= 0x7fffffffLL - 256 && N >= 1 && K >= 1 && ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N),
-             TT_ERR_BAD_SHAPE);
+  TT_REQUIRE(shape_ok(M, N, K) && ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N), TT_ERR_BAD_SHAPE);
   if (M == 0) return TT_OK;
   TT_REQUIRE(x && w && y, TT_ERR_NULL_POINTER);
   const size_t need = tt_linear_act_workspace_bytes(x, ldx, w, ldw, M, N, K, dtype);
@@ -576,7 +577,7 @@ BwdPlan bwd_plan(const void* dy, int64_t lddy, const void* x, int64_t ldx, const
 
 extern "C" size_t tt_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
                                                     int64_t ldw, int64_t M, int N, int K, int dtype, int act) {
-  if (!known_dtype(dtype) || M < 0 || N < 1 || K < 1) return 0;
+  if (!known_dtype(dtype) || !shape_ok(M, N, K)) return 0;
   return bwd_plan(dy, lddy, x, ldx, w, ldw, M, N, K, dtype, act, true).total;
 }
 
@@ -585,7 +586,7 @@ extern "C" int tt_linear_act_bwd(const void* dy, int64_t lddy, const void* x, in
                                  void* workspace, size_t workspace_bytes, tt_stream_t stream) {
   TT_REQUIRE(known_dtype(dtype), TT_ERR_BAD_DTYPE);
   TT_REQUIRE(act >= TT_ACT_NONE && act <= TT_ACT_SILU, TT_ERR_UNSUPPORTED);
-  TT_REQUIRE(M >= 0 && M <= 0x7fffffffLL - 256 && N >= 1 && K >= 1 && lddy >= N && ldx >= K && ldw >= K, TT_ERR_BAD_SHAPE);
+  TT_REQUIRE(shape_ok(M, N, K) && lddy >= N && ldx >= K && ldw >= K, TT_ERR_BAD_SHAPE);
   TT_REQUIRE(workspace, TT_ERR_NULL_POINTER);
   TT_REQUIRE(M == 0 || (dy && (!dx || w) && (!dw || x) && (act == TT_ACT_NONE || preact)), TT_ERR_NULL_POINTER);
   TT_REQUIRE(tt_aligned16(workspace), TT_ERR_ALIGNMENT);

@@ -273,9 +273,11 @@ Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long 
   p.rows = M;
   p.pieces = p.blocks = 1;
   if (dtype == TT_F32) {
-    const long long cap = kPieceBytes / (vp * width) / 128 * 128, most = cap < 128 ? 128 : cap;
+    const long long cap = kPieceBytes / (vp * width) / 128 * 128, reach = (1LL << 32) / (vp * width);  // a tile's 32-bit offsets
+    const long long most = cap >= 128 ? cap : (reach < 128 ? reach : 128);
     p.blocks = (int)((M + most - 1) / most);
-    p.rows = pad_to((M + p.blocks - 1) / p.blocks, 128);
+    p.rows = (M + p.blocks - 1) / p.blocks;
+    if (most >= 128) p.rows = pad_to(p.rows, 128);
     if (p.rows > M) p.rows = M;
     p.blocks = (int)((M + p.rows - 1) / p.rows);
     p.others = align256((size_t)((vp + 63) / 64) * 2 * p.rows * 4);  // at least the parts of any tile shape
@@ -297,7 +299,8 @@ Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long 
 
 int check(int64_t ldx, int64_t ldw, int64_t N, int V, int D, int dtype, float scale) {
   TT_REQUIRE(dtype == TT_F32 || dtype == TT_BF16 || dtype == TT_F16, TT_ERR_BAD_DTYPE);
-  TT_REQUIRE(N >= 0 && N <= 0x7fffffffLL - 256 && V >= 1 && V <= 0x7fffffff - 256 && D >= 1 && ldx >= D && ldw >= D && scale > 0.f,
+  // 2^28 candidates: two rows of float G are within a tile's 32-bit offsets; 2^22 features: 256 packed rows are
+  TT_REQUIRE(N >= 0 && N <= 1LL << 30 && V >= 1 && V <= 1 << 28 && D >= 1 && D <= 1 << 22 && ldx >= D && ldw >= D && scale > 0.f,
              TT_ERR_BAD_SHAPE);
   return TT_OK;
 }

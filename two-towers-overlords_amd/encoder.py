@@ -163,7 +163,7 @@ class PackedBertEncoder:
         cu = F.pad(lens.cumsum(0), (1, 0)).to(torch.int32)
         dt = self._compute_type(emb.word_embeddings.weight)
         with torch.autocast("cuda", enabled=False):
-            x = F.embedding(input_ids.reshape(-1)[slots].long(), emb.word_embeddings.weight)
+            x = F.embedding(input_ids.reshape(-1)[slots].long(), emb.word_embeddings.weight, padding_idx=emb.word_embeddings.padding_idx)
             x = x + F.embedding(slots % S, emb.position_embeddings.weight)
             types = emb.token_type_embeddings.weight
             x = x + (types[0] if token_type_ids is None else F.embedding(token_type_ids.reshape(-1)[slots].long(), types))

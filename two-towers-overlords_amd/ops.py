@@ -655,6 +655,8 @@ def packed_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     if grads is None:
         grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     dq, dk, dv = grads
+    if any(n > 1 and st == 0 for t in grads for n, st in zip(t.shape, t.stride())):
+        raise ValueError("packed_attention_bwd: a gradient to write into must not be an expanded tensor")
     views += [_head_view(dq, "dq", q, q.shape), _head_view(dk, "dk", q, k.shape), _head_view(dv, "dv", q, v.shape)]
     if T:
         delta = torch.empty((H, T), dtype=torch.float32, device=q.device)
