@@ -596,3 +596,45 @@ def test_softmax_loss_of_nearly_certain_targets_keeps_its_digits(ops, scale):
     # the row's common factor exp(-lse) carries lse's rounding, 2^-24 of |lse| <= scale + log 300, once
     rg = rel + E * (scale + 8) + (300 + F) * E
     within("dx", dx, DX, 4 * rg * scale * (G.abs() @ w.double().abs()) + tiny(torch.float32))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("Dh", [32, 128])
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=30.0, slopes=True), dict(causal=True), dict(prefix=True)], ids=["full", "cap", "causal", "prefix"])
+def test_attention_single_key_has_exactly_no_gradient_of_scores(ops, dt, Dh, kw):
+    """A query that sees one key has p = 1 whatever q and k are: dq and dk are 0, dv = dO."""
+    docs, H = 37, 4
+    g = gen(Dh)
+    q, k, v, do = (randn(g, docs, H, Dh).to(dt) for _ in range(4))
+    cu = torch.arange(docs + 1, dtype=torch.int32, device="cuda")
+    kw = dict(kw)
+    if "slopes" in kw:
+        kw["slopes"] = torch.full((H,), 0.5, device="cuda")
+    if "prefix" in kw:
+        kw["prefix"] = torch.ones(docs, dtype=torch.int32, device="cuda")
+    o, lse = ops.packed_attention(q, k, v, cu, **kw)
+    dq, dk, dv = ops.packed_attention_bwd(do, q, k, v, o, lse, cu, **kw)
+    assert not bool(dq.any()) and not bool(dk.any())
+    within("dv", dv, do.double(), 2 * half(dt) * do.double().abs() + (64 * E) * do.double().abs())  # p and dv are rounded
+    if "causal" in kw or "prefix" in kw:  # the first query of longer documents
+        cu = torch.tensor([0, 5, docs], dtype=torch.int32, device="cuda")
+        if "prefix" in kw:
+            kw["prefix"] = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+        o, lse = ops.packed_attention(q, k, v, cu, **kw)
+        dq, dk, dv = ops.packed_attention_bwd(do, q, k, v, o, lse, cu, **kw)
+        assert not bool(dq[0].any()) and not bool(dq[5].any()) and bool(dq[1].any())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_softmax_loss_of_a_single_candidate_is_exactly_nothing(ops, dt):
+    """The target is the row's only candidate, by itself or because its group's others are left out: loss and gradients are 0."""
+    N, D = 300, 72
+    g = gen(5)
+    x = randn(g, N, D).to(dt)
+    for V in (1, 2, 700):
+        w = randn(g, V, D).to(dt)
+        t = torch.randint(0, V, (N,), generator=g, device="cuda")
+        kw = dict(row_ids=torch.full((N,), 3, device="cuda"), cand_ids=torch.full((V,), 3, device="cuda")) if V > 1 else {}
+        loss, lse = ops.softmax_loss(x, w, t, scale=1.7, **kw)
+        dx, dw = ops.softmax_loss_bwd(torch.ones(N, device="cuda"), x, w, t, lse, scale=1.7, **kw)
+        assert not any(bool(a.any()) for a in (loss, dx, dw)), V

@@ -336,6 +336,11 @@ __device__ __forceinline__ f32x16 through_cap(f32x16 x, f32x16 s, const Args& a)
   return x;
 }
 
+// The document's first query sees one key: its p is 1 and its dS exactly 0, which dP less delta, rounded apart, would miss.
+__device__ __forceinline__ bool first_alone(const Args& a, int prefix, int len) {
+  return len == 1 || ((a.causal || a.prefix) && prefix <= 1);
+}
+
 // number of keys (from the document's start) that some query of [i0, i1) sees, and the first from which masking is needed
 __device__ __forceinline__ int key_end(const Args& a, int prefix, int i1, int len) {
   if (!a.causal && !a.prefix) return len;
@@ -540,7 +545,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     delta += __shfl_xor(delta, 32, 64);
     if (live) {
       const float t = a.lse[(long long)head * a.T + tok];
-      if (t != -INFINITY) lse2 = t * kLog2e;
+      if (t != -INFINITY && !(i == 0 && first_alone(a, prefix, w.len))) lse2 = t * kLog2e;
     }
   }
   float rest[4] = {0.f, 0.f, 0.f, 0.f};  // sum_j p_ij (dp_ij - delta): what the rounding of o left out of delta (sum_j p_ij = 1)
@@ -678,6 +683,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   const int wfirst = !limited || j0 + wave * 32 < prefix ? 0 : j0 + wave * 32;
   const int bfirst = (!limited || j0 < prefix ? 0 : j0) / D::TILE * D::TILE;
   const float c = units(a, 0).c;
+  const bool lone = j0 + wave * 32 == 0 && first_alone(a, prefix, w.len);
 
   u32x4 kf[D::G], vf[D::G];
   load_own<T, DP>(kf, static_cast<const T*>(a.k) + tok * a.kt + kvh * a.kh, live, a.Dh, h);
@@ -752,6 +758,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
           dp[e] = s[e] * (dp[e] - de[i]);
         }
       }
+      if (lone && q0 + 32 * t == 0) dp[0] = lane == 0 ? 0.f : dp[0];
       if constexpr (!PLAIN) dp = through_cap(dp, sc, a);
       if (masked) {
         const uint32_t bits = ~lane_bits<T>(~0ull, t, first - q0, h);  // queries from `first` on

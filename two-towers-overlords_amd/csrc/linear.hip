@@ -120,7 +120,8 @@ __device__ __forceinline__ f32x4 kept(f32x4 v, int act) {
 template <class T, int ACT, class B>
 __device__ __forceinline__ void epilogue(B& blk, const FwdArgs& a, char* __restrict__ b0, char* __restrict__ b1, int m0, int n0) {
   using R = typename B::template Rows<T>;
-  const int n = blk.template row_col<T>(n0), M = a.s.M;
+  static_assert(R::WHOLE, "a lane's bias");
+  const int n = blk.template row_col<T>(n0, 0), M = a.s.M;
   const bool col = n < a.s.N;
   const T* __restrict__ res = static_cast<const T*>(a.res);
   Chunk<T> bias;
@@ -371,18 +372,17 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
     }
     using R = typename B::template Rows<float>;
     f32x4 old[R::STEPS];
-    const int n = blk.template row_col<float>(n0);
     blk.template for_rows<float>(
         b0, b1, m0, n0,
         [&](int j) {
           if (!more) return;
 #pragma unroll
           for (int s = 0; s < R::STEPS; ++s) {
-            const int m = blk.template row_at<float>(m0, j, s);
+            const int m = blk.template row_at<float>(m0, j, s), n = blk.template row_col<float>(n0, s);
             if (m < M && n < N) old[s] = *reinterpret_cast<const f32x4*>(c + (long long)m * N + n);
           }
         },
-        [&](int j, int s, int m, int, f32x4 (&v)[R::Q]) {
+        [&](int j, int s, int m, int n, f32x4 (&v)[R::Q]) {
           if (more) v[0] += old[s];
           if (m < M && n < N) *reinterpret_cast<f32x4*>(c + (long long)m * N + n) = v[0];
         });
@@ -444,12 +444,23 @@ int tt_launch_slab_sum(const float* slab, int ns, long long n, void* out, int dt
   });
 }
 
-int tt_grad_splits(long long M, long long N, long long K) {
-  const long long tiles = ((M + 127) / 128) * ((N + 127) / 128);
-  long long s = (512 + tiles - 1) / tiles;        // two workgroups per compute unit
-  if (s > K / 512) s = K / 512;                   // at least eight 16-bit K-steps each
-  if (s > 32) s = 32;
-  return s < 1 ? 1 : (int)s;
+// the least estimated time: dx of 8192 x 30522 bf16 logits, 384 wide, by "two workgroups per compute unit" (three parts of 576
+// tiles) 352 us, by this 265 with 128-wide tiles (five parts), 201 with 256 x 192 (four, one round)
+int tt_grad_splits(long long M, long long N, long long K, int dtype) {
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= 32 && (s == 1 || K / s >= 512); ++s) {  // at least eight 16-bit steps of K each
+    double cost;
+    pick_tile(M, N, s, dtype, true, &cost);
+    // seconds: the slowest compute unit's product; the parts written and read once
+    double t = cost * (2. * K / s) / (dtype == TT_F32 ? 5.2e11 : 4.4e12);
+    if (s > 1) t += s * 8. * M * N / 4e12 + 4e-6;
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
 }
 
 int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
@@ -458,21 +469,24 @@ int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st) {
   const int bk = kRowBytes / dtype_bytes(dtype);
   a.s = Shape{g.M, g.N, g.K, (int)(pad_to((g.K + g.nsplit - 1) / g.nsplit, bk))};
   a.vec = g.slab ? g.N % 4 == 0 && tt_aligned16(g.slab) : chunk_ok(g.out, g.ldo, dtype_bytes(dtype)) && g.N % (16 / dtype_bytes(dtype)) == 0;
-  const int b = pick_tile(g.M, g.N, g.nsplit, dtype);
-  a.gm = (g.M + b - 1) / b;
+  const int b = pick_tile(g.M, g.N, g.nsplit, dtype, true), bm = b == 192 ? 256 : b;
+  a.gm = (g.M + bm - 1) / bm;
   a.gn = (g.N + b - 1) / b;
   const long long grid = (long long)a.gm * a.gn * g.nsplit;
   if (grid == 0) return TT_OK;
   TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
   return with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
-    return with_block<T>(b, [&](auto* shape) {
+    auto go = [&](auto* shape) {
       using B = std::remove_pointer_t<decltype(shape)>;
       if (g.xks) hipLaunchKernelGGL((grad_product_kernel<T, true, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
       else hipLaunchKernelGGL((grad_product_kernel<T, false, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
       TT_CHECK_LAUNCH();
       return (int)TT_OK;
-    });
+    };
+    if constexpr (sizeof(T) == 2)
+      if (b == 192) return go(static_cast<Three*>(nullptr));
+    return with_block<T>(b, go);
   });
 }
 
@@ -556,7 +570,7 @@ BwdPlan bwd_plan(const void* dy, int64_t lddy, const void* x, int64_t ldx, const
   const int width = dtype_bytes(dtype);
   p.own_dz = act != TT_ACT_NONE || !packed_ok(dy, lddy, N, dtype);
   p.ldz = p.own_dz ? pad_to(N, 16 / width) : lddy;
-  p.splits = need_dw ? tt_grad_splits(N, K, M) : 1;
+  p.splits = need_dw ? tt_grad_splits(N, K, M, dtype) : 1;
   const long long gx = (N + 1024 / width - 1) / (1024 / width);
   long long rb = (1024 + gx - 1) / gx;
   if (rb > (M + 15) / 16) rb = (M + 15) / 16;

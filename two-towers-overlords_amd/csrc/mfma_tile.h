@@ -304,18 +304,24 @@ struct Block {
 
   // Rows of the output instead: the accumulators of 32 rows at a time go through the wave's own part of LDS and come back as
   // KPF consecutive columns per lane, so that 16 lanes read and write 256 consecutive bytes of a row (a quad per lane and row
-  // touched 16 bytes of 32 rows at a time).  fn(j, step, m, n, v): v holds KPF / 4 quads; n does not depend on j and step.
+  // touched 16 bytes of 32 rows at a time).  fn(j, step, m, n, v): v holds KPF / 4 quads; n does not depend on j, nor, where
+  // 64 lanes are whole rows, on the step.
   // The 16-byte chunk of a row is XORed with the row: no bank conflicts either way.  pre(j): before the rows of j.
   template <class T>
   struct Rows {
-    static constexpr int W = NI * 32, Q = Type<T>::KPF / 4, LPR = W / Type<T>::KPF, RPS = 64 / LPR, STEPS = 32 / RPS;
+    static constexpr int W = NI * 32, Q = Type<T>::KPF / 4, LPR = W / Type<T>::KPF, STEPS = LPR / 2;
+    static constexpr bool WHOLE = 64 % LPR == 0;  // a lane keeps its columns
   };
   template <class T>
-  __device__ __forceinline__ int row_col(int n0) const { return n0 + wn * Rows<T>::W + (lane % Rows<T>::LPR) * Type<T>::KPF; }
+  __device__ __forceinline__ int chunk_at(int step) const { return ((Rows<T>::WHOLE ? 0 : step * 64) + lane) % Rows<T>::LPR; }
   template <class T>
-  __device__ __forceinline__ int row_at(int m0, int j, int step) const {
-    return m0 + (wm * MJ + j) * 32 + step * Rows<T>::RPS + lane / Rows<T>::LPR;
+  __device__ __forceinline__ int row_in(int step) const {
+    return Rows<T>::WHOLE ? step * (64 / Rows<T>::LPR) + lane / Rows<T>::LPR : (step * 64 + lane) / Rows<T>::LPR;
   }
+  template <class T>
+  __device__ __forceinline__ int row_col(int n0, int step) const { return n0 + wn * Rows<T>::W + chunk_at<T>(step) * Type<T>::KPF; }
+  template <class T>
+  __device__ __forceinline__ int row_at(int m0, int j, int step) const { return m0 + (wm * MJ + j) * 32 + row_in<T>(step); }
   template <class T, class P, class F>
   __device__ __forceinline__ void for_rows(char* __restrict__ b0, char* __restrict__ b1, int m0, int n0, P&& pre, F&& fn) {
     using R = Rows<T>;
@@ -336,12 +342,12 @@ struct Block {
       wave_lds_sync();
 #pragma unroll
       for (int s = 0; s < R::STEPS; ++s) {
-        const int row = s * R::RPS + lane / R::LPR;
+        const int row = row_in<T>(s);
         f32x4 v[R::Q];
 #pragma unroll
         for (int q = 0; q < R::Q; ++q)
-          v[q] = *reinterpret_cast<const f32x4*>(area + row * (R::W * 4) + ((((lane % R::LPR) * R::Q + q) ^ (row & 7)) * 16));
-        fn(j, s, row_at<T>(m0, j, s), row_col<T>(n0), v);
+          v[q] = *reinterpret_cast<const f32x4*>(area + row * (R::W * 4) + (((chunk_at<T>(s) * R::Q + q) ^ (row & 7)) * 16));
+        fn(j, s, row_at<T>(m0, j, s), row_col<T>(n0, s), v);
       }
       wave_lds_sync();
     }
@@ -350,28 +356,34 @@ struct Block {
 using Small = Block<64, 64, 2, 2>;
 using Mid = Block<128, 128, 2, 2>;
 using Large = Block<256, 256, 4, 2>;
+using Three = Block<256, 192, 4, 2>;  // gradients of 384 columns: two of these, where 256 leave a quarter empty
 
 // Edge of the output tile, 64, 128 or 256, for a product of M x N outputs in `splits` parts: the least estimated time, in units
-// of a compute unit's work.  A round of tiles takes as long as the tiles that share a compute unit; `rate` is what a tile
+// of a compute unit's work (`cost`).  A round of tiles takes as long as the tiles that share a compute unit; `rate` is what a tile
 // shape reaches of the best one's on full rounds: bf16 8192 cubed 460 / 998 / 1120 TFLOP/s, float 16384 x 4096 x 1024 120 / 131;
-// float has no registers for the largest.
-inline int pick_tile(long long M, long long N, long long splits, int dtype) {
-  static const struct { int edge, share; float rate16, rate32; } kinds[] = {{64, 4, 0.42f, 0.92f}, {128, 2, 0.9f, 1.f}, {256, 1, 1.f, 0.f}};
+// float has no registers for the largest.  A tile alone on a compute unit takes (1 + kAlone / 2) / 2 of two (float 2048 x 2048 x
+// 384, 256 tiles of 128 against 1024 of 64: both passes of the loss 171 -> 161 us; 0.4 to 1 choose alike).
+// `three`: 192 stands for 256 x 192 (dx and dw of 8192 x 30522 logits, 384 wide, bf16: 352 + 278 -> 201 + 207 us).
+constexpr double kAlone = 0.68;
+inline int pick_tile(long long M, long long N, long long splits, int dtype, bool three = false, double* cost = nullptr) {
+  static const struct { int edge, m, n, share; float rate16, rate32; } kinds[] = {
+      {64, 64, 64, 4, 0.42f, 0.92f}, {128, 128, 128, 2, 0.9f, 1.f}, {192, 256, 192, 1, 0.95f, 0.f}, {256, 256, 256, 1, 1.f, 0.f}};
   int best = 64;
   double least = 1e300;
   for (const auto& k : kinds) {
-    if (dtype == TT_F32 && k.rate32 == 0.f) continue;
-    const long long tiles = ((M + k.edge - 1) / k.edge) * ((N + k.edge - 1) / k.edge) * splits;
+    if ((dtype == TT_F32 && k.rate32 == 0.f) || (k.edge == 192 && !three)) continue;
+    const long long tiles = ((M + k.m - 1) / k.m) * ((N + k.n - 1) / k.n) * splits;
     const double rounds = (double)((tiles + 256 * k.share - 1) / (256 * k.share));
-    // the last round's compute units share their tiles only as far as there are any
+    // the last round's compute units share their tiles only as far as there are any; fewer workgroups hide less of their waits
     const long long last = tiles - (long long)(rounds - 1) * 256 * k.share;
-    const double share = rounds - 1 + (double)((last + 255) / 256) / k.share;
-    const double t = share * k.share * k.edge * k.edge / (dtype == TT_F32 ? k.rate32 : k.rate16);
+    const double n = (double)((last + 255) / 256), share = rounds - 1 + (n + kAlone * (1. - n / k.share)) / k.share;
+    const double t = share * k.share * k.m * k.n / (dtype == TT_F32 ? k.rate32 : k.rate16);
     if (t < least) {
       least = t;
       best = k.edge;
     }
   }
+  if (cost) *cost = least;
   return best;
 }
 
@@ -468,7 +480,7 @@ int tt_launch_grad_product(const GradProduct& g, int dtype, hipStream_t st);
 int tt_launch_slab_sum(const float* slab, int nsplit, long long n, void* out, int dtype, float alpha, const float* alpha_dev,
                        hipStream_t st);
 // splits of a [M, N] gradient product of contraction K
-int tt_grad_splits(long long M, long long N, long long K);
+int tt_grad_splits(long long M, long long N, long long K, int dtype);
 
 // packs a [rows, cols] matrix (row stride ld elements of `width` bytes) to row stride `ldp`, zeros behind cols (linear.hip)
 int tt_launch_pack(const void* src, long long ld, void* dst, long long ldp, long long rows, long long cols, int width,

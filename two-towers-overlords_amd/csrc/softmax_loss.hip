@@ -4,7 +4,8 @@
 //   G_ij = c_i (exp(l_ij - lse_i) - [j = target_i]),  dx = scale G w,  dw = scale G^T x
 //
 // float: a target that is nearly certain has G = c (p - 1), of which fp32's lse leaves few digits (5e-6 of dx where the logits reach
-// 20), so G is kept for whole rows and the target's entry is minus the sum of the row's others.
+// 20), so G is kept for whole rows and the target's entry is minus the sum of the row's others.  16-bit: an entry within twice
+// lse's rounding of 0 is 0.
 //
 // Forward: the product's epilogue leaves each row's maximum and sum of a tile's candidates (fp32, base 2); a second launch
 // joins them.  Backward: G is recomputed from x, w and lse into the workspace piece by piece.  16-bit types take pieces of the
@@ -115,15 +116,22 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   }
 }
 
-// joins the tiles' (maximum, sum) of each row: 16 rows x 16 lanes per workgroup, tiles in a fixed order
+// joins the tiles' (maximum, sum) of each row: ROWS rows x 256 / ROWS lanes per workgroup, tiles in a fixed order
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float mx = fmaxf(a.x, b.x), base = mx == -INFINITY ? 0.f : mx;
+  // a NaN sum is carried on
+  return make_float2(mx, a.y * __builtin_amdgcn_exp2f(a.x - base) + b.y * __builtin_amdgcn_exp2f(b.x - base));
+}
+template <int ROWS>
 __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restrict__ part, const float* __restrict__ tlogit,
                                                            const long long* __restrict__ target, long long ignore, int M, int V,
                                                            int gn, float scale2, float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ float2 red[16][17];
-  const int rl = threadIdx.x & 15, q = threadIdx.x >> 4, m = blockIdx.x * 16 + rl;
+  constexpr int LANES = 256 / ROWS;
+  __shared__ float2 red[256];
+  const int rl = threadIdx.x % ROWS, q = threadIdx.x / ROWS, m = blockIdx.x * ROWS + rl;
   float mx = -INFINITY, sum = 0.f;
   if (m < M) {
-    for (int t = q; t < gn; t += 16) {
+    for (int t = q; t < gn; t += LANES) {
       const float2 p = part[(long long)t * M + m];
       if (p.x > mx) {
         sum = fmaf(sum, __builtin_amdgcn_exp2f(mx - p.x), p.y);
@@ -133,18 +141,24 @@ __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restr
       }
     }
   }
-  red[rl][q] = make_float2(mx, sum);
-  __syncthreads();
+  red[threadIdx.x] = make_float2(mx, sum);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (q < o) red[threadIdx.x] = join(red[threadIdx.x], red[threadIdx.x + o * ROWS]);
+  }
   if (q != 0 || m >= M) return;
-  mx = -INFINITY;
-  for (int t = 0; t < 16; ++t) mx = fmaxf(mx, red[rl][t].x);
+  mx = red[rl].x;
+  sum = red[rl].y;
   const float base = mx == -INFINITY ? 0.f : mx;
-  sum = 0.f;
-  for (int t = 0; t < 16; ++t) sum += red[rl][t].y * __builtin_amdgcn_exp2f(red[rl][t].x - base);
   // in 64 bits, a row each: a row whose target is nearly certain has a loss far below its lse's rounding
   const double l = log2((double)sum), ln2 = 0.6931471805599453094;
   lse[m] = mx == -INFINITY && sum == 0.f ? -INFINITY : (float)((base + l) * ln2);
   const long long t = target[m];
+  if (t >= 0 && t < V && sum == __builtin_amdgcn_exp2f(fmaf(tlogit[m], scale2, -base))) {  // the target's term is the whole sum
+    loss[m] = 0.f;
+    return;
+  }
   loss[m] = t == ignore ? 0.f : (t < 0 || t >= V ? NAN : (float)(((double)base - (double)tlogit[m] * scale2 + l) * ln2));
 }
 
@@ -176,11 +190,15 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[q][e] = cp * __builtin_amdgcn_exp2f(fmaf(v[q][e], a.scale2, -lse2));
         if (t >= n && t < n + 4 * R::Q) {
+          const float least = fabsf(c) * fmaf(1.1920929e-7f, fabsf(lse), 2.3841858e-7f);
 #pragma unroll
           for (int q = 0; q < R::Q; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (n + 4 * q + e == t) v[q][e] = sizeof(T) == 4 ? 0.f : v[q][e] - c;
+              if (n + 4 * q + e == t) {
+                const float d = v[q][e] - c;  // a target that is the row's only candidate has 0
+                v[q][e] = sizeof(T) == 4 || fabsf(d) <= least ? 0.f : d;
+              }
         }
         const bool off = t == a.ignore;
         if (off || a.rid || n + 4 * R::Q > a.V) {
@@ -287,8 +305,8 @@ Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long 
     p.piece = pad_to((vp + p.pieces - 1) / p.pieces, 128);
     p.pieces = (int)((vp + p.piece - 1) / p.piece);
   }
-  p.sx = tt_grad_splits(p.rows, D, p.piece);
-  p.sw = p.blocks > 1 ? 1 : tt_grad_splits(p.piece, D, M);  // several blocks of rows add up in dw itself
+  p.sx = tt_grad_splits(p.rows, D, p.piece, dtype);
+  p.sw = p.blocks > 1 ? 1 : tt_grad_splits(p.piece, D, M, dtype);  // several blocks of rows add up in dw itself
   p.cmax = 256;
   p.G = align256((size_t)p.rows * p.piece * width);
   p.dx = p.pieces > 1 || p.sx > 1 ? align256((size_t)p.sx * p.rows * D * 4) : 0;
@@ -363,8 +381,10 @@ extern "C" int tt_softmax_loss(const void* x, int64_t ldx, const void* w, int64_
     });
   });
   if (rc != TT_OK) return rc;
-  hipLaunchKernelGGL(softmax_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, a.part, a.tlogit, a.target, a.ignore,
-                     (int)N, V, p.gn, a.scale2, loss, lse);
+  const bool few = N <= 2048 && p.gn > 64;  // 203 rows x 977 tiles: 24 us with 16 rows per workgroup, the pass 85 -> 67 with two
+  const int per = few ? 2 : 16;
+  hipLaunchKernelGGL(few ? softmax_join_kernel<2> : softmax_join_kernel<16>, dim3((unsigned)((N + per - 1) / per)), dim3(256), 0, st,
+                     a.part, a.tlogit, a.target, a.ignore, (int)N, V, p.gn, a.scale2, loss, lse);
   TT_CHECK_LAUNCH();
   return TT_OK;
 }
