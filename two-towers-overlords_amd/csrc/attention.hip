@@ -9,7 +9,7 @@
 // forms S^T = K Q^T, so a lane holds scores of ONE query: a row maximum is an in-lane maximum and one exchange with lane ^ 32,
 // and running maximum, sum and rescaling are one register per lane.  O^T = V^T P^T takes P^T straight from the score registers:
 // the K rows are read from LDS in an order (`fold`) that puts eight consecutive keys into a 16-bit lane's fragment (float:
-// four, in place).  V is transposed on its way into LDS.  The backward pass does the same from both sides: one kernel owns
+// four, in place).  V lies in LDS as in memory and is read across its rows (ds_read_b64_tr_b16).  The backward pass does the same from both sides: one kernel owns
 // queries (dq, and delta = dO.O), one owns keys (dk, dv); each recomputes S.  No atomics: results do not depend on the order.
 //
 // Which document a workgroup works on: document b gets floor(cu[b] / BM) + b as its first tile, which leaves every document
@@ -348,6 +348,12 @@ __device__ __forceinline__ int key_end(const Args& a, int prefix, int i1, int le
 }
 
 // ------------------------------------------------------------------------------------------------ forward
+// K and V tiles stream into one pair of LDS images while the other is in use: one barrier a tile.  A row's sum and output are
+// rescaled only when its maximum has grown by 2^8 (the probabilities stay below 2^8, fp32 sums do not mind).
+// Bound by vector arithmetic at heads of 32 and 64 (two matrix instructions of 32 x 32 x 16 per 32 keys and 16 exponentials, masks
+// and conversions per lane beside them), by bytes for short documents.  512 documents of 12-128 tokens, 12 heads of 32, float: 97
+// us (floor 45 by bytes); 5 of 1001-4096, heads of 64, bf16, prefix, cap and bias: 173 us, about 90 % of its cycles vector
+// instructions; 16 of 700-2048, 16 heads of 128 on 4, causal, fp16: 239 us, 575 TFLOP/s.
 template <class T, int DP, int WAVES, bool PLAIN>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 4 : DP == 64 ? 3 : 2))) void attention_fwd_kernel(Args a) {
   using D = Dim<T, DP>;
@@ -492,7 +498,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 // ------------------------------------------------------------------------------------------------ dq, delta
 // dS = P (dO V^T - delta) d,  dq_i = scale sum_j dS_ij k_j,  delta_i = dO_i . o_i
 // bf16 rounds dS to eight bits, as much again as dq's own rounding: its product takes dS in two parts (256 documents of 8-512
-// tokens, heads of 32: this kernel 181 -> 187 us, dq's error 1.5 -> 1.2 roundings).
+// tokens, 12 heads of 32, distance bias: this kernel 181 -> 220 us, dq's error 1.5 -> 1.2 roundings).
+// 10 operations per pair and head element against the forward's 4, 16 exponentials per lane and 32 keys as there: bound by vector
+// arithmetic at heads of 32, by the matrix units at 128 (16 documents of 700-2048, fp16, causal: 324 us, 640 TFLOP/s).
 template <class T, int DP, int WAVES, bool PLAIN>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 3 : DP == 64 || sizeof(T) == 2 ? 2 : 1))) void attention_dq_kernel(Args a) {
   using D = Dim<T, DP>;
@@ -648,6 +656,10 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 // ------------------------------------------------------------------------------------------------ dk, dv
 // A wave owns 32 keys (columns) and walks the queries, for every query head that shares the key head:
 // dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i
+// 8 operations per pair and head element.  256 documents of 8-512 tokens, 12 heads of 32, bf16: 272 us, vector arithmetic as in dq
+// (the statistics are per accumulator row here: 16 reads of lse and delta).  16 of 700-2048, 16 heads of 128 on 4, fp16: 695 us,
+// 395 TFLOP/s: two accumulators of the head's width and two operands take 392 registers, one wave per SIMD, so waits show;
+// dk and dv in kernels of their own (two waves) recompute S and took 312 + 421 us.
 template <class T, int DP, int WAVES, bool PLAIN>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 || (DP == 64 && sizeof(T) == 2) ? 2 : 1))) void attention_dkv_kernel(Args a) {
   using D = Dim<T, DP>;
