@@ -753,7 +753,7 @@ int tt_packed_attention_bwd(const tt_attention_args* args /* host */, tt_stream_
  *   lse[i] = log sum_j exp l_ij,   loss[i] = lse[i] - l_i,target[i]      (fp32)
  *   target [N] int64; a row whose target is ignore_index has loss 0 and no gradient, one whose target is otherwise outside
  *   [0, V) has loss NaN (and poisons the gradients).  row_ids [N] / cand_ids [V] (both or neither): candidates j != target
- *   with cand_ids[j] == row_ids[i] are left out of row i's sum.
+ *   with cand_ids[j] == row_ids[i] are left out of row i's sum (a row without a target keeps candidate 0).
  * tt_softmax_loss_bwd: row_coef [N] = d objective / d loss[i];  dx [N,D], dw [V,D] contiguous, of `dtype`, either may be null.
  */
 size_t tt_softmax_loss_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int V, int D, int dtype);

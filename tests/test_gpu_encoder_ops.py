@@ -472,7 +472,7 @@ def check_softmax(ops, dt, N, V, D, scale=1.0, groups=False, ignore=(), unit=Fal
     out = torch.zeros_like(l, dtype=torch.bool)
     if groups:
         out = rid[:, None] == cid[None]
-        out &= torch.arange(V, device="cuda")[None] != t[:, None]
+        out &= torch.arange(V, device="cuda")[None] != at
     l = torch.where(out, -math.inf, l)
     el = torch.where(out, 0.0, el)
     LSE = torch.logsumexp(l, 1)
@@ -638,3 +638,16 @@ def test_softmax_loss_of_a_single_candidate_is_exactly_nothing(ops, dt):
         loss, lse = ops.softmax_loss(x, w, t, scale=1.7, **kw)
         dx, dw = ops.softmax_loss_bwd(torch.ones(N, device="cuda"), x, w, t, lse, scale=1.7, **kw)
         assert not any(bool(a.any()) for a in (loss, dx, dw)), V
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_softmax_loss_rows_without_a_target_keep_candidate_0(ops, dt):
+    """All candidates in one group: a row's sum holds its target alone, or candidate 0 where it has none."""
+    g = gen(11)
+    x, w = randn(g, 9, 16).to(dt), randn(g, 300, 16).to(dt)
+    t = torch.tensor([5, -100, 299, -100, 0, 1, 2, -100, 3], device="cuda")
+    one = torch.ones(300, dtype=torch.int64, device="cuda")
+    loss, lse = ops.softmax_loss(x, w, t, row_ids=one[:9], cand_ids=one)
+    l = (x.double() * w[t.clamp(min=0)].double()).sum(1)
+    within("lse", lse, l, (16 + 3 * F) * E * (x.double().abs() * w[t.clamp(min=0)].double().abs()).sum(1) + 4 * E)
+    assert not bool(loss.any())

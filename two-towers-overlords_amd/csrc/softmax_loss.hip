@@ -16,7 +16,8 @@
 // into G; fp16 takes c / max|c| times 2^14, and the products' epilogues take both out again: probabilities keep their
 // precision down to 2^-28 of the largest.
 //
-// The candidates of the same group as a row (cand_ids[j] == row_ids[i], j not the target) are left out of its sum.
+// The candidates of the same group as a row (cand_ids[j] == row_ids[i], j not the target) are left out of its sum.  A row without a
+// target keeps candidate 0: its lse is defined, and nothing but lse depends on it.
 #include <type_traits>
 #include "mfma_tile.h"
 
@@ -83,12 +84,12 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
           if (at == i * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) a.tlogit[m] = acc[i][j][e];
     }
     if (!plain) {
-      const long long rid = in && a.rid ? a.rid[m] : 0;
+      const long long rid = in && a.rid ? a.rid[m] : 0, keep = t == a.ignore ? 0 : t;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (left_out(a, nw + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3), t, rid)) acc[i][j][e] = -INFINITY;
+          if (left_out(a, nw + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3), keep, rid)) acc[i][j][e] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll

@@ -691,7 +691,7 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, scale: 
     """Softmax cross entropy of every row of x [N, D] over the candidates w [V, D] -> (loss [N], lse [N]), both float32: the logits
     are scale * x @ w.T and are never stored.  target [N] int64: the row's candidate; `ignore_index` = no loss and no gradient
     for the row; any other value outside [0, V) gives NaN.  row_ids [N] / cand_ids [V] int64: candidates of the row's own id
-    other than its target are left out of its sum (the documents of the same query in an in-batch loss).
+    other than its target (candidate 0 where it has none) are left out of its sum (the documents of the same query in an in-batch loss).
     x and w: float32, bfloat16 or float16, row-strided views allowed."""
     dt, ldx, ldw, N, V, D = _softmax_args(x, w, target, scale, row_ids, cand_ids)
     loss = torch.empty(N, dtype=torch.float32, device=x.device)
