@@ -497,8 +497,10 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 
 // ------------------------------------------------------------------------------------------------ dq, delta
 // dS = P (dO V^T - delta) d,  dq_i = scale sum_j dS_ij k_j,  delta_i = dO_i . o_i
-// bf16 rounds dS to eight bits, as much again as dq's own rounding: its product takes dS in two parts (256 documents of 8-512
-// tokens, 12 heads of 32, distance bias: this kernel 181 -> 220 us, dq's error 1.5 -> 1.2 roundings).
+// dS rounded to 16 bits would cost as much again as dq's own rounding: its product takes dS in two parts (bf16, 256 documents of
+// 8-512 tokens, 12 heads of 32, distance bias: this kernel 181 -> 220 us, dq's error 1.5 -> 1.2 roundings; fp16, 16 of 700-2048,
+// 16 heads of 128: both passes 1140 -> 1176 us, 1.5 -> 1.2).  Where one tile holds all keys, delta is formed from P and dP before
+// dS: with a few keys dS is a small difference, and o's rounding in dO.o was 2 to 3 roundings of dq.
 // 10 operations per pair and head element against the forward's 4, 16 exponentials per lane and 32 keys as there: bound by vector
 // arithmetic at heads of 32, by the matrix units at 128 (16 documents of 700-2048, fp16, causal: 324 us, 640 TFLOP/s).
 template <class T, int DP, int WAVES, bool PLAIN>
@@ -573,7 +575,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
   fv(v0img, 0, vis, a.Dh, wave, lane);
   kb = mask_byte(D::TILE);
 
-  auto tile = [&](int k0, const char* __restrict__ kimg, const char* __restrict__ vimg, char* __restrict__ kn, char* __restrict__ vn) {
+  auto tile = [&](int k0, const char* __restrict__ kimg, const char* __restrict__ vimg, char* __restrict__ kn, char* __restrict__ vn, auto first) {
     stage_wait();
     const unsigned long long now = vis;
     if (k0 + D::TILE < kend) {
@@ -588,10 +590,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     const int rem = wend - k0;
     const Bias bias = bias_of<T, PLAIN>(a, un, i0 + wave * 32, i, k0, h);
     const float off = fmaf(bias.own, c, -lse2);
-#pragma unroll
-    for (int t = 0; t < D::SUB; ++t) {
-      if (32 * t >= rem) break;
-      f32x16 s, dp;
+    f32x16 s, sc;
+    auto scores = [&](int t) {  // s = P (dO V^T - delta), sc = the capped scores
+      f32x16 dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
 #pragma unroll
@@ -599,7 +600,6 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         mma<T>(s, Image<T, DP>::row(kimg, 32 * t + fold<T>(r), 2 * g + h), qf[g]);
         mma<T>(dp, Image<T, DP>::row(vimg, 32 * t + fold<T>(r), 2 * g + h), df[g]);
       }
-      f32x16 sc;
       if constexpr (!PLAIN) {
         sc = capped<T>(s, a);
         s = biased<T>(sc, bias, t);
@@ -611,6 +611,22 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = pick(bits, row_of<T>(e, 0), s[e], 0.f);
       }
+    };
+    if constexpr (decltype(first)::value && sizeof(T) == 2) {
+      if (kend <= D::TILE && k0 == 0) {  // all keys are here: delta without o's rounding first, few keys' dS cancel in it
+        float sum = 0.f;
+        for (int t = 0; t < D::SUB && 32 * t < rem; ++t) {
+          scores(t);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum += s[e];
+        }
+        delta += sum + __shfl_xor(sum, 32, 64);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < D::SUB; ++t) {
+      if (32 * t >= rem) break;
+      scores(t);
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) rest[e & 3] += s[e];
@@ -621,8 +637,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
         const u32x4 f = acc_frag<T>(s, g);
 #pragma unroll
         for (int u = 0; u < D::DT; ++u) mma<T>(acc[u], Image<T, DP>::col(kimg, t * D::PER + g, u, lane), f);
-        if constexpr (__is_same(T, __bf16)) {  // what bf16's eight bits left of dS
-          const bf16x8 hi = __builtin_bit_cast(bf16x8, f);
+        if constexpr (sizeof(T) == 2) {  // what the type's bits left of dS
+          typedef T t8 __attribute__((ext_vector_type(8)));
+          const t8 hi = __builtin_bit_cast(t8, f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[8 * g + e] -= (float)hi[e];
           const u32x4 lo = acc_frag<T>(s, g);
@@ -633,8 +650,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
     }
   };
   for (int k0 = 0; k0 < kend; k0 += 2 * D::TILE) {
-    tile(k0, k0img, v0img, k1img, v1img);
-    if (k0 + D::TILE < kend) tile(k0 + D::TILE, k1img, v1img, k0img, v0img);
+    tile(k0, k0img, v0img, k1img, v1img, std::true_type{});
+    if (k0 + D::TILE < kend) tile(k0 + D::TILE, k1img, v1img, k0img, v0img, std::false_type{});
   }
   if constexpr (sizeof(T) == 2) {  // the keys' kernel runs next and takes the better delta
     float r = (rest[0] + rest[1]) + (rest[2] + rest[3]);

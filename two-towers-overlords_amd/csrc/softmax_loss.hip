@@ -3,18 +3,18 @@
 //   l_ij = scale x_i.w_j,  lse_i = log sum_j exp l_ij,  loss_i = lse_i - l_i,target
 //   G_ij = c_i (exp(l_ij - lse_i) - [j = target_i]),  dx = scale G w,  dw = scale G^T x
 //
-// float: a target that is nearly certain has G = c (p - 1), of which fp32's lse leaves few digits (5e-6 of dx where the logits reach
-// 20), so G is kept for whole rows and the target's entry is minus the sum of the row's others.  16-bit: an entry within twice
-// lse's rounding of 0 is 0.
+// A target that is nearly certain has G = c (p - 1), of which fp32's lse leaves few digits (float, logits up to 20: 5e-6 of dx), so
+// where a piece holds whole rows (float always) the target's entry is minus the sum of the row's others, in 16-bit types if the
+// target's p is above 1/4.  Elsewhere an entry within twice lse's rounding of 0 is 0.
 //
 // Forward: the product's epilogue leaves each row's maximum and sum of a tile's candidates (fp32, base 2); a second launch
 // joins them.  Backward: G is recomputed from x, w and lse into the workspace piece by piece.  16-bit types take pieces of the
 // candidates (dw of a piece is final, dx is summed in fp32 over the pieces), float pieces of the rows (the other way round).
 // 8 N V D operations instead of 6 with stored logits.
 //
-// G is rounded to the operands' type (it feeds matrix instructions).  float and bf16 share fp32's exponent range, so c goes
-// into G; fp16 takes c / max|c| times 2^14, and the products' epilogues take both out again: probabilities keep their
-// precision down to 2^-28 of the largest.
+// G is rounded to the operands' type (it feeds matrix instructions).  float takes c as it is; 16-bit types take c / max|c|, so that
+// the rounding of a mean's 1 / N is not in every target's entry (bf16: up to 2^-8 of all of dx), fp16 times 2^14, which keeps its
+// precision down to 2^-28 of the largest.  The products' epilogues take the factor out again.
 //
 // The candidates of the same group as a row (cand_ids[j] == row_ids[i], j not the target) are left out of its sum.  A row without a
 // target keeps candidate 0: its lse is defined, and nothing but lse depends on it.
@@ -36,7 +36,8 @@ struct Args {
   int v0, V, gm, gn;     // first candidate of the piece; candidates in all; tiles along the rows and the candidates
   float scale2;          // scale * log2 e
   float2* part;          // [gn, M] (maximum, sum) of a tile's candidates
-  float* others;         // float's backward: [gn * WN, M] sums of G's entries, the target's left out
+  float* others;         // backward, where a piece holds whole rows: [gn * WN, M] sums of G's entries, the target's left out
+  int* near;             // 16-bit: [M] is the target's p large?
   float scale;
   float* tlogit;         // [M] the target's x.w
   const float *lse, *coef, *cmax;  // backward
@@ -179,14 +180,16 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   B blk;
   blk.template product<T, false, false>(b0, b1, a.X, a.W, a.s, m0, n0, 0, a.s.K);
   T* __restrict__ G = static_cast<T*>(a.G);
-  // what a row's coefficient is scaled by in G; the products' alpha takes fp16's out again, and has float's already
-  const float up = __is_same(T, _Float16) ? kF16Up / *a.cmax : (sizeof(T) == 4 ? a.scale : 1.f);
+  // what a row's coefficient is scaled by in G; the products' alpha takes 16-bit types' out again, and has float's already
+  const float up = sizeof(T) == 4 ? a.scale : (__is_same(T, _Float16) ? kF16Up : 1.f) / *a.cmax;
   using R = typename B::template Rows<T>;
   blk.template for_rows<T>(
       b0, b1, m0, n0, [](int) {},
       [&](int j, int s, int m, int nl, f32x4 (&v)[R::Q]) {
         if (m >= a.s.M || nl >= a.ldg) return;  // whole rows of lanes
         const long long t = a.target[m];
+        // the target's entry comes from the others: always in float, for a likely target in 16-bit types
+        const bool sums = sizeof(T) == 4 || (a.near && a.near[m]);
         const float lse = a.lse[m], c = t == a.ignore ? 0.f : (t < 0 || t >= a.V ? NAN : a.coef[m] * up);
         // lse in base 2 as two floats; the second one scales the row
         const float lse2 = lse * kLog2e, cp = c * __builtin_amdgcn_exp2f(-fmaf(lse, kLog2e, -lse2) - lse * kLog2eLow);
@@ -203,7 +206,7 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
             for (int e = 0; e < 4; ++e)
               if (n + 4 * q + e == t) {
                 const float d = v[q][e] - c;  // a target that is the row's only candidate has 0
-                v[q][e] = sizeof(T) == 4 || fabsf(d) <= least ? 0.f : d;
+                v[q][e] = sums || fabsf(d) <= least ? 0.f : d;
               }
         }
         const bool off = t == a.ignore;
@@ -214,8 +217,9 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[q][e] = (off | left_out(a, n + 4 * q + e, t, rid)) ? 0.f : v[q][e];
         }
-        if constexpr (sizeof(T) == 4) {
+        if (sizeof(T) == 4 || __any(sums)) {
           float sum = (v[0][0] + v[0][1]) + (v[0][2] + v[0][3]);
+          if constexpr (R::Q == 2) sum += (v[1][0] + v[1][1]) + (v[1][2] + v[1][3]);
 #pragma unroll
           for (int o = R::LPR / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
           if (blk.lane % R::LPR == 0) a.others[(long long)(tn * B::WN + blk.wn) * a.s.M + m] = sum;
@@ -227,10 +231,38 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
       });
 }
 
-// float: G's target entries, minus the sum of the row's others; 16 rows x 16 lanes per workgroup, parts in a fixed order
+// near[m]: is the target's p above 1/4?  A wave per row.  (With every row's sums the training pass of 8192 x 30522 bf16 took 1074 us,
+// without 993.)
+template <class T>
+__global__ __launch_bounds__(256) void softmax_near_kernel(Args a, int* __restrict__ near) {
+  const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (m >= a.s.M) return;
+  const long long t = a.target[m];
+  float dot = 0.f;
+  if (t >= 0 && t < a.V) {
+    const T* __restrict__ x = static_cast<const T*>(a.X.p) + m * a.X.ld;
+    const T* __restrict__ w = static_cast<const T*>(a.W.p) + t * a.W.ld;
+    for (int k = lane * Type<T>::KPF; k < a.s.K; k += 64 * Type<T>::KPF) {  // zeros behind K
+      Chunk<T> u, v;
+      u.load(x + k);
+      v.load(w + k);
+#pragma unroll
+      for (int q = 0; q < Chunk<T>::Q; ++q) {
+        const f32x4 y = from_quad<T>(u.q[q]) * from_quad<T>(v.q[q]);
+        dot += (y[0] + y[1]) + (y[2] + y[3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+  if (lane == 0) near[m] = fmaf(dot, a.scale2, -a.lse[m] * kLog2e) > -2.f;
+}
+
+// G's target entries, minus the sum of the row's others; 16 rows x 16 lanes per workgroup, parts in a fixed order
+template <class T>
 __global__ __launch_bounds__(256) void softmax_target_kernel(const float* __restrict__ others, const long long* __restrict__ target,
-                                                             long long ignore, int M, int V, int parts, float* __restrict__ G,
-                                                             long long ldg) {
+                                                             const int* __restrict__ near, long long ignore, int M, int V, int parts,
+                                                             T* __restrict__ G, long long ldg) {
   __shared__ float red[16][17];
   const int rl = threadIdx.x & 15, q = threadIdx.x >> 4, m = blockIdx.x * 16 + rl;
   float sum = 0.f;
@@ -240,15 +272,15 @@ __global__ __launch_bounds__(256) void softmax_target_kernel(const float* __rest
   __syncthreads();
   if (q != 0 || m >= M) return;
   const long long t = target[m];
-  if (t == ignore || t < 0 || t >= V) return;
+  if (t == ignore || t < 0 || t >= V || (near && !near[m])) return;
   sum = 0.f;
   for (int i = 0; i < 16; ++i) sum += red[rl][i];
-  G[m * ldg + t] = -sum;
+  G[m * ldg + t] = (T)-sum;
 }
 
-// cmax[0] = max |coef| over the rows that have a target (1 if that is 0 or not finite), cmax[1] = cmax[0] / kF16Up
+// cmax[0] = max |coef| over the rows that have a target (1 if that is 0 or not finite), cmax[1] = cmax[0] / up
 __global__ __launch_bounds__(1024) void softmax_cmax_kernel(const float* __restrict__ coef, const long long* __restrict__ target,
-                                                            long long ignore, int M, float* __restrict__ cmax) {
+                                                            long long ignore, int M, float up, float* __restrict__ cmax) {
   __shared__ float red[16];
   float v = 0.f;
   for (int m = threadIdx.x; m < M; m += 1024)
@@ -261,7 +293,7 @@ __global__ __launch_bounds__(1024) void softmax_cmax_kernel(const float* __restr
   for (int i = 1; i < 16; ++i) v = fmaxf(v, red[i]);
   if (!(v > 0.f) || v == INFINITY) v = 1.f;
   cmax[0] = v;
-  cmax[1] = v / kF16Up;
+  cmax[1] = v / up;
 }
 
 template <class F>
@@ -279,7 +311,7 @@ struct Plan {
   long long piece, rows;  // candidates (a multiple of 128) and rows of a piece of G
   int pieces, blocks;     // pieces of the candidates, pieces of the rows (one of them is 1)
   int sx, sw;             // splits of the two gradient products
-  size_t x, w, part, tlogit, cmax, G, others, dx, dw, fwd, bwd;
+  size_t x, w, part, tlogit, cmax, G, others, near, dx, dw, fwd, bwd;
 };
 constexpr long long kPieceBytes = 512LL << 20;  // of G; 8192 rows x 30522 bf16 candidates: 64 MB 1421 us, 128 1279, 256 1272, 512 1217
 Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long M, int V, int D, int dtype) {
@@ -304,20 +336,22 @@ Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long 
     if (most >= 128) p.rows = pad_to(p.rows, 128);
     if (p.rows > M) p.rows = M;
     p.blocks = (int)((M + p.rows - 1) / p.rows);
-    p.others = align256((size_t)((vp + 63) / 64) * 2 * p.rows * 4);  // at least the parts of any tile shape
   } else {
     const long long cap = kPieceBytes / (M * width) / 128 * 128, most = cap < 1024 ? 1024 : cap;
     p.pieces = (int)((vp + most - 1) / most);
     p.piece = pad_to((vp + p.pieces - 1) / p.pieces, 128);
     p.pieces = (int)((vp + p.piece - 1) / p.piece);
   }
+  // whole rows of G: sums of a row's parts, as many as any tile shape has
+  if (p.pieces == 1) p.others = align256((size_t)((vp + 63) / 64) * 2 * p.rows * 4);
+  if (p.pieces == 1 && dtype != TT_F32) p.near = align256((size_t)p.rows * 4);
   p.sx = tt_grad_splits(p.rows, D, p.piece, dtype);
   p.sw = p.blocks > 1 ? 1 : tt_grad_splits(p.piece, D, M, dtype);  // several blocks of rows add up in dw itself
   p.cmax = 256;
   p.G = align256((size_t)p.rows * p.piece * width);
   p.dx = p.pieces > 1 || p.sx > 1 ? align256((size_t)p.sx * p.rows * D * 4) : 0;
   p.dw = p.sw > 1 ? align256((size_t)p.sw * p.piece * D * 4) : 0;
-  p.bwd = p.x + p.w + p.cmax + p.G + p.others + p.dx + p.dw;
+  p.bwd = p.x + p.w + p.cmax + p.G + p.others + p.near + p.dx + p.dw;
   return p;
 }
 
@@ -419,13 +453,16 @@ extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t
   ws += p.w;
   float* cmax = (float*)ws;   ws += p.cmax;
   a.G = ws;                   ws += p.G;
-  a.others = (float*)ws;      ws += p.others;
+  a.others = p.others ? (float*)ws : nullptr;
+  ws += p.others;
+  a.near = p.near ? (int*)ws : nullptr;
+  ws += p.near;
   float* dxs = (float*)ws;    ws += p.dx;
   float* dws = (float*)ws;
   const float* alpha_dev = nullptr;
-  if (dtype == TT_F16) {
+  if (dtype != TT_F32) {
     hipLaunchKernelGGL(softmax_cmax_kernel, dim3(1), dim3(1024), 0, st, row_coef, (const long long*)target, (long long)ignore_index,
-                       (int)N, cmax);
+                       (int)N, dtype == TT_F16 ? kF16Up : 1.f, cmax);
     TT_CHECK_LAUNCH();
     alpha_dev = cmax + 1;
   }
@@ -451,13 +488,17 @@ extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t
     TT_REQUIRE(grid <= 0x7fffffffLL, TT_ERR_BAD_SHAPE);
     rc = with_type(dtype, [&](auto tag) {
       using T = decltype(tag);
+      if (a.near) {
+        hipLaunchKernelGGL(softmax_near_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, a.near);
+        TT_CHECK_LAUNCH();
+      }
       return with_block<T>(b, [&](auto* shape) {
         using B = std::remove_pointer_t<decltype(shape)>;
         hipLaunchKernelGGL((softmax_grad_kernel<T, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
         TT_CHECK_LAUNCH();
-        if (sizeof(T) == 4) {
-          hipLaunchKernelGGL(softmax_target_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a.others, a.target, a.ignore,
-                             rows, V, a.gn * B::WN, (float*)a.G, a.ldg);
+        if (a.others) {
+          hipLaunchKernelGGL(softmax_target_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a.others, a.target, a.near, a.ignore,
+                             rows, V, a.gn * B::WN, (T*)a.G, a.ldg);
           TT_CHECK_LAUNCH();
         }
         return (int)TT_OK;
