@@ -651,3 +651,20 @@ def test_softmax_loss_rows_without_a_target_keep_candidate_0(ops, dt):
     l = (x.double() * w[t.clamp(min=0)].double()).sum(1)
     within("lse", lse, l, (16 + 3 * F) * E * (x.double().abs() * w[t.clamp(min=0)].double().abs()).sum(1) + 4 * E)
     assert not bool(loss.any())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("c", [0.0, 1e-44, 1e-39, 1e-20, 1e20])
+def test_softmax_loss_coefficients_of_any_size(ops, dt, c):
+    """16-bit gradients of the logits are relative to the largest coefficient, whatever its size."""
+    g = gen(3)
+    x, w = randn(g, 33, 24).to(dt), randn(g, 70, 24).to(dt)
+    t = torch.randint(0, 70, (33,), generator=g, device="cuda")
+    _, lse = ops.softmax_loss(x, w, t)
+    dx, dw = ops.softmax_loss_bwd(torch.full((33,), c, device="cuda"), x, w, t, lse)
+    if c <= 1e-39:
+        assert all(bool((a.abs() <= 1e-36).all()) for a in (dx, dw))
+    elif dt != torch.float16:  # beyond fp16's range
+        one = ops.softmax_loss_bwd(torch.ones(33, device="cuda"), x, w, t, lse)
+        for a, b in zip((dx, dw), one):  # each G and each result rounded once on either side
+            within("scaled", a.double() / c, b.double(), 4 * half(dt) * (b.double().abs() + b.double().abs().amax()) + 64 * E * b.double().abs().amax())

@@ -502,7 +502,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 // 16 heads of 128: both passes 1140 -> 1176 us, 1.5 -> 1.2).  Where one tile holds all keys, delta is formed from P and dP before
 // dS: with a few keys dS is a small difference, and o's rounding in dO.o was 2 to 3 roundings of dq.
 // 10 operations per pair and head element against the forward's 4, 16 exponentials per lane and 32 keys as there: bound by vector
-// arithmetic at heads of 32, by the matrix units at 128 (16 documents of 700-2048, fp16, causal: 324 us, 640 TFLOP/s).
+// arithmetic at heads of 32, by the matrix units at 128 (16 documents of 700-2048, fp16, causal: 344 us, 600 TFLOP/s).
 template <class T, int DP, int WAVES, bool PLAIN>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 3 : DP == 64 || sizeof(T) == 2 ? 2 : 1))) void attention_dq_kernel(Args a) {
   using D = Dim<T, DP>;
@@ -674,8 +674,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 // A wave owns 32 keys (columns) and walks the queries, for every query head that shares the key head:
 // dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i
 // 8 operations per pair and head element.  256 documents of 8-512 tokens, 12 heads of 32, bf16: 272 us, vector arithmetic as in dq
-// (the statistics are per accumulator row here: 16 reads of lse and delta).  16 of 700-2048, 16 heads of 128 on 4, fp16: 695 us,
-// 395 TFLOP/s: two accumulators of the head's width and two operands take 392 registers, one wave per SIMD, so waits show;
+// (the statistics are per accumulator row here: 16 reads of lse and delta).  16 of 700-2048, 16 heads of 128 on 4, fp16: 670 us,
+// 410 TFLOP/s: two accumulators of the head's width and two operands take 392 registers, one wave per SIMD, so waits show;
 // dk and dv in kernels of their own (two waves) recompute S and took 312 + 421 us.
 template <class T, int DP, int WAVES, bool PLAIN>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 || (DP == 64 && sizeof(T) == 2) ? 2 : 1))) void attention_dkv_kernel(Args a) {

@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restr
 }
 
 // G of a piece of the candidates, [M, ldg] in T; columns behind the last candidate are zero.  The logits' product again, then 500 MB of
-// G at 8192 x 30522 bf16: 364 us (product and exponentials 258, the rest the stores, through LDS as whole rows).  Keeping the
+// G at 8192 x 30522 bf16: 388 us (product and exponentials 258, the rest the stores, through LDS as whole rows).  Keeping the
 // logits instead would write and read them once more and need N V elements.
 template <class T, class B>
 __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void softmax_grad_kernel(Args a) {
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256) void softmax_target_kernel(const float* __rest
   __shared__ float red[16][17];
   const int rl = threadIdx.x & 15, q = threadIdx.x >> 4, m = blockIdx.x * 16 + rl;
   float sum = 0.f;
-  if (m < M)
+  if (m < M && (!near || near[m]))
     for (int t = q; t < parts; t += 16) sum += others[(long long)t * M + m];
   red[rl][q] = sum;
   __syncthreads();
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(256) void softmax_target_kernel(const float* __rest
   G[m * ldg + t] = (T)-sum;
 }
 
-// cmax[0] = max |coef| over the rows that have a target (1 if that is 0 or not finite), cmax[1] = cmax[0] / up
+// cmax[0] = max |coef| over the rows that have a target (1 if that is infinite, at least 10^-30), cmax[1] = cmax[0] / up
 __global__ __launch_bounds__(1024) void softmax_cmax_kernel(const float* __restrict__ coef, const long long* __restrict__ target,
                                                             long long ignore, int M, float up, float* __restrict__ cmax) {
   __shared__ float red[16];
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(1024) void softmax_cmax_kernel(const float* __restr
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int i = 1; i < 16; ++i) v = fmaxf(v, red[i]);
-  if (!(v > 0.f) || v == INFINITY) v = 1.f;
+  v = v == INFINITY ? 1.f : fmaxf(v, 1e-30f);  // 1 / v times 2^14 is finite
   cmax[0] = v;
   cmax[1] = v / up;
 }
