@@ -36,7 +36,7 @@ struct Args {
   int v0, V, gm, gn;     // first candidate of the piece; candidates in all; tiles along the rows and the candidates
   float scale2;          // scale * log2 e
   float2* part;          // [gn, M] (maximum, sum) of a tile's candidates
-  float* others;         // backward, where a piece holds whole rows: [gn * WN, M] sums of G's entries, the target's left out
+  float* others;         // backward, where a piece holds whole rows: [row_parts, M] sums of G's entries, the target's left out
   int* near;             // 16-bit: [M] is the target's p large?
   float scale;
   float* tlogit;         // [M] the target's x.w
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2)))
   blk.template for_rows<T>(
       b0, b1, m0, n0, [](int) {},
       [&](int j, int s, int m, int nl, f32x4 (&v)[R::Q]) {
-        if (m >= a.s.M || nl >= a.ldg) return;  // whole rows of lanes
+        if (m >= a.s.M || nl >= a.ldg) return;  // whole rows of lanes; behind ldg whole waves, whose part of `others` is no row_part
         const long long t = a.target[m];
         // the target's entry comes from the others: always in float, for a likely target in 16-bit types
         const bool sums = sizeof(T) == 4 || (a.near && a.near[m]);
@@ -497,8 +497,9 @@ extern "C" int tt_softmax_loss_bwd(const float* row_coef, const void* x, int64_t
         hipLaunchKernelGGL((softmax_grad_kernel<T, B>), dim3((unsigned)grid), dim3(B::THREADS), 0, st, a);
         TT_CHECK_LAUNCH();
         if (a.others) {
+          static_assert(B::WN == 2 && B::NI * 64 == B::BN && 128 % (B::NI * 32) == 0, "row_parts");
           hipLaunchKernelGGL(softmax_target_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a.others, a.target, a.near, a.ignore,
-                             rows, V, a.gn * B::WN, (T*)a.G, a.ldg);
+                             rows, V, row_parts(B::BN, a.gn, a.ldg), (T*)a.G, a.ldg);
           TT_CHECK_LAUNCH();
         }
         return (int)TT_OK;
