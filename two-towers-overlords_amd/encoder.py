@@ -112,8 +112,9 @@ def attention_qkv(qkv: Tensor, heads: int, cu_seqlens: Tensor, *, scale: Optiona
 
 class PackedBertEncoder:
     """A transformers `BertModel`'s forward on packed tokens.  Holds the module, not copies of its weights: loading a
-    checkpoint, moving or fine-tuning it needs nothing here.  Under `torch.autocast` everything runs in the autocast type;
-    else in the weights' own.  Differentiable in the weights that require a gradient."""
+    checkpoint, moving or fine-tuning it needs nothing here.  Under `torch.autocast` the products and the attention run in the
+    autocast type, the residual sums and the norms in float32, like the stock forward's; else everything in the weights' own
+    type.  Differentiable in the weights that require a gradient."""
 
     def __init__(self, model: nn.Module):
         cfg = getattr(model, "config", None)
@@ -139,8 +140,9 @@ class PackedBertEncoder:
         self.model = model
 
     @staticmethod
-    def _compute_type(weight: Tensor) -> torch.dtype:
-        return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else weight.dtype
+    def _types(weight: Tensor) -> Tuple[torch.dtype, torch.dtype]:
+        """(type of the products, type of the rows between them)"""
+        return (torch.get_autocast_dtype("cuda"), torch.float32) if torch.is_autocast_enabled("cuda") else (weight.dtype, weight.dtype)
 
     def __call__(self, input_ids: Tensor, attention_mask: Optional[Tensor] = None, token_type_ids: Optional[Tensor] = None):
         """input_ids [B, S] (padded, any mask pattern) -> (hidden [T, D] of the T attended tokens in row order, slots [T]: their
@@ -161,13 +163,13 @@ class PackedBertEncoder:
             slots = keep.reshape(-1).nonzero().squeeze(1)
             lens = keep.sum(1)
         cu = F.pad(lens.cumsum(0), (1, 0)).to(torch.int32)
-        dt = self._compute_type(emb.word_embeddings.weight)
+        dt, rows = self._types(emb.word_embeddings.weight)
         with torch.autocast("cuda", enabled=False):
             x = F.embedding(input_ids.reshape(-1)[slots].long(), emb.word_embeddings.weight, padding_idx=emb.word_embeddings.padding_idx)
             x = x + F.embedding(slots % S, emb.position_embeddings.weight)
             types = emb.token_type_embeddings.weight
             x = x + (types[0] if token_type_ids is None else F.embedding(token_type_ids.reshape(-1)[slots].long(), types))
-            x = self._norm(x, emb.LayerNorm).to(dt)
+            x = self._norm(x.to(rows), emb.LayerNorm)
             for layer in (m.encoder.layer if slots.numel() else ()):  # no token, nothing to do
                 x = self._layer(x, cu, layer, dt)
         return x, slots
@@ -181,15 +183,17 @@ class PackedBertEncoder:
         qkv = (at.self.query, at.self.key, at.self.value)
         w = torch.cat([p.weight for p in qkv]).to(dt)
         b = torch.cat([p.bias for p in qkv]).to(dt)
-        h = linear(x, w, b).view(-1, 3 * self.heads, self.head_dim)
+        h = linear(x.to(dt), w, b).view(-1, 3 * self.heads, self.head_dim)
         h = attention_qkv(h, self.heads, cu).reshape(-1, self.heads * self.head_dim)
         x = self._norm(self._dense(h, at.output.dense, dt, residual=x), at.output.LayerNorm)
-        h = self._dense(x, layer.intermediate.dense, dt, activation=self.activation)
+        h = self._dense(x.to(dt), layer.intermediate.dense, dt, activation=self.activation)
         return self._norm(self._dense(h, layer.output.dense, dt, residual=x), layer.output.LayerNorm)
 
     @staticmethod
     def _dense(x: Tensor, d: nn.Linear, dt: torch.dtype, residual: Optional[Tensor] = None, activation: str = "none") -> Tensor:
-        return linear(x, d.weight.to(dt), None if d.bias is None else d.bias.to(dt), residual, activation)
+        fused = residual if residual is None or residual.dtype == dt else None
+        y = linear(x, d.weight.to(dt), None if d.bias is None else d.bias.to(dt), fused, activation)
+        return y if fused is residual else y + residual  # autocast: rows of float32
 
     def padded(self, input_ids: Tensor, attention_mask: Optional[Tensor] = None, token_type_ids: Optional[Tensor] = None) -> Tensor:
         """The stock forward's last_hidden_state [B, S, D] in float32, zero where a token is not attended."""
