@@ -24,8 +24,8 @@ ACTIVATIONS = {"gelu": "gelu", "gelu_python": "gelu", "gelu_new": "gelu_tanh", "
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        need = any(ctx.needs_input_grad[:3])
+    def forward(ctx, x, weight, bias, residual, activation, recording):
+        need = recording and any(ctx.needs_input_grad[:3])  # (needs_input_grad is set under no_grad as well)
         y, z = ops.linear_act(x, weight, bias, residual, activation, save_preact=True) if need else (
             ops.linear_act(x, weight, bias, residual, activation), None)
         ctx.activation = activation
@@ -40,7 +40,7 @@ class _LinearFn(torch.autograd.Function):
         if dy.stride(-1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
             dy = dy.contiguous()  # a broadcast upstream gradient (sum().backward())
         dx, dw, db = ops.linear_act_bwd(dy, x, weight, z, ctx.activation, bias=nb, need_dx=nx, need_dw=nw) if nx or nw or nb else (None,) * 3
-        return dx, dw, db, dy if nr else None, None
+        return dx, dw, db, dy if nr else None, None, None
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, residual: Optional[Tensor] = None, activation: str = "none") -> Tensor:
@@ -50,7 +50,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, residual: O
         if residual.shape != lead + weight.shape[:1]:
             raise ValueError(f"residual: expected shape {tuple(lead + weight.shape[:1])}, got {tuple(residual.shape)}")
         residual = residual.reshape(-1, weight.shape[0])
-    y = _LinearFn.apply(x.reshape(-1, x.shape[-1]), weight, bias, residual, activation)
+    y = _LinearFn.apply(x.reshape(-1, x.shape[-1]), weight, bias, residual, activation, torch.is_grad_enabled())
     return y.view(*lead, weight.shape[0])
 
 
