@@ -94,3 +94,36 @@ def test_gradients_reach_every_weight_under_autocast():
         err = float((grads["packed"][n] - w).norm())
         # a chain of 2 layers x 8 products either way, each rounded to 2^-9 of its size
         assert err <= 2 * 2 * 8 * 2.0 ** -9 * max(float(w.norm()), 1e-2 * top), (n, err, float(w.norm()))
+
+
+def two_towers(m, **kw):
+    from two_towers_overlords_amd.model import TwoTowersModel
+
+    return TwoTowersModel(projection_dim=16, tokenizer=lambda *a, **k: None, pretrained_model=m, encoder_mode="bert", encoder_impl="hip", **kw).cuda()
+
+
+def test_a_frozen_encoder_with_dropout_runs_in_train_mode():
+    """train_epoch_optimized switches the model to train mode by itself; the frozen encoder's features are eval mode's."""
+    from two_towers_overlords_amd.model import TripletLoss
+    from two_towers_overlords_amd.training import train_epoch_optimized
+
+    model = two_towers(bert(dropout=0.1))
+    ids, mask = texts()
+    want = model.query_tower.pool_tokens({"input_ids": ids, "attention_mask": mask})
+    opt = torch.optim.Adam([p for p in model.parameters() if p.requires_grad], lr=1e-3)
+    batches = [tuple(texts(B=6, S=20, seed=10 * i + r) for r in range(3)) for i in range(2)]
+    avg = train_epoch_optimized(model, batches, TripletLoss(), opt, log_wandb=False)
+    assert avg == avg and model.training and model.query_tower.pretrained_model.training
+    assert torch.equal(model.query_tower.pool_tokens({"input_ids": ids, "attention_mask": mask}), want)
+
+
+def test_a_trained_encoder_with_dropout_is_refused_in_train_mode():
+    from two_towers_overlords_amd.encoder import PackedBertEncoder
+
+    model = two_towers(bert(dropout=0.1), train_encoder=True)
+    ids, mask = texts()
+    model.encode_query_ids(ids, mask)
+    model.train()
+    for f in (lambda: model.encode_query_ids(ids, mask), lambda: PackedBertEncoder(bert(dropout=0.1).train())(ids, mask)):
+        with pytest.raises(RuntimeError, match="dropout"):
+            f()

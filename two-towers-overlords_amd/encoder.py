@@ -114,9 +114,11 @@ class PackedBertEncoder:
     """A transformers `BertModel`'s forward on packed tokens.  Holds the module, not copies of its weights: loading a
     checkpoint, moving or fine-tuning it needs nothing here.  Under `torch.autocast` the products and the attention run in the
     autocast type, the residual sums and the norms in float32, like the stock forward's; else everything in the weights' own
-    type.  Differentiable in the weights that require a gradient."""
+    type.  Differentiable in the weights that require a gradient.  There is no dropout: a module in train mode whose dropout
+    probabilities are not 0 is refused, unless `frozen` says that its weights are not trained — it then runs as in eval mode,
+    which is what a feature cache of it holds."""
 
-    def __init__(self, model: nn.Module):
+    def __init__(self, model: nn.Module, frozen: bool = False):
         cfg = getattr(model, "config", None)
         try:
             emb, layers = model.embeddings, list(model.encoder.layer)
@@ -138,6 +140,7 @@ class PackedBertEncoder:
             raise ValueError(f"encoder_impl='hip': head size {cfg.hidden_size}/{self.heads} is not a multiple of 8 in 8..128")
         self.activation = ACTIVATIONS[act]
         self.model = model
+        self.frozen = frozen
 
     @staticmethod
     def _types(weight: Tensor) -> Tuple[torch.dtype, torch.dtype]:
@@ -148,7 +151,7 @@ class PackedBertEncoder:
         """input_ids [B, S] (padded, any mask pattern) -> (hidden [T, D] of the T attended tokens in row order, slots [T]: their
         places in the padded [B * S]).  One read-back: the number of attended tokens."""
         m = self.model
-        if m.training and any(isinstance(d, nn.Dropout) and d.p > 0 for d in m.modules()):
+        if m.training and not self.frozen and any(isinstance(d, nn.Dropout) and d.p > 0 for d in m.modules()):
             raise RuntimeError("encoder_impl='hip' has no dropout: put the encoder in eval mode, or set its dropout probabilities to 0")
         B, S = input_ids.shape
         emb = m.embeddings

@@ -108,7 +108,8 @@ class AveragePoolingTower(nn.Module):
         train_encoder: bool = False,
     ):
         """encoder_impl (`bert` mode): "torch" = the stock PyTorch forward, padded like the reference's; "hip" = the same
-        encoder on packed tokens and this package's kernels (encoder.PackedBertEncoder; equal up to rounding).
+        encoder on packed tokens and this package's kernels (encoder.PackedBertEncoder; equal up to rounding to the stock
+        forward in eval mode: it has no dropout, and a frozen encoder runs without it in train mode too).
         train_encoder (`bert` mode on "hip"): the encoder's weights are not frozen, and gradients reach them — an
         extension, backend/model.py:29-30 always freezes them."""
         super().__init__()
@@ -221,7 +222,7 @@ class AveragePoolingTower(nn.Module):
             from .encoder import PackedBertEncoder
 
             with torch.set_grad_enabled(torch.is_grad_enabled() and self.train_encoder):
-                hidden = PackedBertEncoder(self.pretrained_model).padded(ids, mask, tokens.get("token_type_ids"))
+                hidden = PackedBertEncoder(self.pretrained_model, frozen=not self.train_encoder).padded(ids, mask, tokens.get("token_type_ids"))
                 if not hidden.requires_grad:
                     return ops.pool_norm_dense(hidden, None if mask is None else mask.contiguous())
                 # model.py:55-56,63-72, differentiable; tokens that are not attended are zero rows already
