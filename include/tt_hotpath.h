@@ -705,6 +705,8 @@ int tt_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
  * Gradients of tt_linear_act: dz = dy act'(preact);  dx [M,K] = dz w,  dw [N,K] = dz^T x,  dbias [N] = column sums of dz
  * (each may be null; all contiguous, of `dtype`).  The residual's gradient is dy itself.  preact may be null for
  * TT_ACT_NONE.  dz is rounded to `dtype` for the products (dbias is summed before that).  M == 0: dw and dbias are zero.
+ * The workspace query counts what the wanted gradients need: w null = no dx, x null = no dw (the call reads w for dx only and x
+ * for dw only).  A larger workspace is always enough.
  */
 size_t tt_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
                                          int64_t M, int N, int K, int dtype, int act);
@@ -755,6 +757,7 @@ int tt_packed_attention_bwd(const tt_attention_args* args /* host */, tt_stream_
  *   [0, V) has loss NaN (and poisons the gradients).  row_ids [N] / cand_ids [V] (both or neither): candidates j != target
  *   with cand_ids[j] == row_ids[i] are left out of row i's sum (a row without a target keeps candidate 0).
  * tt_softmax_loss_bwd: row_coef [N] = d objective / d loss[i];  dx [N,D], dw [V,D] contiguous, of `dtype`, either may be null.
+ *   Its workspace covers both (the logits' gradients, which either needs, are the larger part).
  */
 size_t tt_softmax_loss_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int V, int D, int dtype);
 int tt_softmax_loss(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, const int64_t* row_ids,

@@ -49,3 +49,31 @@ def test_small_values_are_good_to_the_types_rounding(dt, act, rows):
     dz, _, _ = ops.linear_act_bwd(torch.ones_like(z), z, one, z, act)  # = act'(z)
     worst = ((dz.double() - D).abs() - (u * D.abs() + (1 + u) * rel * mag + floor + times * 2.0 ** -126)).max()
     assert float(worst) <= 0
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("odd", [False, True])
+def test_each_gradient_alone_in_the_workspace_that_it_asks_for(dt, act, odd):
+    """The C entry with dx, dw and dbias in every combination: the same bits as together, nothing written behind the workspace."""
+    import two_towers_overlords_amd as pkg
+    from two_towers_overlords_amd import _lib, ops
+
+    lib = pkg.load()
+    code = {torch.float32: _lib.TT_F32, torch.bfloat16: _lib.TT_BF16, torch.float16: _lib.TT_F16}[dt]
+    M, N, K = 3001, 72, 40 + odd
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, w, dy = (torch.randn(*s, generator=g, device="cuda").to(dt) for s in ((M, K), (N, K), (M, N)))
+    _, z = ops.linear_act(x, w, None, None, act, save_preact=True)
+    want = ops.linear_act_bwd(dy, x, w, z, act)
+    for need in range(1, 8):
+        outs = [torch.empty_like(t) if need >> i & 1 else None for i, t in enumerate(want)]
+        ptr = [None if o is None else o.data_ptr() for o in outs]
+        n = lib.tt_linear_act_bwd_workspace_bytes(dy.data_ptr(), N, x.data_ptr() if need & 2 else None, K, w.data_ptr() if need & 1 else None, K,
+                                                  M, N, K, code, _lib.ACTIVATIONS[act])
+        ws = torch.full((n + 4096,), 77, dtype=torch.uint8, device="cuda")
+        rc = lib.tt_linear_act_bwd(dy.data_ptr(), N, x.data_ptr(), K, w.data_ptr(), K, None if z is None else z.data_ptr(), *ptr, M, N, K, code,
+                                   _lib.ACTIVATIONS[act], ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        assert bool((ws[n:] == 77).all())
+        assert all(o is None or torch.equal(o, t) for o, t in zip(outs, want))

@@ -584,7 +584,7 @@ struct BwdPlan {
   size_t dz, x, w, slab, part, total;
 };
 BwdPlan bwd_plan(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K,
-                 int dtype, int act, bool need_dw) {
+                 int dtype, int act, bool need_dx, bool need_dw) {
   BwdPlan p{};
   const int width = dtype_bytes(dtype);
   p.own_dz = act != TT_ACT_NONE || !packed_ok(dy, lddy, N, dtype);
@@ -598,9 +598,9 @@ BwdPlan bwd_plan(const void* dy, int64_t lddy, const void* x, int64_t ldx, const
   if (p.rows < 1) p.rows = 1;
   p.row_blocks = (int)((M + p.rows - 1) / p.rows);
   if (p.row_blocks < 1) p.row_blocks = 1;
-  p.dz = p.own_dz ? align256((size_t)M * p.ldz * width) : 0;
-  p.x = pack_bytes(x, ldx, M, K, dtype);
-  p.w = pack_bytes(w, ldw, N, K, dtype);
+  p.dz = p.own_dz && (need_dx || need_dw) ? align256((size_t)M * p.ldz * width) : 0;
+  p.x = need_dw ? pack_bytes(x, ldx, M, K, dtype) : 0;
+  p.w = need_dx ? pack_bytes(w, ldw, N, K, dtype) : 0;
   p.slab = p.splits > 1 ? align256((size_t)p.splits * N * K * 4) : 0;
   p.part = align256((size_t)p.row_blocks * N * 4);
   p.total = p.dz + p.x + p.w + p.slab + p.part;
@@ -611,7 +611,7 @@ BwdPlan bwd_plan(const void* dy, int64_t lddy, const void* x, int64_t ldx, const
 extern "C" size_t tt_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
                                                     int64_t ldw, int64_t M, int N, int K, int dtype, int act) {
   if (!known_dtype(dtype) || !shape_ok(M, N, K)) return 0;
-  return bwd_plan(dy, lddy, x, ldx, w, ldw, M, N, K, dtype, act, true).total;
+  return bwd_plan(dy, lddy, x, ldx, w, ldw, M, N, K, dtype, act, w != nullptr, x != nullptr).total;
 }
 
 extern "C" int tt_linear_act_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
@@ -623,7 +623,7 @@ extern "C" int tt_linear_act_bwd(const void* dy, int64_t lddy, const void* x, in
   TT_REQUIRE(workspace, TT_ERR_NULL_POINTER);
   TT_REQUIRE(M == 0 || (dy && (!dx || w) && (!dw || x) && (act == TT_ACT_NONE || preact)), TT_ERR_NULL_POINTER);
   TT_REQUIRE(tt_aligned16(workspace), TT_ERR_ALIGNMENT);
-  const BwdPlan p = bwd_plan(dy, lddy, x, ldx, w, ldw, M, N, K, dtype, act, true);
+  const BwdPlan p = bwd_plan(dy, lddy, x, ldx, w, ldw, M, N, K, dtype, act, dx != nullptr, dw != nullptr);
   TT_REQUIRE(workspace_bytes >= p.total, TT_ERR_WORKSPACE);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int width = dtype_bytes(dtype);

@@ -539,8 +539,8 @@ def linear_act_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact: O
     db = torch.empty(N, dtype=x.dtype, device=x.device) if bias else None
     if dx is not None or dw is not None or db is not None:
         with _enter(x.device):
-            nbytes = _lib.load().tt_linear_act_bwd_workspace_bytes(dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K,
-                                                                   dt, act)
+            nbytes = _lib.load().tt_linear_act_bwd_workspace_bytes(dy.data_ptr(), lddy, x.data_ptr() if need_dw else None, ldx,
+                                                                   w.data_ptr() if need_dx else None, ldw, M, N, K, dt, act)
             ws = _workspace(nbytes, x.device)
             call("tt_linear_act_bwd", dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(preact) if act else None,
                  _ptr(dx), _ptr(dw), _ptr(db), M, N, K, dt, act, ws.data_ptr(), nbytes, _stream_on(x.device))
