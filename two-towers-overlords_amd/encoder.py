@@ -122,13 +122,20 @@ class PackedBertEncoder:
         cfg = getattr(model, "config", None)
         try:
             emb, layers = model.embeddings, list(model.encoder.layer)
-            for part in (emb.word_embeddings, emb.position_embeddings, emb.token_type_embeddings, emb.LayerNorm):
-                part.weight  # noqa: B018
+            embeddings = [emb.word_embeddings, emb.position_embeddings, emb.token_type_embeddings]
+            denses, norms = [], [emb.LayerNorm]
             for l in layers:
-                l.attention.self.query, l.attention.self.key, l.attention.self.value, l.attention.output.dense  # noqa: B018
-                l.attention.output.LayerNorm, l.intermediate.dense, l.output.dense, l.output.LayerNorm  # noqa: B018
+                at = l.attention
+                denses += [at.self.query, at.self.key, at.self.value, at.output.dense, l.intermediate.dense, l.output.dense]
+                norms += [at.output.LayerNorm, l.output.LayerNorm]
         except AttributeError as e:
             raise ValueError(f"encoder_impl='hip' runs BERT-shaped encoders only ({e})") from None
+        # other families carry the same names and compute something else (RoBERTa counts positions from the padding id, ...)
+        if getattr(cfg, "model_type", None) != "bert":
+            raise ValueError(f"encoder_impl='hip' runs BERT-shaped encoders only (model_type {getattr(cfg, 'model_type', None)!r})")
+        for part, kind in [*((p, nn.Embedding) for p in embeddings), *((p, nn.Linear) for p in denses), *((p, nn.LayerNorm) for p in norms)]:
+            if getattr(type(part), "forward", None) is not kind.forward:  # an adapter or a quantised layer: its weight is not all of it
+                raise ValueError(f"encoder_impl='hip' reads the weights of plain layers: {type(part).__name__} is not an nn.{kind.__name__}")
         act = getattr(cfg, "hidden_act", None)
         if act not in ACTIVATIONS:
             raise ValueError(f"encoder_impl='hip': hidden_act {act!r} is not one of {', '.join(ACTIVATIONS)}")
