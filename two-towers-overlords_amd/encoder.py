@@ -56,37 +56,40 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, residual: O
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens, kw):
-        out, lse = ops.packed_attention(q, k, v, cu_seqlens, **kw)
+    def forward(ctx, q, k, v, cu_seqlens, prefix, slopes, key_mask, kw):
+        masks = dict(prefix=prefix, slopes=slopes, key_mask=key_mask)
+        out, lse = ops.packed_attention(q, k, v, cu_seqlens, **masks, **kw)
         ctx.kw = kw
-        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens, prefix, slopes, key_mask)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, cu = ctx.saved_tensors
-        return (*ops.packed_attention_bwd(dout.contiguous(), q, k, v, out, lse, cu, **ctx.kw), None, None)
+        q, k, v, out, lse, cu, prefix, slopes, key_mask = ctx.saved_tensors
+        grads = ops.packed_attention_bwd(dout.contiguous(), q, k, v, out, lse, cu, prefix=prefix, slopes=slopes, key_mask=key_mask, **ctx.kw)
+        return (*grads, None, None, None, None, None)
 
 
 class _QkvAttentionFn(torch.autograd.Function):
     """q, k, v are column blocks of one projection's output, and so are their gradients: no concatenation."""
 
     @staticmethod
-    def forward(ctx, qkv, heads, cu_seqlens, kw):
+    def forward(ctx, qkv, heads, cu_seqlens, prefix, slopes, key_mask, kw):
         q, k, v = _blocks(qkv, heads)
-        out, lse = ops.packed_attention(q, k, v, cu_seqlens, **kw)
+        out, lse = ops.packed_attention(q, k, v, cu_seqlens, prefix=prefix, slopes=slopes, key_mask=key_mask, **kw)
         ctx.heads, ctx.kw = heads, kw
-        ctx.save_for_backward(qkv, out, lse, cu_seqlens)
+        ctx.save_for_backward(qkv, out, lse, cu_seqlens, prefix, slopes, key_mask)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, out, lse, cu = ctx.saved_tensors
+        qkv, out, lse, cu, prefix, slopes, key_mask = ctx.saved_tensors
         grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        ops.packed_attention_bwd(dout.contiguous(), *_blocks(qkv, ctx.heads), out, lse, cu, **ctx.kw, grads=_blocks(grad, ctx.heads))
-        return grad, None, None, None
+        ops.packed_attention_bwd(dout.contiguous(), *_blocks(qkv, ctx.heads), out, lse, cu, prefix=prefix, slopes=slopes, key_mask=key_mask,
+                                 **ctx.kw, grads=_blocks(grad, ctx.heads))
+        return grad, None, None, None, None, None, None
 
 
 def _blocks(qkv: Tensor, heads: int) -> Tuple[Tensor, Tensor, Tensor]:
@@ -98,7 +101,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, *, scale: Opt
               prefix: Optional[Tensor] = None, softcap: float = 0.0, slopes: Optional[Tensor] = None,
               key_mask: Optional[Tensor] = None) -> Tensor:
     """`ops.packed_attention`, differentiable in q, k and v -> out [T, H, Dh]."""
-    return _AttentionFn.apply(q, k, v, cu_seqlens, dict(scale=scale, causal=causal, prefix=prefix, softcap=softcap, slopes=slopes, key_mask=key_mask))
+    return _AttentionFn.apply(q, k, v, cu_seqlens, prefix, slopes, key_mask, dict(scale=scale, causal=causal, softcap=softcap))
 
 
 def attention_qkv(qkv: Tensor, heads: int, cu_seqlens: Tensor, *, scale: Optional[float] = None, causal: bool = False,
@@ -107,7 +110,7 @@ def attention_qkv(qkv: Tensor, heads: int, cu_seqlens: Tensor, *, scale: Optiona
     """`attention` on one projection's output [T, heads + 2 kv_heads, Dh] (query heads first, then keys, then values)."""
     if qkv.dim() != 3 or qkv.shape[1] <= heads or (qkv.shape[1] - heads) % 2:
         raise ValueError(f"qkv: expected [tokens, heads + 2 kv_heads, head_dim] with {heads} query heads, got {tuple(qkv.shape)}")
-    return _QkvAttentionFn.apply(qkv, heads, cu_seqlens, dict(scale=scale, causal=causal, prefix=prefix, softcap=softcap, slopes=slopes, key_mask=key_mask))
+    return _QkvAttentionFn.apply(qkv, heads, cu_seqlens, prefix, slopes, key_mask, dict(scale=scale, causal=causal, softcap=softcap))
 
 
 class PackedBertEncoder:
