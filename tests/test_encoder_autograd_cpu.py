@@ -68,3 +68,13 @@ def test_a_mask_changed_before_the_backward_pass_is_noticed(attention_calls, nam
         (cu if name == "cu" else given[name]).zero_()
         with pytest.raises(RuntimeError, match="inplace"):
             out.sum().backward()
+
+
+def test_slopes_that_want_a_gradient_are_refused(attention_calls):
+    q, k, v = (torch.randn(6, 2, 8, requires_grad=True) for _ in range(3))
+    slopes = torch.rand(2, requires_grad=True)
+    for run, _ in both(q, k, v, torch.tensor([0, 6], dtype=torch.int32), slopes=slopes):
+        with pytest.raises(ValueError, match="no gradient"):
+            run()
+        with torch.no_grad():
+            run()

@@ -97,10 +97,17 @@ def _blocks(qkv: Tensor, heads: int) -> Tuple[Tensor, Tensor, Tensor]:
     return qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
 
 
+def _refuse_bias_gradient(slopes: Optional[Tensor]) -> None:
+    # here: inside an autograd function's forward no gradient is recorded, and ops.packed_attention's own check sees none asked for
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise ValueError("slopes: the distance bias has no gradient")
+
+
 def attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, *, scale: Optional[float] = None, causal: bool = False,
               prefix: Optional[Tensor] = None, softcap: float = 0.0, slopes: Optional[Tensor] = None,
               key_mask: Optional[Tensor] = None) -> Tensor:
     """`ops.packed_attention`, differentiable in q, k and v -> out [T, H, Dh]."""
+    _refuse_bias_gradient(slopes)
     return _AttentionFn.apply(q, k, v, cu_seqlens, prefix, slopes, key_mask, dict(scale=scale, causal=causal, softcap=softcap))
 
 
@@ -110,6 +117,7 @@ def attention_qkv(qkv: Tensor, heads: int, cu_seqlens: Tensor, *, scale: Optiona
     """`attention` on one projection's output [T, heads + 2 kv_heads, Dh] (query heads first, then keys, then values)."""
     if qkv.dim() != 3 or qkv.shape[1] <= heads or (qkv.shape[1] - heads) % 2:
         raise ValueError(f"qkv: expected [tokens, heads + 2 kv_heads, head_dim] with {heads} query heads, got {tuple(qkv.shape)}")
+    _refuse_bias_gradient(slopes)
     return _QkvAttentionFn.apply(qkv, heads, cu_seqlens, prefix, slopes, key_mask, dict(scale=scale, causal=causal, softcap=softcap))
 
 
