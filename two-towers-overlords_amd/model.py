@@ -406,7 +406,8 @@ class InBatchSoftmaxLoss(nn.Module):
         if anchor.shape != documents.shape:
             raise ValueError(f"anchor {tuple(anchor.shape)} and documents {tuple(documents.shape)}: document i belongs to query i")
         B = anchor.shape[0]
-        q, d = F.normalize(anchor, dim=1, eps=1e-8), F.normalize(documents, dim=1, eps=1e-8)
+        # norms in float32: fp16 has no 1e-8, a zero row would be 0 / 0
+        q, d = (F.normalize(t.float(), dim=1, eps=1e-8).to(t.dtype).contiguous() for t in (anchor, documents))
         qid = None if query_ids is None else query_ids.to(torch.int64).contiguous()
         target = torch.arange(B, device=anchor.device)
         if B == 0:
