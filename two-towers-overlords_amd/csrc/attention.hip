@@ -259,7 +259,7 @@ __device__ __forceinline__ Units units(const Args& a, int head) {
   return u;
 }
 // cap tanh(s scale / cap).  16-bit operands: where no score of the tile is beyond 0.35 cap, the series to x^9 (the next term is
-// below 10^-7); else 1 - 2 / (1 + exp 2x), good to 2^-22 absolute and +-1 far out.  float: the accurate function.
+// below 10^-7; not where the cap is so small that the factors of its powers leave fp32: 0 times them would be NaN); else 1 - 2 / (1 + exp 2x), good to 2^-22 absolute and +-1 far out.  float: the accurate function.
 template <class T>
 __device__ __forceinline__ f32x16 capped(f32x16 s, const Args& a) {
   if (!(a.cap > 0.f)) return s;
@@ -272,7 +272,7 @@ __device__ __forceinline__ f32x16 capped(f32x16 s, const Args& a) {
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(s[i]));
-  if (!__any(top * r > 0.35f)) {
+  if (r < 4096.f && !__any(top * r > 0.35f)) {
     const float r2 = r * r, k9 = 62.f / 2835.f * r2 * r2 * r2 * r2 * a.scale, k7 = -17.f / 315.f * r2 * r2 * r2 * a.scale,
                 k5 = 2.f / 15.f * r2 * r2 * a.scale, k3 = -1.f / 3.f * r2 * a.scale;
 #pragma unroll
