@@ -729,6 +729,7 @@ typedef struct {
  *   start).  A query that sees no key gets o = 0, lse = -inf and no gradient.
  *   Document b holds tokens [cu_seqlens[b], cu_seqlens[b + 1]); cu_seqlens[0] = 0, ascending, at most T; documents may be
  *   empty.  Tokens behind the last document get o = 0 and zero gradients.  What masked keys hold (NaN included) does not matter.
+ *   scale: 1e-15..1e15; softcap: 0 (none) or 1e-15..1e15.
  *   heads % kv_heads == 0: query head h reads key head h / (heads / kv_heads).  head_dim: a multiple of 8, 8..128.
  *   lse [heads, T] fp32: natural logarithm of the softmax's denominator (output of the forward, input of the backward call).
  *   delta [heads, T] fp32: scratch of the backward call.  Null: slopes, key_mask, prefix where not used.
@@ -755,7 +756,7 @@ int tt_packed_attention_bwd(const tt_attention_args* args /* host */, tt_stream_
  *   lse[i] = log sum_j exp l_ij,   loss[i] = lse[i] - l_i,target[i]      (fp32)
  *   target [N] int64; a row whose target is ignore_index has loss 0 and no gradient, one whose target is otherwise outside
  *   [0, V) has loss NaN (and poisons the gradients).  row_ids [N] / cand_ids [V] (both or neither): candidates j != target
- *   with cand_ids[j] == row_ids[i] are left out of row i's sum (a row without a target keeps candidate 0).
+ *   with cand_ids[j] == row_ids[i] are left out of row i's sum (a row without a target keeps candidate 0).  scale: 1e-15..1e15.
  * tt_softmax_loss_bwd: row_coef [N] = d objective / d loss[i];  dx [N,D], dw [V,D] contiguous, of `dtype`, either may be null.
  *   Its workspace covers both (the logits' gradients, which either needs, are the larger part).
  */

@@ -880,7 +880,8 @@ int check(const tt_attention_args* p) {
   TT_REQUIRE(p->T >= 0 && p->T <= 1LL << 30 && p->docs >= 1 && p->heads >= 1 && p->kv_heads >= 1 &&
                  p->heads % p->kv_heads == 0 && p->head_dim >= 8 && p->head_dim <= 128 && p->head_dim % 8 == 0,
              TT_ERR_BAD_SHAPE);
-  TT_REQUIRE(p->scale > 0.f && p->softcap >= 0.f, TT_ERR_BAD_SHAPE);
+  // (within these bounds quotients and products of scale, cap and a score stay in fp32's range)
+  TT_REQUIRE(tt_scale_ok(p->scale) && (p->softcap == 0.f || tt_scale_ok(p->softcap)), TT_ERR_BAD_SHAPE);
   TT_REQUIRE(!(p->causal && p->prefix), TT_ERR_UNSUPPORTED);
   return TT_OK;
 }

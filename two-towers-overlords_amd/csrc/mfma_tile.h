@@ -409,6 +409,8 @@ struct Chunk {
 // ---- host side ----------------------------------------------------------------------------------------------
 inline long long pad_to(long long n, int m) { return (n + m - 1) / m * m; }
 inline int dtype_bytes(int dtype) { return dtype == TT_F32 ? 4 : 2; }
+// scales and caps of scores that are taken (false for NaN)
+inline bool tt_scale_ok(float s) { return s >= 1e-15f && s <= 1e15f; }
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Can a [rows, cols] matrix of row stride ld be read in 16-byte chunks as it is?

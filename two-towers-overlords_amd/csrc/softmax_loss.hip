@@ -358,7 +358,7 @@ Plan plan(const void* x, long long ldx, const void* w, long long ldw, long long 
 int check(int64_t ldx, int64_t ldw, int64_t N, int V, int D, int dtype, float scale) {
   TT_REQUIRE(dtype == TT_F32 || dtype == TT_BF16 || dtype == TT_F16, TT_ERR_BAD_DTYPE);
   // 2^28 candidates: two rows of float G are within a tile's 32-bit offsets; 2^22 features: 256 packed rows are
-  TT_REQUIRE(N >= 0 && N <= 1LL << 30 && V >= 1 && V <= 1 << 28 && D >= 1 && D <= 1 << 22 && ldx >= D && ldw >= D && scale > 0.f,
+  TT_REQUIRE(N >= 0 && N <= 1LL << 30 && V >= 1 && V <= 1 << 28 && D >= 1 && D <= 1 << 22 && ldx >= D && ldw >= D && tt_scale_ok(scale),
              TT_ERR_BAD_SHAPE);
   return TT_OK;
 }

@@ -478,6 +478,11 @@ def _activation(name: str) -> int:
     return _lib.ACTIVATIONS[name]
 
 
+def _scale_ok(scale: float) -> bool:
+    """Within these bounds what is formed of a scale, a cap and a score stays in float32's range."""
+    return 1e-15 <= float(scale) <= 1e15
+
+
 def _workspace(nbytes: int, device) -> torch.Tensor:
     # from the caching allocator on every call: a buffer kept between calls would be shared by captured graphs and streams
     return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
@@ -614,8 +619,8 @@ def _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes,
         if key_mask.shape[0] != T or key_mask.device != q.device:
             raise ValueError(f"key_mask: expected shape {(T,)} on {q.device}")
     scale = Dh ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf") or not 0.0 <= softcap < float("inf"):
-        raise ValueError(f"packed_attention: scale must be positive and softcap >= 0, got {scale}, {softcap}")
+    if not _scale_ok(scale) or not (softcap == 0.0 or _scale_ok(softcap)):
+        raise ValueError(f"packed_attention: scale must be in 1e-15..1e15 and softcap 0 or in 1e-15..1e15, got {scale}, {softcap}")
     return dt, [vq, vk, vv], (scale, causal, prefix, softcap, slopes, key_mask), T, docs, H, Hkv, Dh
 
 
@@ -681,8 +686,8 @@ def _softmax_args(x, w, target, scale, row_ids, cand_ids):
         _req(t, name, torch.int64, 1)
         if t.shape[0] != n or t.device != x.device:
             raise ValueError(f"{name}: expected shape {(n,)} on {x.device}")
-    if not 0.0 < float(scale) < float("inf"):
-        raise ValueError(f"softmax_loss: scale must be positive, got {scale}")
+    if not _scale_ok(scale):
+        raise ValueError(f"softmax_loss: scale must be in 1e-15..1e15, got {scale}")
     return dt, ldx, ldw, N, V, D
 
 
