@@ -269,10 +269,10 @@ __device__ __forceinline__ f32x16 capped(f32x16 s, const Args& a) {
     for (int i = 0; i < 16; ++i) s[i] = a.cap * tanhf(s[i] * r);
     return s;
   }
-  float top = 0.f;
+  float top = 0.35f / 4096.f;  // no series from r = 4096 on.  (As a condition of its own it moved scores to scratch memory)
 #pragma unroll
   for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(s[i]));
-  if (r < 4096.f && !__any(top * r > 0.35f)) {
+  if (!__any(top * r > 0.35f)) {
     const float r2 = r * r, k9 = 62.f / 2835.f * r2 * r2 * r2 * r2 * a.scale, k7 = -17.f / 315.f * r2 * r2 * r2 * a.scale,
                 k5 = 2.f / 15.f * r2 * r2 * a.scale, k3 = -1.f / 3.f * r2 * a.scale;
 #pragma unroll
