@@ -728,7 +728,8 @@ typedef struct {
  *   zero, and with causal only j <= i, with prefix only j <= i or j < prefix[document] (positions count from the document's
  *   start).  A query that sees no key gets o = 0, lse = -inf and no gradient.
  *   Document b holds tokens [cu_seqlens[b], cu_seqlens[b + 1]); cu_seqlens[0] = 0, ascending, at most T; documents may be
- *   empty.  Tokens behind the last document get o = 0 and zero gradients.  What masked keys hold (NaN included) does not matter.
+ *   empty.  Tokens behind the last document get o = 0 and zero gradients.  What the keys that key_mask takes out
+ *   hold (NaN included) does not matter.
  *   scale: 1e-15..1e15; softcap: 0 (none) or 1e-15..1e15.
  *   heads % kv_heads == 0: query head h reads key head h / (heads / kv_heads).  head_dim: a multiple of 8, 8..128.
  *   lse [heads, T] fp32: natural logarithm of the softmax's denominator (output of the forward, input of the backward call).

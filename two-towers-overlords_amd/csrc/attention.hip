@@ -350,10 +350,13 @@ __device__ __forceinline__ int key_end(const Args& a, int prefix, int i1, int le
 // ------------------------------------------------------------------------------------------------ forward
 // K and V tiles stream into one pair of LDS images while the other is in use: one barrier a tile.  A row's sum and output are
 // rescaled only when its maximum has grown by 2^8 (the probabilities stay below 2^8, fp32 sums do not mind).
-// Bound by vector arithmetic at heads of 32 and 64 (two matrix instructions of 32 x 32 x 16 per 32 keys and 16 exponentials, masks
-// and conversions per lane beside them), by bytes for short documents.  512 documents of 12-128 tokens, 12 heads of 32, float: 97
-// us (floor 45 by bytes); 5 of 1001-4096, heads of 64, bf16, prefix, cap and bias: 173 us, about 90 % of its cycles vector
-// instructions; 16 of 700-2048, 16 heads of 128 on 4, causal, fp16: 239 us, 575 TFLOP/s.
+// P is rounded to the type for P V (a matrix instruction takes no wider operand beside V): bf16 o is 1.9e-3 of its size from exact,
+// its own rounding 1.7e-3.
+// Bound by vector arithmetic where there are a cap and a bias (5 documents of 1001-4096 tokens, heads of 64, bf16, prefix and key
+// mask: 198 us, vector instructions in all of a busy compute unit's cycles), by it and by waits at heads of 32 (256 of 8-512, bf16,
+// bias: 133 us, vector 76 %, 47 % of the waves' time waiting) and 128 (16 of 700-2048, 16 heads on 4, causal, fp16: 215 us, 640
+// TFLOP/s, vector 37 %, matrix 31 %), by bytes and half-filled workgroups for short documents (512 of 12-128, 12 heads of 32, float:
+// 97 us, floor 45 by bytes).
 template <class T, int DP, int WAVES, bool PLAIN>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 4 : DP == 64 ? 3 : 2))) void attention_fwd_kernel(Args a) {
   using D = Dim<T, DP>;
@@ -502,7 +505,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 // 16 heads of 128: both passes 1140 -> 1176 us, 1.5 -> 1.2).  Where one tile holds all keys, delta is formed from P and dP before
 // dS: with a few keys dS is a small difference, and o's rounding in dO.o was 2 to 3 roundings of dq.
 // 10 operations per pair and head element against the forward's 4, 16 exponentials per lane and 32 keys as there: bound by vector
-// arithmetic at heads of 32, by the matrix units at 128 (16 documents of 700-2048, fp16, causal: 344 us, 600 TFLOP/s).
+// arithmetic at heads of 32 (209 us, 76 % of a busy compute unit's cycles); at 128 matrix (44 %) and vector instructions (39 %) take
+// turns with waits (16 documents of 700-2048, fp16, causal: 333 us, 620 TFLOP/s).
 template <class T, int DP, int WAVES, bool PLAIN>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 3 : DP == 64 || sizeof(T) == 2 ? 2 : 1))) void attention_dq_kernel(Args a) {
   using D = Dim<T, DP>;
@@ -673,10 +677,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP =
 // ------------------------------------------------------------------------------------------------ dk, dv
 // A wave owns 32 keys (columns) and walks the queries, for every query head that shares the key head:
 // dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i
-// 8 operations per pair and head element.  256 documents of 8-512 tokens, 12 heads of 32, bf16: 272 us, vector arithmetic as in dq
-// (the statistics are per accumulator row here: 16 reads of lse and delta).  16 of 700-2048, 16 heads of 128 on 4, fp16: 670 us,
-// 410 TFLOP/s: two accumulators of the head's width and two operands take 392 registers, one wave per SIMD, so waits show;
-// dk and dv in kernels of their own (two waves) recompute S and took 312 + 421 us.
+// P and dS are rounded to the type once, where dq takes dS in two parts (that would be half as many products again): dk and dv are 2.4e-3
+// (bf16) and 3.0e-4 (fp16) of their size from exact, their own rounding is 1.7e-3 and 2.1e-4 of it.
+// 8 operations per pair and head element.  256 documents of 8-512 tokens, 12 heads of 32, bf16: 260 us; waits bound it (46 % of the
+// waves' time at two waves per SIMD; vector instructions fill 43 % of a busy compute unit's cycles, the statistics, here per
+// accumulator row, are 16 reads of lse and delta).  16 of 700-2048, 16 heads of 128 on 4, fp16: 627 us, 440 TFLOP/s: two accumulators
+// of the head's width and two operands take 392 registers, one wave per SIMD (vector 22 %, matrix 29 %).
 template <class T, int DP, int WAVES, bool PLAIN>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP == 32 || (DP == 64 && sizeof(T) == 2) ? 2 : 1))) void attention_dkv_kernel(Args a) {
   using D = Dim<T, DP>;

@@ -1,11 +1,15 @@
 // linear_act — y = act(x W^T + b) + r with one epilogue, and its gradients.
 //
 //   forward   z = x W^T + b (fp32), y = act(z) + r rounded once; z is kept (rounded to the type) for the backward pass
-//   backward  dz = dy act'(z), db = column sums of dz       one pass over dy and z
+//   backward  dz = dy act'(z), db = column sums of dz       one pass over dy and z (db before dz is rounded)
 //             dx = dz W                                     K-strided W, transposed on its way into LDS
 //             dW = dz^T x                                   both operands K-strided, contraction over the rows split
 //
 // 2 M N K operations each product; bound by the matrix units from a few hundred rows on, by the epilogue's bytes at small K.
+//
+// 16-bit types round z where it is kept (in fp32 twice the bytes, written and read) and dz where
+// it becomes the products' operand (matrix instructions take no wider one beside 16 bits): the gradients of 16384 x 1024 -> 4096 in
+// bf16 are 2.4e-3 of their size from exact, their own rounding is 1.7e-3 of it.
 //
 // Replaces the nn.Linear (+ activation, + residual add) calls of the frozen encoder of backend/model.py:51-52.
 #include <type_traits>
@@ -165,8 +169,8 @@ __device__ __forceinline__ void epilogue(B& blk, const FwdArgs& a, char* __restr
       });
 }
 
-// float 35841 x 384 -> 1536 with gelu: 384 us, 110 TFLOP/s (the library's product alone reaches 133 on large ones).  bf16 16384 x 1024
-// -> 4096 with gelu, residual and kept z: 219 us, 128 of them the product at 1070 TFLOP/s, the rest the epilogue's 400 MB, which
+// float 35841 x 384 -> 1536 with gelu: 383 us, 110 TFLOP/s (the library's product alone reaches 133 on large ones).  bf16 16384 x 1024
+// -> 4096 with gelu, residual and kept z: 222 us, 128 of them the product at 1070 TFLOP/s, the rest the epilogue's 400 MB, which
 // nothing overlaps (two 128-wide workgroups per compute unit do, at a lower rate: equal; a persistent loop spilled: slower).
 // bf16 35841 x 1536 -> 384 with residual: 58 us, 843 tiles of 128 are 1.65 rounds; floor 33 by bytes.
 template <class T, class B>

@@ -53,8 +53,8 @@ __device__ __forceinline__ bool left_out(const Args& a, int j, long long t, long
 }
 
 // A lane holds 16 NI candidates of MJ rows: maximum and sum are in-lane, one exchange, then the waves' through LDS.  Six K-steps at 384
-// features against an epilogue of an exponential per logit, which nothing overlaps: bf16 8192 x 30522 258 us, 745 TFLOP/s; 203
-// rows x 250000 66 us, 192 MB of candidates at 2.9 TB/s (a tile is 256 rows, 203 in use).
+// features against an epilogue of an exponential per logit, which nothing overlaps: bf16 8192 x 30522 246 us, 780 TFLOP/s; 203
+// rows x 250000 62 us, 192 MB of candidates at 3.1 TB/s (a tile is 256 rows, 203 in use).
 template <class T, class B>
 __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void softmax_lse_kernel(Args a) {
   __shared__ __align__(16) char b0[B::BYTES];
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256) void softmax_join_kernel(const float2* __restr
 }
 
 // G of a piece of the candidates, [M, ldg] in T; columns behind the last candidate are zero.  The logits' product again, then 500 MB of
-// G at 8192 x 30522 bf16: 388 us (product and exponentials 258, the rest the stores, through LDS as whole rows).  Keeping the
+// G at 8192 x 30522 bf16: 375 us (product and exponentials 246, the rest the stores, through LDS as whole rows).  Keeping the
 // logits instead would write and read them once more and need N V elements.
 template <class T, class B>
 __global__ __launch_bounds__(B::THREADS) __attribute__((amdgpu_waves_per_eu(2))) void softmax_grad_kernel(Args a) {

@@ -633,7 +633,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     documents allowed; tokens behind the last document get 0).  scale: 1/sqrt(Dh) by default.  A query sees the keys of its own
     document whose `key_mask` is set; causal: only j <= i; prefix [documents] int32: only j <= i or j < prefix.  softcap > 0: the
     scores become softcap * tanh(score / softcap); slopes [H] float32: slopes[h] * |i - j| is subtracted.  A query that sees
-    nothing gets 0 (lse -inf).  What masked keys hold does not matter, NaN included.
+    nothing gets 0 (lse -inf).  What the keys that key_mask takes out hold does not matter, NaN included.
     The attention of the frozen encoder (backend/model.py:51-52) without its padding."""
     dt, views, mask, T, docs, H, Hkv, Dh = _attention_args(q, k, v, cu_seqlens, scale, causal, prefix, softcap, slopes, key_mask)
     out = torch.empty((T, H, Dh), dtype=q.dtype, device=q.device)
