@@ -26,7 +26,7 @@ constexpr float kGeluC = 0.79788456080286536f, kGeluA = 0.044715f;
 // t = 1 / (1 + p a), a = |z| / sqrt 2, no cancellation on the negative side, where gelu's values are small: Q's error has to be
 // small relative to erfc, not only absolutely.  Q is a Chebyshev fit to exp(a^2) erfc(a) / t on 0 <= a <= 10.  16-bit results: p =
 // 0.48, degree 6, absolute error of Phi 1.5e-7, relative 2e-5 down to the smallest normal float (z = -13), of which the rounding of
-// exp's argument is half; a 256th of bf16's rounding, a 24th of fp16's.  float: p = 0.5, degree 8 (relative error 4e-8).  erff cost
+// exp's argument is half; a 200th of bf16's rounding, a 24th of fp16's.  float: p = 0.5, degree 8 (relative error 4e-8).  erff cost
 // a quarter of the float epilogue's time.
 template <bool FAST>
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
